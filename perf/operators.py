@@ -129,7 +129,7 @@ def prepare(case, seed):
             from fms_b200.kernels import ops
 
             state["own_x"] = ops.QuantizedRows.of(state["x"], state["x_scale"])
-            state["own_w"] = ops.QuantizedRows.of(state["w"], state["w_scale"])
+            state["own_w"] = ops.e4m3_weight(state["w"], state["w_scale"])
         return state
     groups = -(-dim // (case["group"] or dim))
     state["x"] = _activations(g, rows, dim).to(torch.bfloat16)
