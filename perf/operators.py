@@ -104,9 +104,9 @@ def _activations(g, rows, dim):
 
 
 def _to_e4m3(x):
-    scale = x.abs().amax(1) / LARGEST
-    q = (x / scale[:, None]).clamp_(-LARGEST, LARGEST)
-    return torch.where(scale[:, None] > 0, q, 0.0 * x).to(torch.float8_e4m3fn), scale
+    most = x.abs().amax(1)
+    q = (x * LARGEST / most[:, None]).clamp_(-LARGEST, LARGEST)
+    return torch.where(most[:, None] > 0, q, 0.0 * x).to(torch.float8_e4m3fn), most / LARGEST
 
 
 def prepare(case, seed):
@@ -186,10 +186,10 @@ def _weights(state):
 # ---- from the definitions, in 64 bits ----------------------------------------------------------------------------------
 def _e4m3_exactly(y):
     """Scales and the nearest e4m3 values of rows in 64 bits; ties go to the value whose last bit is 0, as ``round`` does."""
-    scales = y.abs().max(dim=1).values / 448
-    v = y / scales.unsqueeze(1)
+    largest = y.abs().max(dim=1).values
+    v = 448 * y / largest.unsqueeze(1)
     step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)  # 8 values from a power of two to the next
-    return (torch.round(v / step) * step).clamp(-448, 448), scales
+    return (torch.round(v / step) * step).clamp(-448, 448), largest / 448
 
 
 def exact(case, seed):
