@@ -1,0 +1,544 @@
+// y[m, n] = sx[m] * sw[n] * sum_k qx[m, k] * qw[n, k] (+ bias[n]): rows and weights of 8 bits (e4m3) with one float32 scale a
+// row of either, on the tcgen05 tensor cores of sm_100a (kind::f8f6f4: twice the rate of 16-bit operands, half the bytes).
+// The products of two e4m3 values and their sums are float32 in tensor memory; the scales come in once, in the epilogue, so
+// that nothing is rounded but the result.  GLU: y = act(gate) * up for weights [gate; up] (fms/modules/feedforward.py:288-297).
+//
+// Both kernels bring operands in by TMA in boxes of 128 k (128 bytes, 128-byte swizzle) and issue 4 instructions of 32 k on a
+// box.  Rows lie `pitch` bytes apart, a multiple of 16, with zeros behind the last value; what lies beyond M, N and the
+// pitch is zeros on the way in (TMA) and is not stored on the way out.  Every wait on an mbarrier is bounded: on a time-out the
+// block records error 4, skips the rest of its work and still frees its tensor memory.
+#include <cuda.h>
+
+#include "common.cuh"
+
+namespace {
+constexpr int TILE = 128, TILE_K = 128, UMMA_K = 32, MAX_STAGES = 12, MAX_KS = 8;
+constexpr int THREADS = 192;
+constexpr int BOX_BYTES = TILE * TILE_K;  // 128 rows of an operand for one step
+
+#include "tcgen05.cuh"
+
+// instruction descriptor of kind::f8f6f4: float32 accumulator, e4m3 a and b, both K-major; the shape M x N
+__host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+__device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+  const uint32_t acc = accumulate ? 1u : 0u, zero = 0u;
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(zero)
+      : "memory");
+}
+// 256 x N x 32 over a pair of blocks: A 128 rows from each block's shared memory, B N/2 rows from each
+__device__ __forceinline__ void umma_e4m3_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+  const uint32_t acc = accumulate ? 1u : 0u, zero = 0u;
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n}\n" ::"r"(tmem_d),
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(zero)
+      : "memory");
+}
+
+// by a whole warp, which gives up as one
+__device__ __forceinline__ bool warp_wait(void* bar, uint32_t parity, volatile int* failed) {
+  return __all_sync(0xffffffffu, wait_or_abort(bar, parity, failed));
+}
+
+__device__ __forceinline__ float activate(float g, int act) {
+  switch (act) {
+    case 0: return g / (1.f + expf(-g));
+    case 1: return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+    case 2: return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g)));
+    default: return fmaxf(g, 0.f);
+  }
+}
+
+struct Epilogue {
+  void* out;                  // [M, outputs] bfloat16 or float32 (GLU: bfloat16)
+  const __nv_bfloat16* bias;  // [N] or null
+  const float *sx, *sw;       // [M], [N]
+  int out_f32, glu, act;
+  int outputs;                // columns of y: N, or the hidden values of GLU (half of N)
+  int tile_n, stages, ks, n_tokens;
+};
+
+__device__ __forceinline__ float scaled(float acc, float s, const __nv_bfloat16* bias, int col) {
+  return fmaf(acc, s, bias ? __bfloat162float(bias[col]) : 0.f);
+}
+__device__ __forceinline__ void store16(const Epilogue& ep, const float* v, int row, int col0, int M) {
+  if (!FMS_IN((size_t)row * ep.outputs + col0, (size_t)M * ep.outputs)) return;
+  if (ep.out_f32) {
+    float* o = (float*)ep.out + (size_t)row * ep.outputs + col0;
+    if (col0 + 16 <= ep.outputs && ep.outputs % 4 == 0) {
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (col0 + j < ep.outputs) o[j] = v[j];
+    }
+    return;
+  }
+  __nv_bfloat16* o = (__nv_bfloat16*)ep.out + (size_t)row * ep.outputs + col0;
+  if (col0 + 16 <= ep.outputs && ep.outputs % 8 == 0) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 8) {
+      uint32_t pk[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        __nv_bfloat162 t = __floats2bfloat162_rn(v[j + 2 * p], v[j + 2 * p + 1]);
+        pk[p] = *reinterpret_cast<uint32_t*>(&t);
+      }
+      *reinterpret_cast<uint4*>(o + j) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (col0 + j < ep.outputs) o[j] = __float2bfloat16_rn(v[j]);
+  }
+}
+
+// ---- many rows (prefill) --------------------------------------------------------------------------------------------
+// Persistent pairs of thread blocks (a cluster of two, cta_group::2): a pair owns a tile of 256 rows of x by TN rows of w, of
+// which each block brings 128 rows of x and half the rows of w (GLU: block 0 the gate rows, block 1 the up rows) into its own
+// shared memory.  What a multiprocessor takes in, 128 + TN / 2 bytes a k, against 2 * 128 * TN operations is what limits
+// tiles without a pair.  Two accumulators: the epilogue of a tile runs under the products of the next.
+//   warp 0 TMA, warp 1 (of block 0) the instructions, warps 2-5 the epilogue, 32 rows of this block's 128 each
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    e4m3_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, Epilogue ep, int M,
+                     int k_steps, int* __restrict__ error_flag) {
+  extern __shared__ unsigned char smem_unaligned[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
+  const int b_rows = ep.tile_n / 2, stage_bytes = BOX_BYTES + b_rows * TILE_K, stages = ep.stages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)stages * stage_bytes);
+  uint64_t* empty = full + MAX_STAGES;
+  uint64_t* acc_full = empty + MAX_STAGES;  // [2]
+  uint64_t* acc_empty = acc_full + 2;       // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  __shared__ int failed_flag;
+  volatile int* failed = &failed_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int tile_n = ep.glu ? ep.tile_n / 2 : ep.tile_n;  // output columns of a tile
+  const int tiles_m = (M + 2 * TILE - 1) / (2 * TILE), n_tiles = tiles_m * ((ep.outputs + tile_n - 1) / tile_n);
+  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    failed_flag = 0;
+    for (int s = 0; s < MAX_STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 8);  // one arrival per epilogue warp of either block (used in block 0)
+    }
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the partner's barriers exist before anything is sent to them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();  // now: a block of the next kernel must not take the tensor memory that this one still needs
+  pdl_wait();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int it = 0;
+      for (int tile = pair; tile < n_tiles && !*failed; tile += pairs) {
+        const int m0 = (tile % tiles_m) * 2 * TILE + (int)rank * TILE, n0 = (tile / tiles_m) * tile_n;
+        const int w_row = ep.glu ? (leader ? n0 : ep.outputs + n0) : n0 + (int)rank * b_rows;
+        for (int i = 0; i < k_steps; ++i, ++it) {
+          const int s = it % stages;
+          if (!wait_or_abort(&empty[s], ((it / stages) & 1) ^ 1, failed)) break;
+          unsigned char* a = smem + (size_t)s * stage_bytes;
+          if (leader) mbar_arrive_expect_tx(&full[s], 2 * stage_bytes);  // the bytes of both blocks
+          tma_load_2d_pair(a, &map_x, i * TILE_K, m0, &full[s]);
+          tma_load_2d_pair(a + BOX_BYTES, &map_w, i * TILE_K, w_row, &full[s]);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (leader && elect_one()) {
+      const uint32_t idesc = idesc_e4m3(2 * TILE, ep.tile_n);
+      int it = 0, j = 0;
+      for (int tile = pair; tile < n_tiles && !*failed; tile += pairs, ++j) {
+        const int acc = j & 1;
+        if (!wait_or_abort(&acc_empty[acc], ((j >> 1) & 1) ^ 1, failed)) break;  // both epilogues have read this buffer
+        tc_fence_after();
+        for (int i = 0; i < k_steps; ++i, ++it) {
+          const int s = it % stages;
+          if (!wait_or_abort(&full[s], (it / stages) & 1, failed)) break;
+          tc_fence_after();
+          const uint32_t a = smem_u32(smem + (size_t)s * stage_bytes), b = a + BOX_BYTES;
+#pragma unroll
+          for (int kk = 0; kk < TILE_K / UMMA_K; ++kk)
+            umma_e4m3_pair(tmem + acc * 256, umma_desc(a + kk * UMMA_K), umma_desc(b + kk * UMMA_K), idesc, i > 0 || kk > 0);
+          tc_commit_pair(&empty[s]);
+        }
+        tc_commit_pair(&acc_full[acc]);
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    int j = 0;
+    for (int tile = pair; tile < n_tiles; tile += pairs, ++j) {
+      const int acc = j & 1;
+      const int row = (tile % tiles_m) * 2 * TILE + (int)rank * TILE + quarter * 32 + lane, n0 = (tile / tiles_m) * tile_n;
+      const float sx = row < M ? ep.sx[row] : 0.f;
+      if (!warp_wait(&acc_full[acc], (j >> 1) & 1, failed)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem + acc * 256 + ((uint32_t)(quarter * 32) << 16);
+      for (int c0 = 0; c0 < tile_n; c0 += 16) {  // every lane loads: tensor-memory loads are warp-wide
+        float v[16], u[16];
+        const int col0 = n0 + c0;
+        if (ep.glu) tmem_load_16(taddr + tile_n + c0, u);
+        tmem_load_16(taddr + c0, v);
+        if (row >= M || col0 >= ep.outputs) continue;
+#pragma unroll
+        for (int jj = 0; jj < 16; ++jj) {
+          const int col = min(col0 + jj, ep.outputs - 1);
+          v[jj] = scaled(v[jj], sx * ep.sw[col], ep.bias, col);
+          if (ep.glu) v[jj] = activate(v[jj], ep.act) * scaled(u[jj], sx * ep.sw[ep.outputs + col], ep.bias, ep.outputs + col);
+        }
+        store16(ep, v, row, col0, M);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (leader) mbar_arrive(&acc_empty[acc]);
+        else mbar_arrive_remote(&acc_empty[acc], 0);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_sync_all();  // nothing is sent to a block that has left
+  if (threadIdx.x == 0 && *failed && error_flag) atomicExch(error_flag, 4);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ---- up to 256 rows (decode) ---------------------------------------------------------------------------------------
+// The operands swapped: 128 rows of w fill the instruction's rows and the tokens are its columns (16 to 256), since a product
+// of this size is bound by reading w once.  A block owns 128 rows of w (GLU: 64 gate rows and the 64 up rows that belong to
+// them) for a slice of k; the ks blocks of a tile form a cluster and add their sums through distributed shared memory in the
+// order of their ranks.  ks depends on the weights' shape alone, so a row's result does not depend on the rest of the batch.
+// The first stages' boxes of w are asked for before griddepcontrol.wait: weights do not depend on the kernel before.
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t local_addr, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n.reg .b32 remote;\nmapa.shared::cluster.u32 remote, %4, %5;\nld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [remote];\n}\n"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(local_addr), "r"(rank)
+      : "memory");
+  return v;
+}
+
+__global__ void __launch_bounds__(THREADS) e4m3_rows_kernel(const __grid_constant__ CUtensorMap map_x,
+                                                            const __grid_constant__ CUtensorMap map_w, Epilogue ep, int M,
+                                                            int k_steps_all, int* __restrict__ error_flag) {
+  extern __shared__ unsigned char smem_unaligned[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
+  const int stage_bytes = BOX_BYTES + ep.n_tokens * TILE_K, stages = ep.stages, ks = ep.ks;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)stages * stage_bytes);
+  uint64_t* empty = full + MAX_STAGES;
+  uint64_t* acc_full = empty + MAX_STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  __shared__ int failed_flag;
+  volatile int* failed = &failed_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = ks > 1 ? (int)cluster_rank() : 0;
+  const int n0 = blockIdx.y * (ep.glu ? TILE / 2 : TILE);
+  const int per = (k_steps_all + ks - 1) / ks;
+  const int step_lo = min(rank * per, k_steps_all), k_steps = min(step_lo + per, k_steps_all) - step_lo;  // may be 0
+  uint32_t tmem_cols = 32;
+  while ((int)tmem_cols < ep.n_tokens) tmem_cols *= 2;
+
+  if (threadIdx.x == 0) {
+    failed_flag = 0;
+    for (int s = 0; s < MAX_STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, tmem_cols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();  // now: a block of the next kernel must not take the tensor memory that this one still needs
+
+  if (warp == 0) {
+    if (elect_one()) {
+      auto load_w = [&](int i) {
+        const int s = i % stages;
+        unsigned char* a = smem + (size_t)s * stage_bytes;
+        mbar_arrive_expect_tx(&full[s], stage_bytes);
+        tma_load_2d(a, &map_w, (step_lo + i) * TILE_K, n0, &full[s]);
+        if (ep.glu) tma_load_2d(a + BOX_BYTES / 2, &map_w, (step_lo + i) * TILE_K, ep.outputs + n0, &full[s]);
+      };
+      auto load_x = [&](int i) {
+        const int s = i % stages;
+        tma_load_2d(smem + (size_t)s * stage_bytes + BOX_BYTES, &map_x, (step_lo + i) * TILE_K, 0, &full[s]);
+      };
+      const int early = min(stages, k_steps);
+      for (int i = 0; i < early; ++i) load_w(i);
+      pdl_wait();  // x is what the kernel before wrote
+      for (int i = 0; i < early; ++i) load_x(i);
+      for (int i = early; i < k_steps && !*failed; ++i) {
+        if (!wait_or_abort(&empty[i % stages], ((i / stages) & 1) ^ 1, failed)) break;
+        load_w(i);
+        load_x(i);
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t idesc = idesc_e4m3(TILE, ep.n_tokens);
+      for (int i = 0; i < k_steps; ++i) {
+        const int s = i % stages;
+        if (!wait_or_abort(&full[s], (i / stages) & 1, failed)) break;
+        tc_fence_after();
+        const uint32_t a = smem_u32(smem + (size_t)s * stage_bytes), b = a + BOX_BYTES;
+#pragma unroll
+        for (int kk = 0; kk < TILE_K / UMMA_K; ++kk)
+          umma_e4m3(tmem, umma_desc(a + kk * UMMA_K), umma_desc(b + kk * UMMA_K), idesc, i > 0 || kk > 0);
+        tc_commit(&empty[s]);
+      }
+      tc_commit(acc_full);  // arrives when everything issued so far is done (at once if there was nothing)
+    }
+  }
+  // This block's sums as float32 [128][n_tokens + 4] in shared memory, over the stages: every copy into them has landed and
+  // every instruction that read them is done once the accumulator is ready.
+  float* red = reinterpret_cast<float*>(smem);
+  const int red_stride = ep.n_tokens + 4;
+  if (warp >= 2) {
+    pdl_wait();  // these warps read and write what other kernels touch (scales, the error flag, y)
+    const int quarter = warp & 3;
+    const bool ok = warp_wait(acc_full, 0, failed);
+    tc_fence_after();
+    const int row = quarter * 32 + lane;
+    for (int c0 = 0; c0 < ep.n_tokens; c0 += 16) {
+      float v[16];
+      if (ok && k_steps > 0) {
+        tmem_load_16(tmem + ((uint32_t)(quarter * 32) << 16) + c0, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; j += 4)
+        *reinterpret_cast<float4*>(red + row * red_stride + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (ks > 1) cluster_sync_all();  // every block's sums are in its shared memory
+
+  if (warp >= 2 && !*failed) {  // this block's share of the tokens, four at a time; a thread keeps its row of w
+    const int e = threadIdx.x - 64, i = ep.glu ? e & 63 : e, step = ep.glu ? 8 : 4;
+    const int share = ((ep.n_tokens + ks - 1) / ks + 3) / 4 * 4;
+    const int t_hi = min((rank + 1) * share, ep.n_tokens), col = n0 + i;
+    const uint32_t red_addr = smem_u32(red);
+    auto total4 = [&](int row, int t, float* out) {
+      if (ks == 1) {
+        const float4 v = *reinterpret_cast<const float4*>(red + row * red_stride + t);
+        out[0] = v.x; out[1] = v.y; out[2] = v.z; out[3] = v.w;
+        return;
+      }
+      float4 v[MAX_KS];
+      const uint32_t at = red_addr + (uint32_t)(row * red_stride + t) * 4u;
+#pragma unroll
+      for (int r = 0; r < MAX_KS; ++r)  // all loads on their way before the first sum
+        if (r < ks) v[r] = ld_cluster_f32x4(at, (uint32_t)r);
+      out[0] = out[1] = out[2] = out[3] = 0.f;
+#pragma unroll
+      for (int r = 0; r < MAX_KS; ++r)
+        if (r < ks) {
+          out[0] += v[r].x; out[1] += v[r].y; out[2] += v[r].z; out[3] += v[r].w;
+        }
+    };
+    const bool live = col < ep.outputs;
+    const float sw = live ? ep.sw[col] : 0.f, su = live && ep.glu ? ep.sw[ep.outputs + col] : 0.f;
+    for (int t = rank * share + (ep.glu ? 4 * (e >> 6) : 0); t < t_hi; t += step) {
+      float v[4], u[4];
+      total4(i, t, v);
+      if (ep.glu) total4(64 + i, t, u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (t + j >= M || !live) continue;
+        const float sx = ep.sx[t + j];
+        float y = scaled(v[j], sx * sw, ep.bias, col);
+        if (ep.glu) y = activate(y, ep.act) * scaled(u[j], sx * su, ep.bias, ep.outputs + col);
+        const size_t at = (size_t)(t + j) * ep.outputs + col;
+        if (!FMS_IN(at, (size_t)M * ep.outputs)) continue;
+        if (ep.out_f32) ((float*)ep.out)[at] = y;
+        else ((__nv_bfloat16*)ep.out)[at] = __float2bfloat16_rn(y);
+      }
+    }
+  }
+  if (ks > 1) cluster_sync_all();  // nobody leaves while another block still reads its shared memory
+  __syncthreads();
+  if (threadIdx.x == 0 && *failed && error_flag) atomicExch(error_flag, 4);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+// [rows, pitch] bytes in boxes of `box_rows` rows x 128 bytes with the 128-byte swizzle
+int make_byte_map(CUtensorMap* map, const void* base, long rows, long pitch, int box_rows) {
+  EncodeTiled enc = encode_tiled();
+  if (enc == nullptr) return fms_fail("gemm_e4m3: the driver does not export cuTensorMapEncodeTiled");
+  const cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
+  const cuuint32_t box[2] = {TILE_K, (cuuint32_t)box_rows}, elem[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fms_fail("gemm_e4m3: cuTensorMapEncodeTiled failed with %d (rows %ld, pitch %ld)", (int)r, rows, pitch);
+  return 0;
+}
+
+int multiprocessors() {
+  static int sms = 0;
+  if (sms == 0) {
+    int device = 0;
+    cudaGetDevice(&device);
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) sms = 148;
+  }
+  return sms;
+}
+
+// The width of a pair's tile: the one whose tiles cost least in whole rounds of the pairs, a tile costing what its copies or its
+// instructions take, whichever is more.
+int choose_tile_n(int tiles_m, int cols, bool glu, int pairs) {
+  const int step = glu ? 32 : 16;
+  long best_cost = -1;
+  int best = 256;
+  for (int tn = 256; tn >= 64; tn -= step) {
+    const int out = glu ? tn / 2 : tn;
+    const long tiles = (long)tiles_m * ((cols + out - 1) / out);
+    const long cost = ((tiles + pairs - 1) / pairs) * (tn == 256 ? 10000 : 5600 + 14 * tn);
+    if (best_cost < 0 || cost < best_cost) {
+      best_cost = cost;
+      best = tn;
+    }
+  }
+  return best;
+}
+
+// Blocks that share a tile: from the weights' shape alone, enough for two blocks a multiprocessor, at least 4 steps a block
+int choose_ks(int tiles, int k_steps) {
+  int ks = 1;
+  while (ks < MAX_KS && tiles * ks * 2 <= 320 && k_steps / (ks * 2) >= 4) ks *= 2;
+  return ks;
+}
+
+constexpr int ROWS_MOST = 256;  // rows of x that the second kernel takes
+// A block that holds all of the tensor memory takes so much shared memory that no block that wants some fits beside it: one that
+// waits for it could be what this one waits for (the partner of a pair, the kernel before).
+constexpr size_t PAIR_RING = 200 * 1024, EXTRA = 1024 /* alignment */ + 512 /* barriers */;
+
+// Asks for a kernel's shared memory once on every device.
+template <typename Kernel> int allow_smem(const char* what, Kernel kernel, int bytes, uint64_t* done) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && device < 64 && (*done >> device & 1)) return 0;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fms_fail("%s: %d bytes of shared memory refused: %s", what, bytes, cudaGetErrorString(e));
+  if (device < 64) *done |= 1ull << device;
+  return 0;
+}
+
+int launch(const void* x, const void* w, Epilogue ep, int M, int N, long pitch, int* error_flag, cudaStream_t stream) {
+  if (pitch <= 0 || pitch % 16 || pitch > 0x7fffff00L) return fms_fail("gemm_e4m3: rows of %ld bytes, a multiple of 16 is wanted", pitch);
+  if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)ep.out) & 15) return fms_fail("gemm_e4m3: operands and result must be 16-byte aligned");
+  const int k_steps = (int)((pitch + TILE_K - 1) / TILE_K);
+  CUtensorMap map_x, map_w;
+  static uint64_t rows_allowed = 0, pair_allowed = 0;
+  if (M <= ROWS_MOST ? allow_smem("gemm_e4m3", e4m3_rows_kernel, 225 * 1024, &rows_allowed)
+                     : allow_smem("gemm_e4m3", e4m3_pair_kernel, (int)(PAIR_RING + EXTRA), &pair_allowed))
+    return 1;
+  if (M <= ROWS_MOST) {
+    ep.n_tokens = (M + 15) / 16 * 16;
+    const int row_step = ep.glu ? TILE / 2 : TILE, tiles = (ep.outputs + row_step - 1) / row_step;
+    if (tiles > 65535) return fms_fail("gemm_e4m3: %d tiles of rows of w", tiles);
+    ep.ks = choose_ks(tiles, k_steps);
+    const int stage_bytes = BOX_BYTES + ep.n_tokens * TILE_K;
+    // two blocks a multiprocessor; one where the tokens are many or the blocks few
+    const int budget = (ep.n_tokens <= 128 && tiles * ep.ks > 148) ? 104 * 1024 : 200 * 1024;
+    const size_t red_bytes = (size_t)TILE * (ep.n_tokens + 4) * sizeof(float);
+    ep.stages = min(max(budget / stage_bytes, 3), MAX_STAGES);
+    while ((size_t)ep.stages * stage_bytes < red_bytes) ++ep.stages;  // the sums go over the stages
+    if (make_byte_map(&map_x, x, M, pitch, ep.n_tokens) || make_byte_map(&map_w, w, N, pitch, row_step)) return 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ep.ks, tiles);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = (size_t)ep.stages * stage_bytes + EXTRA;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ep.ks;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = fms_pdl_enabled() ? 2 : 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, e4m3_rows_kernel, map_x, map_w, ep, M, k_steps, error_flag);
+    if (e != cudaSuccess) return fms_fail("gemm_e4m3: launch failed: %s", cudaGetErrorString(e));
+    return fms_launch_status("gemm_e4m3");
+  }
+  const int pairs = max(multiprocessors() / 2, 1), tiles_m = (M + 2 * TILE - 1) / (2 * TILE);
+  ep.tile_n = choose_tile_n(tiles_m, ep.outputs, ep.glu != 0, pairs);
+  const int stage_bytes = BOX_BYTES + ep.tile_n / 2 * TILE_K, out = ep.glu ? ep.tile_n / 2 : ep.tile_n;
+  ep.stages = min((int)(PAIR_RING / stage_bytes), MAX_STAGES);
+  if (make_byte_map(&map_x, x, M, pitch, TILE) || make_byte_map(&map_w, w, N, pitch, ep.tile_n / 2)) return 1;
+  const long tiles = (long)((ep.outputs + out - 1) / out) * tiles_m;
+  if (tiles > 0x7fffffffL) return fms_fail("gemm_e4m3: %ld tiles", tiles);
+  const int busy = (int)(tiles < pairs ? tiles : pairs);
+  fms_launch(e4m3_pair_kernel, dim3(2 * busy), dim3(THREADS), PAIR_RING + EXTRA, stream, map_x, map_w, ep, M,
+             k_steps, error_flag);
+  return fms_launch_status("gemm_e4m3");
+}
+}  // namespace
+
+// y [M, N] (bfloat16, or float32 with out_dtype FMS_F32) of x [M, pitch] and w [N, pitch], e4m3, with sx [M], sw [N] float32 and
+// bias [N] bfloat16 or null.
+FMS_API int fms_linear_e4m3(const void* x, const float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype,
+                            int M, int N, long pitch, int* error_flag, cudaStream_t stream) {
+  if (M <= 0 || N <= 0) return 0;
+  if (out_dtype != FMS_F32 && out_dtype != FMS_BF16) return fms_fail("linear_e4m3: out dtype %d", out_dtype);
+  Epilogue ep = {};
+  ep.out = y;
+  ep.bias = (const __nv_bfloat16*)bias;
+  ep.sx = sx;
+  ep.sw = sw;
+  ep.out_f32 = out_dtype == FMS_F32;
+  ep.outputs = N;
+  return launch(x, w, ep, M, N, pitch, error_flag, stream);
+}
+
+// y [M, hidden] bfloat16 = act(gate) * up for w = [gate; up] of 2 hidden rows (sw and bias [2 hidden]).
+FMS_API int fms_glu_e4m3(const void* x, const float* sx, const void* w, const float* sw, const void* bias, void* y, int M, int hidden,
+                         long pitch, int act, int* error_flag, cudaStream_t stream) {
+  if (M <= 0 || hidden <= 0) return 0;
+  if (act < 0 || act > 3) return fms_fail("glu_e4m3: activation %d", act);
+  Epilogue ep = {};
+  ep.out = y;
+  ep.bias = (const __nv_bfloat16*)bias;
+  ep.sx = sx;
+  ep.sw = sw;
+  ep.glu = 1;
+  ep.act = act;
+  ep.outputs = hidden;
+  return launch(x, w, ep, M, 2 * hidden, pitch, error_flag, stream);
+}

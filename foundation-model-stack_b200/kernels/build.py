@@ -44,6 +44,9 @@ PLAIN_LIBRARIES = {
     "gemm_bf16_skinny": ("gemm_bf16_skinny.cu", []),
     "gemm_bf16_mid": ("gemm_bf16_mid.cu", []),
     "gemm_bf16_tc": ("gemm_bf16_tc.cu", []),
+    "quantize_rows": ("quantize_rows.cu", []),
+    "gemm_e4m3": ("gemm_e4m3.cu", []),
+    "gemm_int4": ("gemm_int4.cu", []),
     "sampling": ("sampling.cu", []),
     "recurrent": ("recurrent.cu", []),
     "state_scan": ("state_scan.cu", []),

@@ -66,6 +66,12 @@ _SIGNATURES = {
     "fms_glu_bf16_tc": [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "fms_qkv_rope_store_bf16_tc": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P,
                                    _I, _I, _I, _P],
+    "fms_quantize_rows": [_P, _I, _P, _P, _I, _I, _I, _P],
+    "fms_add_rmsnorm_quantized": [_P, _P, _I, _P, _I, _F, _P, _P, _P, _I, _I, _I, _I, _P],
+    "fms_linear_e4m3": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _L, _P, _P],
+    "fms_glu_e4m3": [_P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _P, _P],
+    "fms_linear_int4": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P],
+    "fms_glu_int4": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
     "fms_embed_pair_hash": [_P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _L, _L, _L, _F, _I, _I, _I, _P, _P],
     "fms_normed_add_rmsnorm": [_P, _P, _I, _P, _F, _F, _P, _F, _F, _I, _P, _I, _P, _I, _I, _I, _P],
     "fms_mingru_scan": [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P, _P],
@@ -519,7 +525,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            out_dtype: Optional[torch.dtype] = None, sequences=None) -> torch.Tensor:
     """x [rows, in] times weight [out, in] transposed (+ bias).  ``out_dtype`` defaults to x's dtype.  ``sequences``: the rows'
     ``Batch`` or how many rows each sequence has, one behind the other (a large float32 product chooses its kernel by it); None:
-    every row stands alone."""
+    every row stands alone.  A quantised weight (``E4M3Weight``, ``Int4Weight``) takes its own product, and x may then be
+    ``QuantizedRows`` for the former."""
+    if isinstance(weight, QUANTIZED_WEIGHTS):
+        return quantized.linear(x, weight, bias, out_dtype)
     out_dtype = out_dtype or x.dtype
     _ptr(x), _ptr(weight)
     if weight.dtype == torch.float32:
@@ -638,6 +647,8 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
                  sequences=None) -> torch.Tensor:
     """act(x Wg^T) * (x Wu^T) for weight = [Wg; Wu]: one kernel for few bfloat16 rows, else the product
     followed by ``gated_activation``."""
+    if isinstance(weight, QUANTIZED_WEIGHTS):
+        return quantized.gated_linear(x, weight, bias, activation)
     hidden = weight.shape[0] // 2
     if (x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and x.shape[0] <= SKINNY_ROWS
             and weight.shape[1] % 8 == 0 and (bias is None or bias.dtype == torch.bfloat16)):
@@ -664,8 +675,8 @@ def activated_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     """act(x weight^T + bias): the first product of an ungated feed-forward.  A few bfloat16 rows: the weight-streaming kernel
     with the activation in its epilogue; many, where its tiles fit (as for the gated product): the tcgen05 kernel with
     the activation in its epilogue; else the product and then the activation in place."""
-    own = x.dtype == weight.dtype == torch.bfloat16 and weight.shape[1] % 8 == 0 and (bias is None or bias.dtype == torch.bfloat16) \
-        and activation <= 3
+    own = not isinstance(weight, QUANTIZED_WEIGHTS) and x.dtype == weight.dtype == torch.bfloat16 and weight.shape[1] % 8 == 0 \
+        and (bias is None or bias.dtype == torch.bfloat16) and activation <= 3
     if own and x.shape[0] <= SKINNY_ROWS:
         y = x.new_empty((x.shape[0], weight.shape[0]))
         _call("gemm_bf16_skinny", "fms_linear_act_bf16_skinny", x, weight, bias, y, x.shape[0],
@@ -774,7 +785,9 @@ def qkv_rope_store(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.T
     """An attention layer's fused projection and what follows it: qkv = x weight^T (+ bias), q and k rotated by each
     token's position, k and v written into the cache, the rotated q returned.  For a few bfloat16 rows (a decode
     step) this is one kernel, the weight-streaming product with the rotation and the cache write in its epilogue;
-    else the product and ``rope_store`` one after the other."""
+    else (and for quantised weights) the product and ``rope_store`` one after the other."""
+    if isinstance(weight, QUANTIZED_WEIGHTS):
+        return rope_store(linear(x, weight, bias), inv_freq, batch, view, nheads, kvheads, head_dim, writes_cache)
     if (FUSE_QKV_ROPE and x.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and x.shape[0] <= SKINNY_ROWS
             and weight.shape[1] % 8 == 0 and head_dim % 2 == 0 and (bias is None or bias.dtype == torch.bfloat16)
             and view.keys.dtype == torch.bfloat16 and weight.shape[0] == (nheads + 2 * kvheads) * head_dim):
@@ -1694,3 +1707,10 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int, seed: int, requ
     _call("sampling", "fms_sample", logits, out, rows, vocab, float(temperature), int(top_k),
           int(seed) & 0xFFFFFFFFFFFFFFFF, requests, int(step), _stream())
     return out
+
+
+# ---- quantised linear layers (kernels/quantized.py) -----------------------------------------------------
+from . import quantized  # noqa: E402  (it takes the launches from this module)
+from .quantized import (  # noqa: E402,F401
+    QUANTIZED_WEIGHTS, E4M3Weight, Int4Weight, QuantizedRows, add_rmsnorm_quantized, e4m3_weight, gated_linear_e4m3,
+    gated_linear_int4, linear_e4m3, linear_int4, pack_int4, quantize_e4m3, quantize_int4, quantize_rows)

@@ -1,0 +1,95 @@
+"""Quantised weights without a device: the packed layout and what it stands for, rounding to 4 bits, and what is refused."""
+import pytest
+import torch
+
+from fms_b200.kernels import ops
+
+BF16 = torch.bfloat16
+
+
+def gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("out,dim,group", [(1, 8, 32), (16, 128, 128), (37, 328, 64), (40, 1000, 32), (17, 136, 136), (5, 1160, 160), (33, 256, 1024)])
+def test_packed_weights_stand_for_what_was_given(out, dim, group, zeros):
+    g = gen(out + dim)
+    groups = -(-dim // min(group, (dim + 31) // 32 * 32))
+    q = torch.randint(0, 16, (out, dim), generator=g, dtype=torch.uint8)
+    s = (torch.rand(out, groups, generator=g) + 0.1).to(BF16)
+    z = torch.randint(0, 16, (out, groups), generator=g, dtype=torch.uint8) if zeros else None
+    w = ops.pack_int4(q, s, z, group)
+    at = torch.arange(dim) // group
+    want = (q.float() - (z.float()[:, at] if zeros else 8.0)) * s.float()[:, at]
+    assert w.shape == (out, dim) and torch.equal(w.dequantize(), want)
+
+
+def test_the_layout_of_a_block():
+    """Value k of row r: word 16 r' + 4 place + k // 32, place = (k // 8 % 4) ^ (r // 2 % 4), bits 4 (k % 8 // 2) + 16 (k % 2)."""
+    q = torch.randint(0, 16, (32, 256), generator=gen(0), dtype=torch.uint8)
+    w = ops.pack_int4(q, torch.ones(32, 2), None, 128)
+    for r, k in ((0, 0), (0, 1), (3, 13), (17, 200), (31, 255), (9, 127), (14, 64)):
+        word = int(w.blocks[r // 16, k // 128, r % 16, (k // 8 % 4) ^ (r // 2 % 4), k % 128 // 32])
+        assert (word >> (4 * (k % 8 // 2) + 16 * (k % 2))) & 15 == int(q[r, k])
+    assert int(w.groups[1, 5]) & 0xFFFF == 0x3F80 and (int(w.groups[1, 5]) >> 16) & 0xFFFF == 0x4308  # bfloat16 1 and 136
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("out,dim,group", [(5, 64, 32), (33, 200, 64), (4, 72, 72), (4100, 32, 32)])
+def test_rounding_to_four_bits(out, dim, group, dtype):
+    w = (torch.randn(out, dim, generator=gen(out)) * 0.02).to(dtype)
+    w[0] = 0.0
+    w[1] = w[1].abs() + 1.0  # one sign: the steps reach down to zero all the same
+    got = ops.quantize_int4(w, group)
+    groups = -(-dim // group)
+    wide = torch.zeros(out, groups * group)
+    wide[:, :dim] = w.float()
+    wide = wide.view(out, groups, group)
+    # half a step for the value and half a step for the zero point that moved it; the scale's rounding moves the ends by up to 15 steps' 2^-8
+    step = ((wide.amax(2).clamp(min=0) - wide.amin(2).clamp(max=0)) / 15)[:, torch.arange(dim) // group]
+    assert bool(((got.dequantize() - w.float()).abs() <= step * (1.0 + 15 * 2.0 ** -8 + 2.0 ** -6) + 1e-30).all())
+    assert float(got.dequantize()[0].abs().max()) == 0.0
+
+
+def test_rows_that_need_a_copy_get_one():
+    v = torch.randn(3, 32, generator=gen(1)).to(torch.float8_e4m3fn)
+    s = torch.ones(3)
+    assert ops.QuantizedRows.of(v, s).values.data_ptr() == v.data_ptr()
+    odd = ops.QuantizedRows.of(v[:, :21], s)
+    assert odd.shape == (3, 21) and odd.values.shape == (3, 32)
+    assert torch.equal(odd.dequantize(), v[:, :21].float()) and float(odd.values[:, 21:].float().abs().max()) == 0.0
+
+
+def test_refusals():
+    E = ops.KernelError
+    q, s = torch.zeros(4, 64, dtype=torch.uint8), torch.ones(4, 2)
+    v = torch.zeros(4, 32).to(torch.float8_e4m3fn)
+    for call in (
+        lambda: ops.pack_int4(q.float(), s, None, 32),
+        lambda: ops.pack_int4(q[0], s, None, 32),
+        lambda: ops.pack_int4(q[:, :60], s, None, 32),                      # no multiple of 8
+        lambda: ops.pack_int4(q, s, None, 48),                              # no multiple of 32
+        lambda: ops.pack_int4(q, s, None, 0),
+        lambda: ops.pack_int4(q, s, None, 64),                              # one group, two scales
+        lambda: ops.pack_int4(q, s.long(), None, 32),
+        lambda: ops.pack_int4(q, s, s, 32),                                 # zero points are whole numbers
+        lambda: ops.pack_int4(q + 16, s, None, 32),
+        lambda: ops.pack_int4(q, s, torch.full((4, 2), 16), 32),
+        lambda: ops.pack_int4(q, s, torch.full((4, 2), -1), 32),
+        lambda: ops.quantize_int4(q, 32),
+        lambda: ops.quantize_int4(torch.ones(4, 64), 40),
+        lambda: ops.QuantizedRows.of(torch.zeros(4, 32), torch.ones(4)),
+        lambda: ops.QuantizedRows.of(v, torch.ones(3)),
+        lambda: ops.QuantizedRows.of(v, torch.ones(4, dtype=BF16)),
+        lambda: ops.QuantizedRows(v, torch.ones(4), 40),
+        lambda: ops.quantize_rows(torch.ones(4, 32)),                       # on the CPU
+        lambda: ops.quantize_e4m3(torch.ones(4, 32)),
+        lambda: ops.add_rmsnorm_quantized(torch.ones(4, 32), None, torch.ones(32), 1e-5),
+        lambda: ops.linear_e4m3(ops.QuantizedRows.of(v, torch.ones(4)), ops.e4m3_weight(v, torch.ones(4))),
+        lambda: ops.linear_int4(torch.ones(2, 64, dtype=BF16), ops.pack_int4(q, s, None, 32)),
+    ):
+        with pytest.raises(E):
+            call()
