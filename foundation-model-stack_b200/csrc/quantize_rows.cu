@@ -4,27 +4,29 @@
 //   add_rmsnorm       x = residual[src] + delta[src]  (float32; written back unless rows are gathered),
 //                     y = x * rsqrt(mean(x^2) + eps) * gain,  s = max |y| / 448,  q = e4m3(y * 448 / max |y|)
 //                                                                   (the norm: fms/modules/layernorm.py:56-69)
-// e4m3() rounds to the nearest value, ties to even.  A row whose scale would lie below the smallest normal float32 (a row
-// of zeros) gets scale 0 and zeros.  A row with a NaN or an infinity gets a scale that is not finite (NaN behind the norm),
+// e4m3() rounds to the nearest value, ties to even.  A row whose scale would lie below 2^-110 (a row of zeros) gets scale 0
+// and zeros.  A row with a NaN or an infinity gets a scale that is not finite (NaN behind the norm),
 // so that what a product makes of it is not finite either, and the other rows do not see it.
 //
 // Both are bound by memory: a value is read once (2 or 4 bytes, behind the norm 4 and 2 or 4), the stream written (4) and
-// one byte stored.  A thread block owns a row and keeps it in registers between the maximum and the rounding, so that
-// nothing is read twice; a thread owns runs of 8 values, 16-byte loads and 8-byte stores.  Rows of q are `pitch` bytes
-// apart, dim rounded up to 16 with zeros behind the last value, as the products' copies want them; rows of x whose width is
-// no multiple of the load's are read value by value.
+// one byte stored.  A thread block owns a row and keeps it in registers, as it was loaded, between the maximum and the rounding,
+// so that nothing is read twice.  A thread owns runs of 8 neighbours, 16-byte loads and 8-byte stores; where an array's rows do
+// not begin on 16 bytes, 8 values a whole block apart, so that a warp's single loads and stores are neighbours.  Rows of q are
+// `pitch` bytes apart, dim rounded up to 16 with zeros behind the last value, as the products' copies want them.
 //
-// q is what the exact quotient rounds to.  Behind the norm the division by the root mean square cancels in it: with t = x * gain it
-// is t * 448 / max |t|.  In float32 it comes out within a few units of its last place, which decides the rounding to 4 bits but
-// for a few values in a million that come out beside the middle of two neighbours; a run of 8 that has one is compared
-// with those middles in float64, where t * 448 and a middle times max |t| are exact.
+// q is what the exact quotient rounds to.  Of bfloat16 rows it is often a tie, and otherwise, a ratio of numbers of 11 and 8 bits,
+// at least 2^-13 away from one, so one step of Newton's, whose remainder x * 448 - q0 * max |x| is exact in a fused
+// multiply-add, decides it.  Behind the norm the division by the root mean square cancels: with t = x * gain, q is t * 448 / max |t|.
+// There, and of float32 rows, the float32 quotient is within a few units of its last place, which decides the rounding but for a
+// few values in a million that come out beside the middle of two neighbours; a run of 8 that has one is compared with
+// those middles in float64, where t * 448 and a middle times max |t| are exact.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
 
 namespace {
 constexpr float E4M3_MAX = 448.f;
-constexpr float LEAST = 1.17549435e-38f;  // the smallest normal float32
+constexpr float LEAST = 0x1p-110f;  // a scale below is none
 
 // the larger of two, NaN where either is one
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -33,39 +35,47 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-__device__ __forceinline__ void load8(const float* p, float* v) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* v) {
-  const uint4 t = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+// 8 values of a row as they were loaded
+template <typename T> struct Run;
+template <> struct Run<float> {
+  static constexpr bool EXACT = false;  // 448 times a value has 24 bits at most
+  float v[8];
+  __device__ __forceinline__ float operator[](int e) const { return v[e]; }
+  __device__ __forceinline__ void set(int e, float x) { v[e] = x; }
+  __device__ __forceinline__ void load(const float* p) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
-}
-// values c0 .. c0 + 7 of a row of `dim`; zeros beyond its end
-template <typename T>
-__device__ __forceinline__ void load_run(const T* row, int c0, int dim, bool vectors, float* v) {
-  if (vectors && c0 + 8 <= dim) {
-    load8(row + c0, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c0 + e < dim ? to_f32(row[c0 + e]) : 0.f;
+};
+template <> struct Run<__nv_bfloat16> {
+  static constexpr bool EXACT = true;
+  uint32_t w[4];
+  __device__ __forceinline__ float operator[](int e) const { return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16); }
+  __device__ __forceinline__ void set(int e, __nv_bfloat16 x) {
+    const uint32_t h = __bfloat16_as_ushort(x);
+    w[e / 2] = e & 1 ? w[e / 2] | (h << 16) : h;
   }
-}
-__device__ __forceinline__ void store_run(float* row, int c0, int dim, bool vectors, const float* v) {
-  if (vectors && c0 + 8 <= dim) {
-    reinterpret_cast<float4*>(row + c0)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(row + c0)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c0 + e < dim) row[c0 + e] = v[e];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    const uint4 t = *reinterpret_cast<const uint4*>(p);
+    w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
   }
+};
+// The place in the row of value e of this thread's run j
+template <bool NEIGHBOURS> __device__ __forceinline__ int place(int j, int e) {
+  return NEIGHBOURS ? 8 * (threadIdx.x + j * blockDim.x) + e : (8 * j + e) * blockDim.x + threadIdx.x;
+}
+// zeros beyond the row's end; neighbours: dim is a multiple of 8 then
+template <bool NEIGHBOURS, typename T> __device__ __forceinline__ void load_run(Run<T>& run, const T* row, int j, int dim) {
+  if (NEIGHBOURS) {
+    const int c0 = place<true>(j, 0);
+    if (c0 < dim) {
+      run.load(row + c0);
+      return;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) run.set(e, !NEIGHBOURS && place<false>(j, e) < dim ? row[place<false>(j, e)] : T(0.f));
 }
 // 8 values as e4m3, nearest and ties to even, beyond 448 to 448
 __device__ __forceinline__ uint2 to_e4m3(const float* v) {
@@ -76,28 +86,39 @@ __device__ __forceinline__ uint2 to_e4m3(const float* v) {
   return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
-// zeros behind a row's last value, whatever the quotients there
-__device__ __forceinline__ uint2 ended(uint2 q, int c0, int dim) {
-  const int left = dim - c0;
-  if (left >= 8) return q;
-  const uint64_t v = left <= 0 ? 0ull : (((uint64_t)q.y << 32) | q.x) & (~0ull >> (64 - 8 * left));
-  return make_uint2((uint32_t)v, (uint32_t)(v >> 32));
+// zeros where the row has ended, where zeros times what is not finite are not
+template <bool NEIGHBOURS> __device__ __forceinline__ float* ended(float* q, int j, int dim) {
+  if (!NEIGHBOURS || place<true>(j, 0) >= dim) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = place<NEIGHBOURS>(j, e) < dim ? q[e] : 0.f;
+  }
+  return q;
 }
 
-// 8 quotients t * 448 / most, t = x (* g), rounded to e4m3 as exact quotients would be; inv = 448 / most in float32.
-// q0, four roundings away from the quotient, is off by less than 4 units of its last place (2^-22 of it).
-template <bool GAIN> __device__ __forceinline__ uint2 quotients(const float* x, const float* g, float inv, double most) {
+// 8 quotients t * 448 / most, t = x (* g), to e4m3 as exact quotients would be, zeros where the row has ended; inv = 448 / most.
+// The float32 quotient, three or four roundings away, is off by less than 4 units of its last place.
+template <bool NEIGHBOURS, bool GAIN, typename X, typename G>
+__device__ __forceinline__ uint2 quotients(const X& x, const G& g, float inv, double most, int j, int dim) {
   float q[8];
-  bool near = false;
+  if (!GAIN && X::EXACT) {  // inv = 448 / most is 0.875 / part, and neither 0.875 x nor part is rounded or out of range
+    const float part = (float)most * 0x1p-9f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float q0 = x[e] * inv;
+      q[e] = fmaf(fmaf(-q0, part, x[e] * 0.875f), inv * (1.f / 0.875f), q0);
+    }
+    return to_e4m3(ended<NEIGHBOURS>(q, j, dim));
+  }
+  // From 2^-6 on a value is beside a middle where its last 20 bits are within 8 of 2^19; below, the middles are the odd
+  // multiples of 2^-10, which 2^-6 more puts where the same test finds them.
+  uint32_t beside = ~0u;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     q[e] = (GAIN ? x[e] * g[e] : x[e]) * inv;
-    // from 2^-6 on the middles have 4 bits of mantissa and a half; below they lie at odd multiples of 2^-10
-    const float m = fabsf(q[e]), steps = m * 512.f;
-    const bool beside = m >= 0x1p-6f ? ((__float_as_uint(m) & 0xfffffu) - 0x7fff8u) <= 16u : fabsf(steps - floorf(steps) - 0.5f) < 0x1p-14f;
-    near |= beside;
+    const float m = fabsf(q[e]);
+    beside = min(beside, __float_as_uint(m < 0x1p-6f ? m + 0x1p-6f : m) * 4096u - (0x7fff8u << 12));  // the 20 bits, first
   }
-  if (near && most < INFINITY) {
+  if (beside <= (16u << 12) && most < INFINITY) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float m = fabsf(q[e]);
@@ -109,7 +130,16 @@ template <bool GAIN> __device__ __forceinline__ uint2 quotients(const float* x, 
       q[e] = copysignf(r, q[e]);
     }
   }
-  return to_e4m3(q);
+  return to_e4m3(ended<NEIGHBOURS>(q, j, dim));
+}
+template <bool NEIGHBOURS> __device__ __forceinline__ void store_run(uint8_t* row, uint2 q, int j, int pitch) {
+  if (NEIGHBOURS) {
+    if (place<true>(j, 0) < pitch) *reinterpret_cast<uint2*>(row + place<true>(j, 0)) = q;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (place<false>(j, e) < pitch) row[place<false>(j, e)] = (uint8_t)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
+  }
 }
 
 __device__ __forceinline__ float block_max(float v, float* scratch) {
@@ -124,27 +154,41 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
   return v;
 }
 
+// the largest magnitude of a run, NaN where one is NaN
+__device__ __forceinline__ float largest(const Run<float>& r) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(r.v[e]));
+  return m;
+}
+__device__ __forceinline__ float largest(const Run<__nv_bfloat16>& r) {
+  __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&r.w[0]));
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&r.w[i])));
+  return max_nan(__low2float(m), __high2float(m));
+}
+
 // RUNS: runs of 8 values that a thread keeps; 0: any width, the row is read a second time.
-template <typename T, int RUNS>
-__global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales, int n_rows,
-                                                             int dim, int pitch, int vectors) {
+template <typename T, int RUNS, bool NEIGHBOURS>
+__global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && RUNS != 1 && RUNS != 8 ? 2 : 1) quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
+                                                             int n_rows, int dim, int pitch) {
   __shared__ float scratch[32];
   pdl_launch_dependents();
   pdl_wait();
+  if (!FMS_IN(blockIdx.x, n_rows)) return;
   const T* row = x + (size_t)blockIdx.x * dim;
   uint8_t* out = q + (size_t)blockIdx.x * pitch;
   constexpr int KEPT = RUNS > 0 ? RUNS : 1;
   const int runs = RUNS > 0 ? RUNS : (pitch / 8 + blockDim.x - 1) / blockDim.x;
-  float v[KEPT][8], most = 0.f;
+  Run<T> v[KEPT];
+  float most = 0.f;
 #pragma unroll
   for (int j = 0; j < KEPT; ++j)
-    if (RUNS > 0) load_run(row, 8 * (threadIdx.x + j * blockDim.x), dim, vectors, v[j]);
+    if (RUNS > 0) load_run<NEIGHBOURS>(v[j], row, j, dim);
 #pragma unroll KEPT
   for (int j = 0; j < runs; ++j) {
-    if (RUNS == 0) load_run(row, 8 * (threadIdx.x + j * blockDim.x), dim, vectors, v[0]);
-    float* u = v[RUNS > 0 ? j : 0];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) most = max_nan(most, fabsf(u[e]));
+    if (RUNS == 0) load_run<NEIGHBOURS>(v[0], row, j, dim);
+    most = max_nan(most, largest(v[RUNS > 0 ? j : 0]));
   }
   most = block_max(most, scratch);
   const float s = most / E4M3_MAX;
@@ -152,13 +196,11 @@ __global__ void __launch_bounds__(1024) quantize_rows_kernel(const T* __restrict
   const float inv = none ? 0.f : E4M3_MAX / most;
 #pragma unroll KEPT
   for (int j = 0; j < runs; ++j) {
-    const int c0 = 8 * (threadIdx.x + j * blockDim.x);
-    if (RUNS == 0) load_run(row, c0, dim, vectors, v[0]);
-    float* u = v[RUNS > 0 ? j : 0];
-    if (c0 < pitch && FMS_IN((size_t)blockIdx.x * pitch + c0 + 7, (size_t)n_rows * pitch))
-      *reinterpret_cast<uint2*>(out + c0) = ended(quotients<false>(u, nullptr, inv, most), c0, dim);
+    if (RUNS == 0) load_run<NEIGHBOURS>(v[0], row, j, dim);
+    const Run<T>& u = v[RUNS > 0 ? j : 0];
+    store_run<NEIGHBOURS>(out, quotients<NEIGHBOURS, false>(u, u, inv, most, j, dim), j, pitch);
   }
-  if (threadIdx.x == 0 && FMS_IN(blockIdx.x, n_rows)) scales[blockIdx.x] = none ? 0.f : s;
+  if (threadIdx.x == 0) scales[blockIdx.x] = none ? 0.f : s;
 }
 
 // a float32 and what rounding to it left over: the larger of two magnitudes
@@ -167,48 +209,70 @@ struct Pair {
 };
 __device__ __forceinline__ Pair larger(Pair a, Pair b) { return b.hi > a.hi || (b.hi == a.hi && b.lo > a.lo) ? b : a; }
 
-template <typename T, typename TG, int RUNS>
-__global__ void __launch_bounds__(1024) add_rmsnorm_quantized_kernel(float* __restrict__ residual, const T* __restrict__ delta,
+template <typename T, typename TG, int RUNS, bool NEIGHBOURS>
+__global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && (RUNS == 0 || RUNS == 2) ? 2 : 1) add_rmsnorm_quantized_kernel(float* __restrict__ residual, const T* __restrict__ delta,
                                                                      const TG* __restrict__ gain, float eps,
-                                                                      uint8_t* __restrict__ q, float* __restrict__ scales,
-                                                                      const int* __restrict__ rows, int n_rows, int dim,
-                                                                      int pitch, int residual_rows, int vec_x, int vec_d, int vec_g) {
+                                                                     uint8_t* __restrict__ q, float* __restrict__ scales,
+                                                                     const int* __restrict__ rows, int dim, int pitch,
+                                                                     int residual_rows) {
   __shared__ float scratch[3][32];
   constexpr int KEPT = RUNS > 0 ? RUNS : 1;
   const int runs = RUNS > 0 ? RUNS : (pitch / 8 + blockDim.x - 1) / blockDim.x;
-  float x[KEPT][8], g[KEPT][8];
+  Run<float> x[KEPT];
+  Run<TG> g[KEPT];
   pdl_launch_dependents();
 #pragma unroll
   for (int j = 0; j < KEPT; ++j)  // the gain is a weight: it can be read before the kernel before this one is done
-    if (RUNS > 0) load_run(gain, 8 * (threadIdx.x + j * blockDim.x), dim, vec_g, g[j]);
+    if (RUNS > 0) load_run<NEIGHBOURS>(g[j], gain, j, dim);
   pdl_wait();
   const int src = rows ? rows[blockIdx.x] : blockIdx.x;
   if (!FMS_IN(src, residual_rows)) return;  // the whole block alike
   float* res = residual + (size_t)src * dim;
   const T* del = delta ? delta + (size_t)src * dim : nullptr;
-  auto load_sum = [&](int c0, float* v) {
-    load_run(res, c0, dim, vec_x, v);
-    if (del) {
-      float d[8];
-      load_run(del, c0, dim, vec_d, d);
+  const bool writes = del && rows == nullptr;
+  auto add = [&](Run<float>& v, const Run<T>& d) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += d[e];
-    }
+    for (int e = 0; e < 8; ++e) v.v[e] += d[e];
   };
+  if (RUNS > 0) {
+    Run<T> d[KEPT];
 #pragma unroll
-  for (int j = 0; j < KEPT; ++j)
-    if (RUNS > 0) load_sum(8 * (threadIdx.x + j * blockDim.x), x[j]);
+    for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(x[j], res, j, dim);
+    if (del) {
+#pragma unroll
+      for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(d[j], del, j, dim);
+#pragma unroll
+      for (int j = 0; j < KEPT; ++j) add(x[j], d[j]);
+    }
+  }
   float ss = 0.f;
   Pair most = {0.f, 0.f};
 #pragma unroll KEPT
   for (int j = 0; j < runs; ++j) {
-    const int c0 = 8 * (threadIdx.x + j * blockDim.x);
-    float *xs = x[RUNS > 0 ? j : 0], *gs = g[RUNS > 0 ? j : 0];
+    Run<float>& xs = x[RUNS > 0 ? j : 0];
+    Run<TG>& gs = g[RUNS > 0 ? j : 0];
     if (RUNS == 0) {
-      load_sum(c0, xs);
-      load_run(gain, c0, dim, vec_g, gs);
+      load_run<NEIGHBOURS>(xs, res, j, dim);
+      load_run<NEIGHBOURS>(gs, gain, j, dim);
+      if (del) {
+        Run<T> d;
+        load_run<NEIGHBOURS>(d, del, j, dim);
+        add(xs, d);
+      }
     }
-    if (del && rows == nullptr && c0 < dim) store_run(res, c0, dim, vec_x, xs);
+    if (writes) {
+      if (NEIGHBOURS) {
+        if (place<true>(j, 0) < dim) {
+          float4* to = reinterpret_cast<float4*>(res + place<true>(j, 0));
+          to[0] = make_float4(xs.v[0], xs.v[1], xs.v[2], xs.v[3]);
+          to[1] = make_float4(xs.v[4], xs.v[5], xs.v[6], xs.v[7]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (place<false>(j, e) < dim) res[place<false>(j, e)] = xs.v[e];
+      }
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       ss += xs[e] * xs[e];
@@ -237,44 +301,50 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_quantized_kernel(float* __re
 
   // a NaN or an infinity in the row leaves `ss` not finite and the scale NaN (infinity times a root of 0, or NaN)
   const float s = ss < INFINITY ? most.hi * rsqrtf(ss / (float)dim + eps) / E4M3_MAX : NAN;
-  const bool none = s < LEAST || most.hi < 0x1p-110f;  // below 2^-110 the reciprocal would overflow
+  const bool none = s < LEAST || most.hi < LEAST;  // far below, the reciprocal would overflow
   const float inv = none ? 0.f : (s == s ? E4M3_MAX / most.hi : NAN);
   const double exact = (double)most.hi + (double)most.lo;
 #pragma unroll KEPT
   for (int j = 0; j < runs; ++j) {
-    const int c0 = 8 * (threadIdx.x + j * blockDim.x);
-    float *xs = x[RUNS > 0 ? j : 0], *gs = g[RUNS > 0 ? j : 0];
+    Run<float>& xs = x[RUNS > 0 ? j : 0];
+    Run<TG>& gs = g[RUNS > 0 ? j : 0];
     if (RUNS == 0) {
-      if (del && rows == nullptr) load_run(res, c0, dim, vec_x, xs);  // as this thread has stored it
-      else load_sum(c0, xs);
-      load_run(gain, c0, dim, vec_g, gs);
+      load_run<NEIGHBOURS>(xs, res, j, dim);  // the sum, where this thread has stored it
+      load_run<NEIGHBOURS>(gs, gain, j, dim);
+      if (del && !writes) {
+        Run<T> d;
+        load_run<NEIGHBOURS>(d, del, j, dim);
+        add(xs, d);
+      }
     }
-    if (c0 < pitch && FMS_IN((size_t)blockIdx.x * pitch + c0 + 7, (size_t)n_rows * pitch))
-      *reinterpret_cast<uint2*>(q + (size_t)blockIdx.x * pitch + c0) = ended(quotients<true>(xs, gs, inv, exact), c0, dim);
+    store_run<NEIGHBOURS>(q + (size_t)blockIdx.x * pitch, quotients<NEIGHBOURS, true>(xs, gs, inv, exact, j, dim), j, pitch);
   }
   if (threadIdx.x == 0) scales[blockIdx.x] = none ? 0.f : s;
 }
 
-// Threads for a row of `runs` runs of 8, and the runs that each keeps (0: too wide for registers).  Few rows: a thread a run
-// as far as 1,024 go, since only latency counts; many: fewer threads with more runs each, so that more rows are in flight.
-int threads_for(int runs, int n_rows, int each, int* kept) {
-  int threads = 64;
-  while (threads < 1024 && threads * (n_rows <= 296 ? 1 : each) < runs) threads *= 2;
-  const int k = (runs + threads - 1) / threads;
-  *kept = k <= 2 ? k : (k <= 4 && each == 4 ? 4 : 0);
-  return threads;
+// The runs of 8 that a thread keeps (0: the row is too wide for registers) and the threads for a row of `runs` of them.  Few
+// rows: a thread a run as far as 1,024 go, since only latency counts.  Many: `many` runs a thread, so that more bytes a thread and
+// more rows a multiprocessor are on their way (8,192 x 4,096 bfloat16 to e4m3 with 1 / 2 / 4 / 8 runs: 27.5 / 22.8 / 18.2 / 19.8 us;
+// behind the norm, whose runs take 12 registers and more, 2,048 x 4,096 with 1 / 2 / 4: 22.4 / 17.3 / 18.4 us).
+int kept_for(int runs, int n_rows, int many, int most_kept, int* threads) {
+  int kept = n_rows <= 296 ? (runs <= 1024 ? 1 : 4) : (runs <= 128 ? 1 : many);
+  if (runs > 512 * kept && kept > 1) kept = runs <= 512 * 4 ? 4 : (runs <= 512 * most_kept ? most_kept : 0);
+  const int wanted = kept ? (runs + kept - 1) / kept : 512;
+  *threads = (wanted + 31) / 32 * 32;
+  return kept;
 }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <typename T, int RUNS>
 void launch_rows(int threads, const void* x, uint8_t* q, float* scales, int n_rows, int dim, int pitch, cudaStream_t stream) {
-  fms_launch(quantize_rows_kernel<T, RUNS>, dim3(n_rows), dim3(threads), 0, stream, (const T*)x, q, scales, n_rows, dim, pitch,
-             (int)(dim % (16 / (int)sizeof(T)) == 0 && aligned16(x)));
+  const bool neighbours = dim % 8 == 0 && aligned16(x);
+  fms_launch(neighbours ? quantize_rows_kernel<T, RUNS, true> : quantize_rows_kernel<T, RUNS, false>, dim3(n_rows), dim3(threads), 0,
+             stream, (const T*)x, q, scales, n_rows, dim, pitch);
 }
 template <typename T> int quantize(const void* x, uint8_t* q, float* scales, int n_rows, int dim, int pitch, cudaStream_t stream) {
-  int kept;
-  const int threads = threads_for(pitch / 8, n_rows, 4, &kept);
-  (kept == 1 ? launch_rows<T, 1> : kept == 2 ? launch_rows<T, 2> : kept == 4 ? launch_rows<T, 4> : launch_rows<T, 0>)(
+  int threads;
+  const int kept = kept_for(pitch / 8, n_rows, 4, 8, &threads);
+  (kept == 1 ? launch_rows<T, 1> : kept == 2 ? launch_rows<T, 2> : kept == 4 ? launch_rows<T, 4> : kept == 8 ? launch_rows<T, 8> : launch_rows<T, 0>)(
       threads, x, q, scales, n_rows, dim, pitch, stream);
   return fms_launch_status("quantize_rows");
 }
@@ -289,15 +359,15 @@ struct NormArgs {
   int n_rows, dim, pitch, residual_rows;
 };
 template <typename T, typename TG, int RUNS> void launch_norm(int threads, const NormArgs& a, cudaStream_t stream) {
-  fms_launch(add_rmsnorm_quantized_kernel<T, TG, RUNS>, dim3(a.n_rows), dim3(threads), 0, stream, a.residual, (const T*)a.delta,
-             (const TG*)a.gain, a.eps, a.q, a.scales, a.rows, a.n_rows, a.dim, a.pitch, a.residual_rows,
-             (int)(a.dim % 4 == 0 && aligned16(a.residual)), (int)(a.dim % (16 / (int)sizeof(T)) == 0 && aligned16(a.delta)),
-             (int)(a.dim % (16 / (int)sizeof(TG)) == 0 && aligned16(a.gain)));
+  const bool neighbours = a.dim % 8 == 0 && aligned16(a.residual) && aligned16(a.delta) && aligned16(a.gain);
+  fms_launch(neighbours ? add_rmsnorm_quantized_kernel<T, TG, RUNS, true> : add_rmsnorm_quantized_kernel<T, TG, RUNS, false>, dim3(a.n_rows),
+             dim3(threads), 0, stream, a.residual, (const T*)a.delta, (const TG*)a.gain, a.eps, a.q, a.scales, a.rows, a.dim, a.pitch,
+             a.residual_rows);
 }
 template <typename T, typename TG> int norm(const NormArgs& a, cudaStream_t stream) {
-  int kept;
-  const int threads = threads_for(a.pitch / 8, a.n_rows, 2, &kept);
-  (kept == 1 ? launch_norm<T, TG, 1> : kept == 2 ? launch_norm<T, TG, 2> : launch_norm<T, TG, 0>)(threads, a, stream);
+  int threads;
+  const int kept = kept_for(a.pitch / 8, a.n_rows, 2, 4, &threads);
+  (kept == 1 ? launch_norm<T, TG, 1> : kept == 2 ? launch_norm<T, TG, 2> : kept == 4 ? launch_norm<T, TG, 4> : launch_norm<T, TG, 0>)(threads, a, stream);
   return fms_launch_status("add_rmsnorm_quantized");
 }
 }  // namespace

@@ -25,16 +25,17 @@ INT4_FEW_ROWS = 16  # rows up to which the 4-bit product runs on mma.sync and ha
 
 
 def _on_device(what: str, *tensors) -> None:
-    """Every tensor lies on the current device, whose stream the launch goes to, contiguous."""
+    """Every tensor lies on the current device, whose stream the launch goes to (that it is contiguous the launch itself sees to)."""
+    device = None
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise ops.KernelError(f"{what}: a tensor on the CPU reached a CUDA kernel; this library has no CPU path")
-        if t.device.index != ops._device():
-            raise ops.KernelError(f"{what}: a tensor lies on {t.device}, the current device is cuda:{ops._device()}")
-        if not t.is_contiguous():
-            raise ops.KernelError(f"{what}: a non-contiguous tensor reached a CUDA kernel")
+        if device is None:
+            device = ops._device()
+        if t.get_device() != device:
+            raise ops.KernelError(f"{what}: a tensor lies on {t.device}, the current device is cuda:{device}")
 
 
 def _settled(t: torch.Tensor) -> None:
@@ -148,20 +149,24 @@ class Int4Weight:
 
 # ---- rows to 8 bits ------------------------------------------------------------------------------------------------
 def _empty_rows(n: int, dim: int, device) -> QuantizedRows:
-    return QuantizedRows(torch.empty((n, _pitch(dim)), dtype=E4M3, device=device),
-                         torch.empty((n,), dtype=torch.float32, device=device), dim)
+    out = QuantizedRows.__new__(QuantizedRows)  # nothing to check: a decode step makes some hundred of them
+    out.values = torch.empty((n, (dim + 15) // 16 * 16), dtype=E4M3, device=device)
+    out.scales = torch.empty((n,), dtype=torch.float32, device=device)
+    out.dim = dim
+    return out
 
 
 def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     """Rows [rows, dim] (float32 or bfloat16) as e4m3: scale = max |x| / 448, value = x * 448 / max |x| to the nearest, ties to even.  A row of
-    zeros (or of values so small that the scale would be no normal float32) gets scale 0 and zeros; one with a NaN or an
+    zeros (or one whose scale would lie below 2^-110) gets scale 0 and zeros; one with a NaN or an
     infinity a scale that is not finite, and what a product makes of it is not finite either."""
     if x.dim() != 2 or x.shape[1] == 0:
         raise ops.KernelError(f"quantize_rows: rows are [rows, dim], not {tuple(x.shape)}")
     _on_device("quantize_rows", x)
-    out = _empty_rows(x.shape[0], x.shape[1], x.device)
-    ops._call("quantize_rows", "fms_quantize_rows", x, ops._code(x.dtype), out.values, out.scales, x.shape[0], x.shape[1],
-              out.values.shape[1], ops._stream())
+    n, dim = x.shape
+    out = _empty_rows(n, dim, x.device)
+    ops._call("quantize_rows", "fms_quantize_rows", x, ops._code(x.dtype), out.values, out.scales, n, dim, (dim + 15) // 16 * 16,
+              ops._stream())
     return out
 
 
@@ -171,12 +176,13 @@ def add_rmsnorm_quantized(residual: torch.Tensor, delta: Optional[torch.Tensor],
     scale = max |y| / 448, value = y * 448 / max |y|.  With ``rows`` (int32) only those rows are computed and the residual is not
     written.  ``delta`` is float32 or bfloat16 or None, ``gain`` float32 or bfloat16.  Rows of zeros and rows that are not
     finite: as ``quantize_rows``, the scale of the latter NaN."""
-    if residual.dtype != torch.float32 or residual.dim() != 2 or residual.shape[1] == 0:
-        raise ops.KernelError(f"the residual stream is float32 [rows, dim], not {residual.dtype} {tuple(residual.shape)}")
-    n_all, dim = residual.shape
-    if delta is not None and tuple(delta.shape) != (n_all, dim):
-        raise ops.KernelError(f"add_rmsnorm_quantized: the sublayer's output is {tuple(delta.shape)}, the stream {(n_all, dim)}")
-    if tuple(gain.shape) != (dim,):
+    shape = residual.shape
+    if residual.dtype != torch.float32 or len(shape) != 2 or shape[1] == 0:
+        raise ops.KernelError(f"the residual stream is float32 [rows, dim], not {residual.dtype} {tuple(shape)}")
+    n_all, dim = shape
+    if delta is not None and delta.shape != shape:
+        raise ops.KernelError(f"add_rmsnorm_quantized: the sublayer's output is {tuple(delta.shape)}, the stream {tuple(shape)}")
+    if gain.shape != shape[1:]:
         raise ops.KernelError(f"add_rmsnorm_quantized: a gain of {tuple(gain.shape)} for rows of {dim}")
     if rows is not None and (rows.dtype != torch.int32 or rows.dim() != 1):
         raise ops.KernelError(f"add_rmsnorm_quantized: rows are a vector of int32, not {rows.dtype} {tuple(rows.shape)}")
@@ -184,7 +190,7 @@ def add_rmsnorm_quantized(residual: torch.Tensor, delta: Optional[torch.Tensor],
     n = n_all if rows is None else rows.shape[0]
     out = _empty_rows(n, dim, residual.device)
     ops._call("quantize_rows", "fms_add_rmsnorm_quantized", residual, delta, ops.F32 if delta is None else ops._code(delta.dtype), gain,
-              ops._code(gain.dtype), float(eps), out.values, out.scales, rows, n, dim, out.values.shape[1], n_all, ops._stream())
+              ops._code(gain.dtype), float(eps), out.values, out.scales, rows, n, dim, (dim + 15) // 16 * 16, n_all, ops._stream())
     return out
 
 

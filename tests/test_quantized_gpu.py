@@ -65,7 +65,7 @@ def test_quantize_rows_of_zeros_tiny_and_not_finite(ops):
     x = normal(gen(1), 8, 70)
     x[1] = 0.0
     x[2] = -0.0
-    x[3] = 1e-44  # a scale below the smallest normal float32
+    x[3] = 3e-32  # a scale below 2^-110
     x[4, 5] = float("nan")
     x[5, 0] = float("inf")
     x[6] *= 1e30
