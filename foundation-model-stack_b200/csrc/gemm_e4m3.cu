@@ -12,8 +12,8 @@
 #include "common.cuh"
 
 namespace {
-constexpr int TILE = 128, TILE_K = 128, UMMA_K = 32, MAX_STAGES = 12, MAX_KS = 8;
-constexpr int THREADS = 192;
+constexpr int TILE = 128, TILE_K = 128, UMMA_K = 32, MAX_STAGES = 12, MAX_KS = 4;
+constexpr int THREADS = 320, EPILOGUE_WARPS = 8;
 constexpr int BOX_BYTES = TILE * TILE_K;  // 128 rows of an operand for one step
 
 #include "tcgen05.cuh"
@@ -61,8 +61,34 @@ struct Epilogue {
   int tile_n, stages, ks, n_tokens;
 };
 
-__device__ __forceinline__ float scaled(float acc, float s, const __nv_bfloat16* bias, int col) {
-  return fmaf(acc, s, bias ? __bfloat162float(bias[col]) : 0.f);
+// four sums times the scales of their row and columns (+ bias)
+__device__ __forceinline__ void scale4(float* v, float sx, const float* scales, const float* biases) {
+  const float4 s = *reinterpret_cast<const float4*>(scales);
+  float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (biases) b = *reinterpret_cast<const float4*>(biases);
+  v[0] = fmaf(v[0], sx * s.x, b.x);
+  v[1] = fmaf(v[1], sx * s.y, b.y);
+  v[2] = fmaf(v[2], sx * s.z, b.z);
+  v[3] = fmaf(v[3], sx * s.w, b.w);
+}
+// twice 16 columns of this thread's row (lane) of tensor memory: both loads are in flight before the one wait
+__device__ __forceinline__ void tmem_load_2x16(uint32_t taddr_a, uint32_t taddr_b, float* va, float* vb) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr_a), "r"(taddr_b)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    va[i] = __uint_as_float(r[i]);
+    vb[i] = __uint_as_float(r[16 + i]);
+  }
 }
 __device__ __forceinline__ void store16(const Epilogue& ep, const float* v, int row, int col0, int M) {
   if (!FMS_IN((size_t)row * ep.outputs + col0, (size_t)M * ep.outputs)) return;
@@ -97,17 +123,29 @@ __device__ __forceinline__ void store16(const Epilogue& ep, const float* v, int 
   }
 }
 
+// values of neighbouring rows of y, one column
+template <int N> __device__ __forceinline__ void store_column(const Epilogue& ep, const float* v, int row0, int col, int M, size_t pitch) {
+  const size_t at = (size_t)row0 * pitch + col;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (row0 + j < M && FMS_IN(at + j * pitch, (size_t)M * pitch)) {
+      if (ep.out_f32) ((float*)ep.out)[at + j * pitch] = v[j];
+      else ((__nv_bfloat16*)ep.out)[at + j * pitch] = __float2bfloat16_rn(v[j]);
+    }
+}
+
 // ---- many rows (prefill) --------------------------------------------------------------------------------------------
 // Persistent pairs of thread blocks (a cluster of two, cta_group::2): a pair owns a tile of 256 rows of x by TN rows of w, of
 // which each block brings 128 rows of x and half the rows of w (GLU: block 0 the gate rows, block 1 the up rows) into its own
 // shared memory.  What a multiprocessor takes in, 128 + TN / 2 bytes a k, against 2 * 128 * TN operations is what limits
 // tiles without a pair.  Two accumulators: the epilogue of a tile runs under the products of the next.
-//   warp 0 TMA, warp 1 (of block 0) the instructions, warps 2-5 the epilogue, 32 rows of this block's 128 each
+//   warp 0 TMA, warp 1 (of block 0) the instructions, warps 2-9 the epilogue: 32 rows of this block's 128 and every second
+//   16 columns each (with four warps the activation of GLU takes longer than the tile's products)
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     e4m3_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, Epilogue ep, int M,
                      int k_steps, int* __restrict__ error_flag) {
   extern __shared__ unsigned char smem_unaligned[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
+  unsigned char* smem = smem_unaligned + (-smem_u32(smem_unaligned) & 1023);
   const int b_rows = ep.tile_n / 2, stage_bytes = BOX_BYTES + b_rows * TILE_K, stages = ep.stages;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)stages * stage_bytes);
   uint64_t* empty = full + MAX_STAGES;
@@ -115,6 +153,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   uint64_t* acc_empty = acc_full + 2;       // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   __shared__ int failed_flag;
+  __shared__ __align__(16) float col_scales[EPILOGUE_WARPS][128], col_biases[EPILOGUE_WARPS][128];  // of a warp's columns of the tile; GLU: the up rows' behind
   volatile int* failed = &failed_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -132,7 +171,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 8);  // one arrival per epilogue warp of either block (used in block 0)
+      mbar_init(&acc_empty[a], 2 * EPILOGUE_WARPS);  // of either block (used in block 0)
     }
     mbar_fence_init();
   }
@@ -183,26 +222,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       }
     }
   } else {
-    const int quarter = warp & 3;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    float *scales = col_scales[warp - 2], *biases = col_biases[warp - 2];
     int j = 0;
     for (int tile = pair; tile < n_tiles; tile += pairs, ++j) {
       const int acc = j & 1;
       const int row = (tile % tiles_m) * 2 * TILE + (int)rank * TILE + quarter * 32 + lane, n0 = (tile / tiles_m) * tile_n;
       const float sx = row < M ? ep.sx[row] : 0.f;
+      // read from global memory in the loop below they would be waited for 16 columns at a time
+      __syncwarp();
+      for (int i = lane; i < 128; i += 32) {
+        const bool up = ep.glu && i >= 64;
+        const int at = up ? i - 64 : i, c = (at >> 4) * 32 + half * 16 + (at & 15);
+        const int col = min(n0 + c, ep.outputs - 1) + (up ? ep.outputs : 0);
+        scales[i] = ep.sw[col];
+        if (ep.bias) biases[i] = __bfloat162float(ep.bias[col]);
+      }
+      __syncwarp();
       if (!warp_wait(&acc_full[acc], (j >> 1) & 1, failed)) break;
       tc_fence_after();
       const uint32_t taddr = tmem + acc * 256 + ((uint32_t)(quarter * 32) << 16);
-      for (int c0 = 0; c0 < tile_n; c0 += 16) {  // every lane loads: tensor-memory loads are warp-wide
+      for (int c0 = half * 16; c0 < tile_n; c0 += 32) {  // every lane loads: tensor-memory loads are warp-wide
         float v[16], u[16];
-        const int col0 = n0 + c0;
-        if (ep.glu) tmem_load_16(taddr + tile_n + c0, u);
-        tmem_load_16(taddr + c0, v);
+        const int col0 = n0 + c0, at = c0 >> 5 << 4;
+        if (ep.glu) tmem_load_2x16(taddr + c0, taddr + tile_n + c0, v, u);
+        else tmem_load_16(taddr + c0, v);
         if (row >= M || col0 >= ep.outputs) continue;
 #pragma unroll
-        for (int jj = 0; jj < 16; ++jj) {
-          const int col = min(col0 + jj, ep.outputs - 1);
-          v[jj] = scaled(v[jj], sx * ep.sw[col], ep.bias, col);
-          if (ep.glu) v[jj] = activate(v[jj], ep.act) * scaled(u[jj], sx * ep.sw[ep.outputs + col], ep.bias, ep.outputs + col);
+        for (int q = 0; q < 4; ++q) {
+          scale4(v + 4 * q, sx, scales + at + 4 * q, ep.bias ? biases + at + 4 * q : nullptr);
+          if (ep.glu) {
+            scale4(u + 4 * q, sx, scales + 64 + at + 4 * q, ep.bias ? biases + 64 + at + 4 * q : nullptr);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * q + e] = activate(v[4 * q + e], ep.act) * u[4 * q + e];
+          }
         }
         store16(ep, v, row, col0, M);
       }
@@ -240,17 +293,18 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t local_addr, uint32_t
   return v;
 }
 
-__global__ void __launch_bounds__(THREADS) e4m3_rows_kernel(const __grid_constant__ CUtensorMap map_x,
+__global__ void __launch_bounds__(THREADS, 2) e4m3_rows_kernel(const __grid_constant__ CUtensorMap map_x,
                                                             const __grid_constant__ CUtensorMap map_w, Epilogue ep, int M,
                                                             int k_steps_all, int* __restrict__ error_flag) {
   extern __shared__ unsigned char smem_unaligned[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
+  unsigned char* smem = smem_unaligned + (-smem_u32(smem_unaligned) & 1023);
   const int stage_bytes = BOX_BYTES + ep.n_tokens * TILE_K, stages = ep.stages, ks = ep.ks;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)stages * stage_bytes);
   uint64_t* empty = full + MAX_STAGES;
   uint64_t* acc_full = empty + MAX_STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   __shared__ int failed_flag;
+  __shared__ float row_scales[256];  // of x: read from global memory they would be waited for four tokens at a time
   volatile int* failed = &failed_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -316,17 +370,23 @@ __global__ void __launch_bounds__(THREADS) e4m3_rows_kernel(const __grid_constan
       tc_commit(acc_full);  // arrives when everything issued so far is done (at once if there was nothing)
     }
   }
-  // This block's sums as float32 [128][n_tokens + 4] in shared memory, over the stages: every copy into them has landed and
-  // every instruction that read them is done once the accumulator is ready.
+  // The sums leave tensor memory as they are where a block has them whole and a thread's row of w is a column of y; else they meet
+  // in shared memory, as float32 [128][n_tokens + 4] over the stages (every copy into them has landed and every instruction
+  // that read them is done once the accumulator is ready).  Thread: a row of w, runs of 8 or 16 tokens.
   float* red = reinterpret_cast<float*>(smem);
-  const int red_stride = ep.n_tokens + 4;
+  const int red_stride = ep.n_tokens + 4, part = (warp - 2) >> 2;
+  const bool direct = ks == 1 && !ep.glu;
+  const size_t pitch = ep.outputs;
   if (warp >= 2) {
     pdl_wait();  // these warps read and write what other kernels touch (scales, the error flag, y)
-    const int quarter = warp & 3;
+    for (int t = threadIdx.x - 64; t < ep.n_tokens; t += 32 * EPILOGUE_WARPS) row_scales[t] = t < M ? ep.sx[t] : 0.f;
+    const int quarter = warp & 3, row = quarter * 32 + lane, col = n0 + row;
+    const bool live = col < ep.outputs;
+    const float sw = direct && live ? ep.sw[col] : 0.f, bias = direct && live && ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;
+    asm volatile("bar.sync 1, %0;\n" ::"n"(32 * EPILOGUE_WARPS) : "memory");
     const bool ok = warp_wait(acc_full, 0, failed);
     tc_fence_after();
-    const int row = quarter * 32 + lane;
-    for (int c0 = 0; c0 < ep.n_tokens; c0 += 16) {
+    for (int c0 = 16 * part; c0 < ep.n_tokens; c0 += 32) {
       float v[16];
       if (ok && k_steps > 0) {
         tmem_load_16(tmem + ((uint32_t)(quarter * 32) << 16) + c0, v);
@@ -334,54 +394,62 @@ __global__ void __launch_bounds__(THREADS) e4m3_rows_kernel(const __grid_constan
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = 0.f;
       }
+      if (!direct) {
 #pragma unroll
-      for (int j = 0; j < 16; j += 4)
-        *reinterpret_cast<float4*>(red + row * red_stride + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        for (int j = 0; j < 16; j += 4)
+          *reinterpret_cast<float4*>(red + row * red_stride + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      } else if (ok && live) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = fmaf(v[j], row_scales[c0 + j] * sw, bias);
+        store_column<16>(ep, v, c0, col, M, pitch);
+      }
     }
     tc_fence_before();
   }
-  __syncthreads();
-  if (ks > 1) cluster_sync_all();  // every block's sums are in its shared memory
-
-  if (warp >= 2 && !*failed) {  // this block's share of the tokens, four at a time; a thread keeps its row of w
-    const int e = threadIdx.x - 64, i = ep.glu ? e & 63 : e, step = ep.glu ? 8 : 4;
-    const int share = ((ep.n_tokens + ks - 1) / ks + 3) / 4 * 4;
-    const int t_hi = min((rank + 1) * share, ep.n_tokens), col = n0 + i;
-    const uint32_t red_addr = smem_u32(red);
-    auto total4 = [&](int row, int t, float* out) {
-      if (ks == 1) {
-        const float4 v = *reinterpret_cast<const float4*>(red + row * red_stride + t);
-        out[0] = v.x; out[1] = v.y; out[2] = v.z; out[3] = v.w;
-        return;
-      }
-      float4 v[MAX_KS];
-      const uint32_t at = red_addr + (uint32_t)(row * red_stride + t) * 4u;
+  if (!direct) {
+    __syncthreads();
+    if (ks > 1) cluster_sync_all();  // every block's sums are in its shared memory
+    if (warp >= 2 && !*failed) {     // this block's share of the tokens, 8 at a time
+      const int e = threadIdx.x - 64, i = ep.glu ? e & 63 : e & 127, col = n0 + i;
+      const int share = ((ep.n_tokens + ks - 1) / ks + 7) / 8 * 8, t_hi = min((rank + 1) * share, ep.n_tokens);
+      const bool live = col < ep.outputs;
+      const float sw = live ? ep.sw[col] : 0.f, su = live && ep.glu ? ep.sw[ep.outputs + col] : 0.f;
+      const float bias = live && ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;
+      const float bias_up = live && ep.glu && ep.bias ? __bfloat162float(ep.bias[ep.outputs + col]) : 0.f;
+      const uint32_t red_addr = smem_u32(red);
+      auto total8 = [&](int row, int t, float* out) {
+        float4 v[MAX_KS][2];
+        const uint32_t at = red_addr + (uint32_t)(row * red_stride + t) * 4u;
 #pragma unroll
-      for (int r = 0; r < MAX_KS; ++r)  // all loads on their way before the first sum
-        if (r < ks) v[r] = ld_cluster_f32x4(at, (uint32_t)r);
-      out[0] = out[1] = out[2] = out[3] = 0.f;
+        for (int r = 0; r < MAX_KS; ++r)  // all loads on their way before the first sum
+          if (r < ks) {
+            v[r][0] = ld_cluster_f32x4(at, (uint32_t)r);
+            v[r][1] = ld_cluster_f32x4(at + 16, (uint32_t)r);
+          }
 #pragma unroll
-      for (int r = 0; r < MAX_KS; ++r)
-        if (r < ks) {
-          out[0] += v[r].x; out[1] += v[r].y; out[2] += v[r].z; out[3] += v[r].w;
+        for (int j = 0; j < 8; ++j) out[j] = 0.f;
+#pragma unroll
+        for (int r = 0; r < MAX_KS; ++r)
+          if (r < ks) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              out[4 * h] += v[r][h].x; out[4 * h + 1] += v[r][h].y; out[4 * h + 2] += v[r][h].z; out[4 * h + 3] += v[r][h].w;
+            }
+          }
+      };
+      const int step = 32 * EPILOGUE_WARPS / (ep.glu ? 64 : 128) * 8;
+      for (int t = rank * share + 8 * (ep.glu ? e >> 6 : e >> 7); t < t_hi; t += step) {
+        float v[8], u[8];
+        total8(i, t, v);
+        if (ep.glu) total8(64 + i, t, u);
+        if (!live) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float sx = row_scales[t + j];
+          v[j] = fmaf(v[j], sx * sw, bias);
+          if (ep.glu) v[j] = activate(v[j], ep.act) * fmaf(u[j], sx * su, bias_up);
         }
-    };
-    const bool live = col < ep.outputs;
-    const float sw = live ? ep.sw[col] : 0.f, su = live && ep.glu ? ep.sw[ep.outputs + col] : 0.f;
-    for (int t = rank * share + (ep.glu ? 4 * (e >> 6) : 0); t < t_hi; t += step) {
-      float v[4], u[4];
-      total4(i, t, v);
-      if (ep.glu) total4(64 + i, t, u);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (t + j >= M || !live) continue;
-        const float sx = ep.sx[t + j];
-        float y = scaled(v[j], sx * sw, ep.bias, col);
-        if (ep.glu) y = activate(y, ep.act) * scaled(u[j], sx * su, ep.bias, ep.outputs + col);
-        const size_t at = (size_t)(t + j) * ep.outputs + col;
-        if (!FMS_IN(at, (size_t)M * ep.outputs)) continue;
-        if (ep.out_f32) ((float*)ep.out)[at] = y;
-        else ((__nv_bfloat16*)ep.out)[at] = __float2bfloat16_rn(y);
+        store_column<8>(ep, v, t, col, M, pitch);
       }
     }
   }
@@ -435,10 +503,10 @@ int choose_tile_n(int tiles_m, int cols, bool glu, int pairs) {
   return best;
 }
 
-// Blocks that share a tile: from the weights' shape alone, enough for two blocks a multiprocessor, at least 4 steps a block
+// Blocks that share a tile: from the weights' shape alone, as many as fill most of the multiprocessors, each with 4 steps at least
 int choose_ks(int tiles, int k_steps) {
   int ks = 1;
-  while (ks < MAX_KS && tiles * ks * 2 <= 320 && k_steps / (ks * 2) >= 4) ks *= 2;
+  while (ks < 4 && tiles * ks < 120 && k_steps / (ks * 2) >= 4) ks *= 2;
   return ks;
 }
 
