@@ -1,15 +1,18 @@
 // y[m, n] = sum_k x[m, k] * (q[n, k] - z[n, g(k)]) * s[n, g(k)] (+ bias[n]): bfloat16 rows, weights of 4 bits with one bfloat16
 // scale and one whole zero point a group of consecutive k.  GLU: act(gate) * up for weights [gate; up].
 //
-// Layout, made once (kernels/quantized.py, pack_int4).  Weights: blocks of 16 rows x 128 k, 1,024 bytes each, [rows / 16]
-// [k / 128][16 rows][4 pieces of 16 bytes]; word w of a row's piece c holds k = 32 w + 8 c .. + 7, value 2 i in bits 4 i and
-// value 2 i + 1 in bits 16 + 4 i, so that one shift and one logical operation leave a pair of neighbours in the halves of a
-// register; piece c lies at place c ^ (row / 2 % 4), which lets the rows of a warp read a piece from shared memory without
-// meeting in a bank.  Groups: [groups][N] words, the scale in the low half and 128 + z, exact in bfloat16, in the high half.
+// Layout, made once (kernels/quantized.py, pack_int4): one stream of blocks of 16 rows x 128 k, [rows / 16][k / 128], each
+//   1,024 bytes of weights: [16 rows][4 pieces of 16 bytes]; word w of a row's piece c holds k = 32 w + 8 c .. + 7, value 2 i in
+//     bits 4 i and value 2 i + 1 in bits 16 + 4 i, so that one shift and one logical operation leave a pair of neighbours in
+//     the halves of a register; piece c lies at place c ^ (row / 2 % 4), which lets the rows of a warp read a piece from shared
+//     memory without meeting in a bank;
+//   PER times 64 bytes (PER 1, 2 or 4, by whether groups are whole blocks, halves or quarters of them): a word a row, the scale in
+//     its low half and 128 + z, exact in bfloat16, in its high half.
+// So all that a tile needs of a block comes in one copy of neighbouring bytes, and groups cost no index arithmetic.
 //
 // 0x4300 | q is the bfloat16 128 + q; minus 128 + z it is q - z, exact.
 //   few rows: mma.sync over q - z, whole numbers, a group's float32 sum times its scale: nothing is rounded but the result.
-//   more rows: tcgen05 over (q - z) * s rounded to bfloat16 on its way into the operand, as the bfloat16 weight would be: the
+//   more rows: tcgen05 over (q - z) * s rounded to bfloat16 on its way into the operand, as a bfloat16 weight would be: the
 //             tensor cores' sums run over all of k and cannot be scaled group by group.
 #include <cuda.h>
 
@@ -18,7 +21,7 @@
 namespace {
 #include "tcgen05.cuh"
 
-constexpr int BLOCK_ROWS = 16, BLOCK_K = 128, BLOCK_BYTES = 1024;
+constexpr int BLOCK_ROWS = 16, BLOCK_K = 128, WEIGHT_BYTES = 1024;
 
 __device__ __forceinline__ float activate(float g, int act) {
   switch (act) {
@@ -33,253 +36,243 @@ __device__ __forceinline__ float activate(float g, int act) {
 __device__ __forceinline__ void unpack8(uint32_t word, __nv_bfloat162 zero, uint32_t* pairs) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t v = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    uint32_t v;  // (word >> 4 i) & 0x000f000f | 0x43004300 as one logical operation
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(v) : "r"(word >> (4 * i)), "r"(0x000f000fu), "r"(0x43004300u));
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), zero);
     pairs[i] = *reinterpret_cast<const uint32_t*>(&d);
   }
 }
-__device__ __forceinline__ __nv_bfloat162 both(uint32_t half) {
-  const uint32_t v = __byte_perm(half, half, 0x1010);
+// a group's word: 128 + z and the scale, each in both halves of a register
+__device__ __forceinline__ __nv_bfloat162 zero_of(uint32_t word) {
+  const uint32_t v = __byte_perm(word, word, 0x3232);
+  return *reinterpret_cast<const __nv_bfloat162*>(&v);
+}
+__device__ __forceinline__ __nv_bfloat162 scale_of(uint32_t word) {
+  const uint32_t v = __byte_perm(word, word, 0x1010);
   return *reinterpret_cast<const __nv_bfloat162*>(&v);
 }
 
 struct Int4Args {
   const __nv_bfloat16* x;     // [M, K]
   const unsigned char* w;     // the packed blocks
-  const uint32_t* groups;     // [n_groups, N]
   const __nv_bfloat16* bias;  // [N] or null
   __nv_bfloat16* y;           // [M, outputs]
-  int M, N, K, k_blocks, n_groups, group, outputs, act;
+  int M, N, K, k_blocks, per, outputs, act;
+  __host__ __device__ int block_bytes() const { return WEIGHT_BYTES + 64 * per; }
+  __host__ __device__ int row_blocks() const { return (N + BLOCK_ROWS - 1) / BLOCK_ROWS; }
 };
 
-// ---- up to 16 rows ------------------------------------------------------------------------------------------------------
-// Bound by reading the weights once.  A block of 8 warps owns RT tiles of 16 rows of w (GLU: 8 gate rows and the 8 up rows that
-// belong to them); the warps take the 128-k blocks in turn and add their sums in shared memory in a fixed order.  A lane
-// copies what it needs (its piece of two rows, of the x rows, the groups' words) into a ring that only it reads, D blocks ahead.
-// PER: scales a block of 128 k (1: groups of whole blocks; 2: of 64 k; 4: any multiple of 32).
-constexpr int WARPS = 8, THREADS = 256;
+// Asks for a kernel's shared memory once on every device.
+template <typename Kernel> int allow_smem(Kernel kernel, int bytes, uint64_t* done) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && device < 64 && (*done >> device & 1)) return 0;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fms_fail("gemm_int4: %d bytes of shared memory refused: %s", bytes, cudaGetErrorString(e));
+  if (device < 64) *done |= 1ull << device;
+  return 0;
+}
+int multiprocessors() {
+  static int sms = 0;
+  if (sms == 0) {
+    int device = 0;
+    cudaGetDevice(&device);
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) sms = 148;
+  }
+  return sms;
+}
 
+// ---- up to 8 rows -------------------------------------------------------------------------------------------------------
+// Bound by reading the weights once, and by the instructions that unpack them (some 190 for 16 rows x 128 k).  Persistent thread
+// blocks take 16 rows of w at a time (GLU: the gate rows and then the up rows that belong to them); their warps share the 128-k
+// blocks and add their sums in shared memory in a fixed order, into one of two buffers in turn, so that a tile costs one barrier
+// and the loads of the next go on across it.  A lane loads its pieces of two rows of a block straight into registers, AHEAD
+// blocks ahead; x comes from the first-level cache.  (28,672 x 4,096 by one row 17.0 us; with rings in shared memory fed by bulk
+// copies 22.7, which take 110 cycles a block, and by asynchronous copies of each lane's own 19.6, for the instructions they cost.)
+constexpr int FEW_ROWS = 8, AHEAD = 2;
+
+__device__ __forceinline__ void mma_bf16_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_bf16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void cp_async16(void* smem, const void* gmem, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
-__device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_u32(smem)), "l"(gmem) : "memory");
+__device__ __forceinline__ uint32_t load_once(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];\n" : "=r"(v) : "l"(p));
+  return v;
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
-template <int NT, int RT, int PER, bool GLU, int D>
-__global__ void __launch_bounds__(THREADS) int4_few_rows_kernel(Int4Args p) {
-  constexpr int WL = RT * 2, XL = NT * 4, LOADS = WL + XL, GL = RT * 2 * PER;
-  constexpr int TILE_ROWS = GLU ? 8 : 16;
-  extern __shared__ uint4 ring[];
-  uint32_t* group_ring = reinterpret_cast<uint32_t*>(ring + (size_t)D * LOADS * THREADS);
+template <int PER, bool GLU>
+__global__ void __launch_bounds__(1024, 1) int4_few_rows_kernel(Int4Args p) {
+  constexpr int BYTES = WEIGHT_BYTES + 64 * PER;
+  extern __shared__ float4 red[];  // [2][warps][32]
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-
-  const unsigned char* wp[RT][2];
-  const uint32_t* gp[RT][2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, c = lane & 3;
+  // GLU: tile 2 i is gate block i, tile 2 i + 1 the up block that belongs to it, both of this thread block
+  const int out_blocks = (p.outputs + BLOCK_ROWS - 1) / BLOCK_ROWS, up = p.outputs / BLOCK_ROWS;
+  const int mine = (out_blocks - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * (GLU ? 2 : 1);
+  auto block_of = [&](int j) {  // the rows of tile j of this thread block
+    return GLU ? (int)(blockIdx.x + (j >> 1) * gridDim.x) + (j & 1) * up : (int)(blockIdx.x + j * gridDim.x);
+  };
+  // what this warp loads next: block `next_kb` of tile `next_j`, at the lane's pieces (those of rows g and g + 8 lie 512 bytes apart)
+  const int piece = g * 64 + (c ^ ((g >> 1) & 3)) * 16, word = WEIGHT_BYTES + g * 4 - piece;
+  int next_j = 0, next_kb = warp;
+  const unsigned char* next = p.w + ((size_t)block_of(0) * p.k_blocks + warp) * BYTES + piece;
+  uint4 w[AHEAD][2];
+  uint32_t gw[AHEAD][2 * PER];
+  auto load = [&](int at) {
+    if (next_j >= mine) return;
+    w[at][0] = load_once(reinterpret_cast<const uint4*>(next));
+    w[at][1] = load_once(reinterpret_cast<const uint4*>(next + 512));
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = (blockIdx.x * RT + t) * TILE_ROWS + g;
-      const int row = min(GLU ? r + h * p.outputs : r + 8 * h, p.N - 1);
-      wp[t][h] = p.w + ((size_t)(row / BLOCK_ROWS) * p.k_blocks) * BLOCK_BYTES + (row % BLOCK_ROWS) * 64 + ((c ^ ((row >> 1) & 3)) * 16);
-      gp[t][h] = p.groups + row;
+    for (int u = 0; u < 2 * PER; ++u) gw[at][u] = load_once(reinterpret_cast<const uint32_t*>(next + word + u * 32));
+    next += (size_t)warps * BYTES;
+    next_kb += warps;
+    if (next_kb >= p.k_blocks) {
+      next_kb = warp;
+      if (++next_j < mine) next = p.w + ((size_t)block_of(next_j) * p.k_blocks + warp) * BYTES + piece;
     }
-  const __nv_bfloat16* xp[NT];
-  bool xok[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    xok[j] = j * 8 + g < p.M;
-    xp[j] = p.x + (size_t)(xok[j] ? j * 8 + g : 0) * p.K + 8 * c;
-  }
-  const int mine = p.k_blocks > warp ? (p.k_blocks - warp + WARPS - 1) / WARPS : 0;
-  auto issue_w = [&](int i) {
-    if (i >= mine) return;
-    const int kb = warp + i * WARPS;
-    uint4* st = ring + (size_t)(i % D) * LOADS * THREADS + threadIdx.x;
-    uint32_t* gs = group_ring + (size_t)(i % D) * GL * THREADS + threadIdx.x;
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        cp_async16(st + (t * 2 + h) * THREADS, wp[t][h] + (size_t)kb * BLOCK_BYTES, true);
-#pragma unroll
-        for (int u = 0; u < PER; ++u) {
-          const int at = min((kb * BLOCK_K + u * (BLOCK_K / PER)) / p.group, p.n_groups - 1);
-          cp_async4(gs + ((t * 2 + h) * PER + u) * THREADS, gp[t][h] + (size_t)at * p.N);
-        }
-      }
   };
-  auto issue_x = [&](int i) {
-    if (i >= mine) return;
-    const int k0 = (warp + i * WARPS) * BLOCK_K;
-    uint4* st = ring + ((size_t)(i % D) * LOADS + WL) * THREADS + threadIdx.x;
+  const int n = warp < p.k_blocks ? (p.k_blocks - warp + warps - 1) / warps : 0;  // blocks of a tile for this warp
+  if (n == 0) next_j = mine;
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {  // K is a multiple of 8: a lane's 8 values are all inside or all outside
-        const bool in = xok[j] && k0 + 32 * u + 8 * c < p.K;
-        cp_async16(st + (j * 4 + u) * THREADS, xp[j] + (in ? k0 + 32 * u : 0), in);
-      }
-  };
-  float acc[RT][NT][4];
-#pragma unroll
-  for (int t = 0; t < RT; ++t)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[t][j][e] = 0.f;
-#pragma unroll
-  for (int i = 0; i < D; ++i) issue_w(i);  // weights: before the wait for the kernel that makes x
+  for (int q = 0; q < AHEAD; ++q) load(q);  // weights: before the wait for the kernel that makes x
+  // a lane without a row of x of its own reads the first: its sums are not stored
+  const __nv_bfloat16* xp = p.x + (size_t)(g < p.M ? g : 0) * p.K + 8 * c;
   pdl_wait();
+
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, gate = 0.f;
+  auto multiply = [&](const uint4* wq, const uint32_t* gq, int kb) {
+    uint4 b[4];
+    const int left = p.K - kb * BLOCK_K;  // K is a multiple of 8: a lane's 8 values are all inside or all outside
+    const uint4* xs = reinterpret_cast<const uint4*>(xp + (size_t)kb * BLOCK_K);
+    if (left >= BLOCK_K) {
 #pragma unroll
-  for (int i = 0; i < D; ++i) {
-    issue_x(i);
-    cp_async_commit();  // the first group holds all stages' weights
-  }
-  for (int i = 0; i < mine; ++i) {
-    cp_async_wait<D - 1>();
-    const uint4* st = ring + (size_t)(i % D) * LOADS * THREADS + threadIdx.x;
-    const uint32_t* gs = group_ring + (size_t)(i % D) * GL * THREADS + threadIdx.x;
-    uint4 b[NT][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) b[j][u] = st[(WL + j * 4 + u) * THREADS];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const uint4 lo = st[(t * 2) * THREADS], hi = st[(t * 2 + 1) * THREADS];
-      const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        const uint32_t gl = gs[((t * 2) * PER + u) * THREADS], gh = gs[((t * 2 + 1) * PER + u) * THREADS];
-        const __nv_bfloat162 zl = both(gl >> 16), zh = both(gh >> 16);
-        float part[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) part[j][e] = 0.f;
-#pragma unroll
-        for (int v = u * (4 / PER); v < (u + 1) * (4 / PER); ++v) {
-          uint32_t a[4], d[4];
-          unpack8(wl[v], zl, a);
-          unpack8(wh[v], zh, d);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            mma_bf16(part[j], a[0], d[0], a[1], d[1], b[j][v].x, b[j][v].y);
-            mma_bf16(part[j], a[2], d[2], a[3], d[3], b[j][v].z, b[j][v].w);
-          }
-        }
-        const float sl = __uint_as_float(gl << 16), sh = __uint_as_float(gh << 16);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          acc[t][j][0] = fmaf(part[j][0], sl, acc[t][j][0]);
-          acc[t][j][1] = fmaf(part[j][1], sl, acc[t][j][1]);
-          acc[t][j][2] = fmaf(part[j][2], sh, acc[t][j][2]);
-          acc[t][j][3] = fmaf(part[j][3], sh, acc[t][j][3]);
-        }
-      }
-    }
-    issue_w(i + D);  // into the stage just consumed
-    issue_x(i + D);
-    cp_async_commit();
-  }
-  cp_async_wait<0>();
-  __syncthreads();  // the ring is free: the warps' sums go over it
-  float* red = reinterpret_cast<float*>(ring);  // [WARPS][RT * NT][32][4]
-#pragma unroll
-  for (int t = 0; t < RT; ++t)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-      *reinterpret_cast<float4*>(red + ((warp * RT * NT + t * NT + j) * 32 + lane) * 4) =
-          make_float4(acc[t][j][0], acc[t][j][1], acc[t][j][2], acc[t][j][3]);
-  __syncthreads();
-  auto total = [&](int t, int j, int l, int e) {
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) s += red[((w * RT * NT + t * NT + j) * 32 + l) * 4 + e];
-    return s;
-  };
-  // element e of lane l is (row l / 4 + 8 (e / 2) of the tile, row 2 (l % 4) + e % 2 of x); neighbouring threads take neighbouring rows of w
-  constexpr int ITEMS = RT * NT * 8 * TILE_ROWS;
-  for (int i = threadIdx.x; i < ITEMS; i += THREADS) {
-    const int r = i % TILE_ROWS, t = i / TILE_ROWS % RT, mm = i / (TILE_ROWS * RT), j = mm / 8, m = mm % 8;
-    const int col = (blockIdx.x * RT + t) * TILE_ROWS + r, l = (r & 7) * 4 + (m >> 1), e = m & 1;
-    if (col >= p.outputs || mm >= p.M) continue;
-    float v;
-    if (GLU) {
-      float gate = total(t, j, l, e), up = total(t, j, l, e + 2);
-      if (p.bias) {
-        gate += __bfloat162float(p.bias[col]);
-        up += __bfloat162float(p.bias[p.outputs + col]);
-      }
-      v = activate(gate, p.act) * up;
+      for (int u = 0; u < 4; ++u) b[u] = __ldg(xs + 4 * u);
     } else {
-      v = total(t, j, l, e + 2 * (r >> 3));
-      if (p.bias) v += __bfloat162float(p.bias[col]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) b[u] = left > 32 * u + 8 * c ? __ldg(xs + 4 * u) : make_uint4(0, 0, 0, 0);
     }
-    if (FMS_IN((size_t)mm * p.outputs + col, (size_t)p.M * p.outputs)) p.y[(size_t)mm * p.outputs + col] = __float2bfloat16_rn(v);
+    const uint32_t wl[4] = {wq[0].x, wq[0].y, wq[0].z, wq[0].w}, wh[4] = {wq[1].x, wq[1].y, wq[1].z, wq[1].w};
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const uint32_t gl = gq[2 * u], gh = gq[2 * u + 1];
+      const __nv_bfloat162 zl = zero_of(gl), zh = zero_of(gh);
+      float part[4];
+#pragma unroll
+      for (int v = u * (4 / PER); v < (u + 1) * (4 / PER); ++v) {
+        uint32_t a[4], d[4];
+        unpack8(wl[v], zl, a);
+        unpack8(wh[v], zh, d);
+        if (v == u * (4 / PER)) mma_bf16_first(part, a[0], d[0], a[1], d[1], b[v].x, b[v].y);
+        else mma_bf16(part, a[0], d[0], a[1], d[1], b[v].x, b[v].y);
+        mma_bf16(part, a[2], d[2], a[3], d[3], b[v].z, b[v].w);
+      }
+      const float sl = __uint_as_float(gl << 16), sh = __uint_as_float(gh << 16);
+      acc[0] = fmaf(part[0], sl, acc[0]);
+      acc[1] = fmaf(part[1], sl, acc[1]);
+      acc[2] = fmaf(part[2], sh, acc[2]);
+      acc[3] = fmaf(part[3], sh, acc[3]);
+    }
+  };
+  auto finish = [&](int j) {  // all warps have their sums of tile j
+    float4* sums = red + (size_t)(j & 1) * warps * 32;
+    sums[warp * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+    __syncthreads();
+    // thread: element e of lane l, which is (row l / 4 + 8 (e / 2) of the tile, row 2 (l % 4) + e % 2 of x)
+    for (int t = threadIdx.x; t < 128; t += blockDim.x) {
+      const int l = t >> 2, e = t & 3, m = 2 * (l & 3) + (e & 1), col = block_of(GLU ? j & ~1 : j) * BLOCK_ROWS + (l >> 2) + 8 * (e >> 1);
+      if (m >= p.M || col >= p.outputs) continue;
+      float v = p.bias ? __bfloat162float(p.bias[GLU && (j & 1) ? p.outputs + col : col]) : 0.f, total = 0.f;
+      for (int i = 0; i < warps; ++i) total += reinterpret_cast<const float*>(sums + i * 32)[t];
+      v += total;
+      if (GLU && !(j & 1)) {
+        gate = v;  // at least 128 threads: the same one finishes the up rows
+        continue;
+      }
+      if (GLU) v = activate(gate, p.act) * v;
+      if (FMS_IN((size_t)m * p.outputs + col, (size_t)p.M * p.outputs)) p.y[(size_t)m * p.outputs + col] = __float2bfloat16_rn(v);
+    }
+  };
+  int i = 0, j = 0;  // block of the tile, tile
+  if (n == 0) {
+    for (; j < mine; ++j) finish(j);
+    return;
+  }
+  while (j < mine) {
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q)
+      if (j < mine) {  // of the whole warp
+        multiply(w[q], gw[q], warp + i * warps);
+        load(q);
+        if (++i == n) {
+          i = 0;
+          finish(j++);
+        }
+      }
   }
 }
 
-// Asks for a kernel's shared memory once on every device.
-template <typename Kernel> int allow_smem(const char* what, Kernel kernel, int bytes, uint64_t* done) {
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess && device < 64 && (*done >> device & 1)) return 0;
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return fms_fail("%s: %d bytes of shared memory refused: %s", what, bytes, cudaGetErrorString(e));
-  if (device < 64) *done |= 1ull << device;
-  return 0;
-}
-
-template <int NT, int RT, int PER, bool GLU> int launch_few(const Int4Args& p, cudaStream_t stream) {
-  constexpr int STAGE = (RT * 2 + NT * 4) * THREADS * 16 + RT * 2 * PER * THREADS * 4;
-  constexpr int D = STAGE * 4 <= 100 * 1024 ? 4 : 3;
-  constexpr int RED = WARPS * RT * NT * 32 * 16;
-  constexpr int SMEM = STAGE * D > RED ? STAGE * D : RED;
-  static_assert(SMEM <= 227 * 1024, "shared memory");
-  auto kernel = int4_few_rows_kernel<NT, RT, PER, GLU, D>;
-  static uint64_t allowed = 0;
-  if (allow_smem("gemm_int4", kernel, SMEM, &allowed)) return 1;
-  const int rows = RT * (GLU ? 8 : 16);
-  fms_launch(kernel, dim3((p.outputs + rows - 1) / rows), dim3(THREADS), SMEM, stream, p);
+template <int PER, bool GLU> int launch_few(const Int4Args& p, int warps, int grid, cudaStream_t stream) {
+  const int smem = 2 * warps * 32 * (int)sizeof(float4);  // 32 KB at most
+  fms_launch(int4_few_rows_kernel<PER, GLU>, dim3(grid), dim3(32 * warps), smem, stream, p);
   return fms_launch_status("gemm_int4");
 }
-template <int NT, int RT, bool GLU> int launch_few_per(const Int4Args& p, cudaStream_t stream) {
-  if (p.group % 128 == 0 || p.n_groups == 1) return launch_few<NT, RT, 1, GLU>(p, stream);
-  return p.group % 64 == 0 ? launch_few<NT, RT, 2, GLU>(p, stream) : launch_few<NT, RT, 4, GLU>(p, stream);
-}
 template <bool GLU> int few(const Int4Args& p, cudaStream_t stream) {
-  // two tiles a block share the rows of x, where that still leaves two blocks a multiprocessor
-  const int tiles = (p.outputs + (GLU ? 7 : 15)) / (GLU ? 8 : 16);
-  if (p.M <= 8) return tiles >= 592 ? launch_few_per<1, 2, GLU>(p, stream) : launch_few_per<1, 1, GLU>(p, stream);
-  return tiles >= 592 ? launch_few_per<2, 2, GLU>(p, stream) : launch_few_per<2, 1, GLU>(p, stream);
+  // 32 warps a multiprocessor, as thread blocks of 8, 16 or 32: the cut whose rounds of tiles, each as long as its warps' blocks of k
+  // and a barrier, take least (8 / 16 / 32 warps in us: 28,672 x 4,096 17.1 / 17.6 / 20.6, 4,096 x 14,336 17.2 / 9.3 / 10.1,
+  // 6,144 x 4,096 6.3 / 6.0 / 5.8, 4,096 x 4,096 6.1 / 3.7 / 4.4)
+  const int sms = multiprocessors(), tiles = (p.outputs + BLOCK_ROWS - 1) / BLOCK_ROWS;
+  int best = 0, warps = 32;
+  for (int w = 8; w <= 32; w *= 2) {
+    const int slots = sms * (32 / w), cost = (tiles + slots - 1) / slots * (GLU ? 2 : 1) * ((p.k_blocks + w - 1) / w + 1);
+    if (best == 0 || cost < best) {
+      best = cost;
+      warps = w;
+    }
+  }
+  const int slots = sms * (32 / warps), grid = tiles < slots ? tiles : slots;
+  return p.per == 1 ? launch_few<1, GLU>(p, warps, grid, stream)
+                    : (p.per == 2 ? launch_few<2, GLU>(p, warps, grid, stream) : launch_few<4, GLU>(p, warps, grid, stream));
 }
 
-// ---- more rows ----------------------------------------------------------------------------------------------------------
-// The weights fill the instruction's 128 rows, as its A operand in tensor memory, where the threads that unpack them put them: lane =
-// row of w, a pair of k a column.  The tokens (16 to 256) are its columns, B, brought by TMA.  So the weights cross shared
-// memory once, as 4 bits, and the instruction reads x alone from there.
-//   warp 0     per step of 128 k: two 64-k boxes of x and eight 1,024-byte blocks of w, into one of up to 8 stages
-//   warp 1     one lane issues 8 instructions (128 x tokens x 16) a step
-//   warps 2-9  two groups of four unpack every second step each, a thread a row of w, into the group's half of the operand
-//   warps 2-5  then read the accumulator; the ks blocks of a tile (a cluster) add their sums through distributed shared memory
-constexpr int ROWS_THREADS = 320, TILE = 128, MAX_STAGES = 8, MAX_KS = 8, A_COLUMNS = 64;
+// ---- what the tcgen05 kernels share --------------------------------------------------------------------------------------
+// The weights fill the instruction's rows, as its A operand in tensor memory, where the threads that unpack them put them: lane =
+// row of w, a pair of k a column.  The tokens are its columns, B, brought by TMA.  So the weights cross shared memory once, as 4
+// bits, and the instruction reads x alone from there; a thread's row of w is a column of y, and a warp stores 64 neighbouring bytes.
+constexpr int TILE = 128, A_COLUMNS = 64;  // columns of the operand for 128 k
 
-struct RowsArgs {
-  Int4Args p;
-  int n_tokens, stages, ks, acc_columns, tmem_columns, per;
-};
-
+// The packed blocks [row_blocks][k_blocks][bytes], in boxes of the eight row blocks of a tile by one k block: one copy a step (eight
+// untiled ones of a block each took 900 cycles)
+int make_block_map(CUtensorMap* map, const Int4Args& p) {
+  EncodeTiled enc = encode_tiled();
+  if (enc == nullptr) return fms_fail("gemm_int4: the driver does not export cuTensorMapEncodeTiled");
+  const cuuint64_t bytes = p.block_bytes();
+  const cuuint64_t dims[3] = {bytes / 8, (cuuint64_t)p.k_blocks, (cuuint64_t)p.row_blocks()}, strides[2] = {bytes, bytes * p.k_blocks};
+  const cuuint32_t box[3] = {(cuuint32_t)bytes / 8, 1, TILE / BLOCK_ROWS}, elem[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT64, 3, const_cast<unsigned char*>(p.w), dims, strides, box, elem,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fms_fail("gemm_int4: cuTensorMapEncodeTiled failed with %d (%d rows, %d k)", (int)r, p.N, p.K);
+  return 0;
+}
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, int c0, int c1, int c2, void* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n" ::"r"(
+                   smem_u32(smem_dst)),
+               "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
 // by a whole warp, which gives up as one
 __device__ __forceinline__ bool warp_wait(void* bar, uint32_t parity, volatile int* failed) {
   return __all_sync(0xffffffffu, wait_or_abort(bar, parity, failed));
@@ -293,6 +286,7 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t local_addr, uint32_t
       : "memory");
   return v;
 }
+// 32 columns of 32 bits of this thread's lane of tensor memory, written; not waited for
 __device__ __forceinline__ void tmem_store_pairs(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
@@ -303,27 +297,103 @@ __device__ __forceinline__ void tmem_store_pairs(uint32_t taddr, const uint32_t*
       "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+// 64 k of a row as 32 columns: words 2 h and 2 h + 1 of its four pieces, with the groups' words of either
+__device__ __forceinline__ void unpack64(const uint2* words, uint32_t group0, uint32_t group1, uint32_t* col) {
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    const uint32_t gw = v ? group1 : group0;
+    const __nv_bfloat162 zero = zero_of(gw), scale = scale_of(gw);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint32_t* to = col + v * 16 + c * 4;
+      unpack8(v ? words[c].y : words[c].x, zero, to);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&to[e]), scale);
+        to[e] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+    }
+  }
+}
+// the group's word of sub-block u (32 k) of a row
+__device__ __forceinline__ uint32_t group_word(const unsigned char* block, int row16, int u, int per) {
+  return reinterpret_cast<const uint32_t*>(block + WEIGHT_BYTES)[(u * per >> 2) * 16 + row16];
+}
+// A warp's 32 rows of a tile's blocks, 128 k, into 64 columns of tensor memory, of which a warp reaches the 32 lanes of its number's
+// rest by 4; done, and in order before what the first lane says next, when it returns.
+__device__ __forceinline__ void unpack_row(const unsigned char* blocks, int bytes, int per, int quarter, int lane, uint32_t tmem_a) {
+  tc_fence_after();
+  const int row = quarter * 32 + lane;
+  const uint32_t to = tmem_a + ((uint32_t)(quarter * 32) << 16);
+  const unsigned char* block = blocks + (row >> 4) * bytes;
+  const uint4* at = reinterpret_cast<const uint4*>(block + (row & 15) * 64);
+  uint4 piece[4];
+  uint32_t g[4], col[32];
+  uint2 words[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    piece[c] = at[c ^ ((row >> 1) & 3)];
+    g[c] = group_word(block, row & 15, c, per);
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) words[c] = make_uint2(piece[c].x, piece[c].y);
+  unpack64(words, g[0], g[1], col);
+  tmem_store_pairs(to, col);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) words[c] = make_uint2(piece[c].z, piece[c].w);
+  unpack64(words, g[2], g[3], col);
+  tmem_store_pairs(to + 32, col);
+  tmem_wait_stores();
+  tc_fence_before();
+  __syncwarp();
+}
+// values of neighbouring rows of y, one column
+template <int N> __device__ __forceinline__ void store_column(const Int4Args& p, const float* v, int row0, int col, float bias) {
+  const size_t pitch = p.N, at = (size_t)row0 * pitch + col;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (row0 + j < p.M && FMS_IN(at + j * pitch, (size_t)p.M * pitch)) p.y[at + j * pitch] = __float2bfloat16_rn(v[j] + bias);
+}
 
-__global__ void __launch_bounds__(ROWS_THREADS) int4_rows_kernel(const __grid_constant__ CUtensorMap map_x, RowsArgs a,
-                                                                 int* __restrict__ error_flag) {
+// ---- 9 to 256 rows -----------------------------------------------------------------------------------------------------
+//   warp 0      per step of 128 k: two 64-k boxes of x and one of the eight blocks of w, into one of up to 8 stages
+//   warp 1      one lane issues 8 instructions (128 x tokens x 16) a step
+//   warps 2-17  up to four groups of four unpack every fourth step each, a thread a row of w, into the group's quarter of the
+//               operand's 256 columns (two groups took 2,500 cycles a step, most of it waiting for one another); then they
+//               read the accumulator.  A group waits for its columns before it waits for a step's copies: the steps up to its last
+//               one are used up then, and with no more groups than stages the copies' barrier cannot be a phase behind.  The ks blocks of a tile (a cluster) add their sums through distributed shared memory.
+// Every wait on an mbarrier is bounded: on a time-out the block records error 4, skips the rest of its work and still meets
+// the cluster's barriers and frees its tensor memory.
+constexpr int GROUPS = 4, UNPACK_WARPS = 4 * GROUPS, ROWS_THREADS = 64 + 32 * UNPACK_WARPS, MAX_STAGES = 8, MAX_KS = 4, A_FIRST = 256;
+
+struct RowsArgs {
+  Int4Args p;
+  int n_tokens, stages, ks, groups;
+};
+
+__global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid_constant__ CUtensorMap map_x,
+                                                                    const __grid_constant__ CUtensorMap map_w, RowsArgs a,
+                                                                    int* __restrict__ error_flag) {
   extern __shared__ unsigned char smem_unaligned[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_unaligned + 1023) & ~(uintptr_t)1023);
+  unsigned char* smem = smem_unaligned + (-smem_u32(smem_unaligned) & 1023);
   const Int4Args& p = a.p;
-  const int x_bytes = a.n_tokens * BLOCK_K * 2, stage_bytes = x_bytes + TILE / BLOCK_ROWS * BLOCK_BYTES, stages = a.stages, ks = a.ks;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)stages * stage_bytes);
+  const int bytes = p.block_bytes(), x_bytes = a.n_tokens * BLOCK_K * 2, stages = a.stages, ks = a.ks;
+  const int stage_bytes = (x_bytes + TILE / BLOCK_ROWS * bytes + 1023) / 1024 * 1024;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + stages * stage_bytes);
   uint64_t* empty = full + MAX_STAGES;
-  uint64_t* a_full = empty + MAX_STAGES;  // [2]
-  uint64_t* a_empty = a_full + 2;         // [2]
-  uint64_t* acc_full = a_empty + 2;
+  uint64_t* a_full = empty + MAX_STAGES;  // [GROUPS]
+  uint64_t* a_empty = a_full + GROUPS;    // [GROUPS]
+  uint64_t* acc_full = a_empty + GROUPS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   __shared__ int failed_flag;
   volatile int* failed = &failed_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = ks > 1 ? (int)cluster_rank() : 0;
-  const int n0 = blockIdx.y * TILE, m0 = blockIdx.z * a.n_tokens;
-  const int per_block = (p.k_blocks + ks - 1) / ks;
-  const int step_lo = min(rank * per_block, p.k_blocks), k_steps = min(step_lo + per_block, p.k_blocks) - step_lo;  // may be 0
+  const int n0 = blockIdx.y * TILE;
+  const int each = (p.k_blocks + ks - 1) / ks;
+  const int step_lo = min(rank * each, p.k_blocks), k_steps = min(step_lo + each, p.k_blocks) - step_lo;  // may be 0
 
   if (threadIdx.x == 0) {
     failed_flag = 0;
@@ -331,35 +401,32 @@ __global__ void __launch_bounds__(ROWS_THREADS) int4_rows_kernel(const __grid_co
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < GROUPS; ++i) {
       mbar_init(&a_full[i], 4);  // the warps of a group
       mbar_init(&a_empty[i], 1);
     }
     mbar_init(acc_full, 1);
     mbar_fence_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, a.tmem_columns);
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot, tmem_a = tmem + a.acc_columns;
+  const uint32_t tmem = *tmem_slot, tmem_a = tmem + A_FIRST;
   pdl_launch_dependents();  // now: a block of the next kernel must not take the tensor memory that this one still needs
 
   if (warp == 0) {
     if (elect_one()) {
-      const int row_blocks = min(TILE / BLOCK_ROWS, (p.N + BLOCK_ROWS - 1) / BLOCK_ROWS - n0 / BLOCK_ROWS);
       auto load_w = [&](int i) {
         const int s = i % stages;
-        unsigned char* to = smem + (size_t)s * stage_bytes + x_bytes;
-        mbar_arrive_expect_tx(&full[s], x_bytes + row_blocks * BLOCK_BYTES);
-        for (int b = 0; b < row_blocks; ++b)
-          bulk_copy_g2s(to + b * BLOCK_BYTES, p.w + ((size_t)(n0 / BLOCK_ROWS + b) * p.k_blocks + step_lo + i) * BLOCK_BYTES, BLOCK_BYTES, &full[s]);
+        mbar_arrive_expect_tx(&full[s], x_bytes + TILE / BLOCK_ROWS * bytes);
+        tma_load_3d(smem + s * stage_bytes + x_bytes, &map_w, 0, step_lo + i, n0 / BLOCK_ROWS, &full[s]);
       };
       auto load_x = [&](int i) {
         const int s = i % stages;
-        unsigned char* to = smem + (size_t)s * stage_bytes;
-        tma_load_2d(to, &map_x, (step_lo + i) * BLOCK_K, m0, &full[s]);
-        tma_load_2d(to + x_bytes / 2, &map_x, (step_lo + i) * BLOCK_K + 64, m0, &full[s]);
+        unsigned char* to = smem + s * stage_bytes;
+        tma_load_2d(to, &map_x, (step_lo + i) * BLOCK_K, 0, &full[s]);
+        tma_load_2d(to + x_bytes / 2, &map_x, (step_lo + i) * BLOCK_K + 64, 0, &full[s]);
       };
       const int early = min(stages, k_steps);
       for (int i = 0; i < early; ++i) load_w(i);  // weights do not depend on the kernel before
@@ -374,86 +441,50 @@ __global__ void __launch_bounds__(ROWS_THREADS) int4_rows_kernel(const __grid_co
   } else if (warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = umma_idesc(TILE, a.n_tokens);
+      int s = 0, group = 0;
+      uint32_t phase = 0, turn = 0;
       for (int i = 0; i < k_steps; ++i) {
-        const int s = i % stages, half = i & 1;
-        if (!wait_or_abort(&full[s], (i / stages) & 1, failed)) break;
-        if (!wait_or_abort(&a_full[half], (i >> 1) & 1, failed)) break;
+        if (!wait_or_abort(&full[s], phase, failed)) break;
+        if (!wait_or_abort(&a_full[group], turn, failed)) break;
         tc_fence_after();
-        const uint32_t b = smem_u32(smem + (size_t)s * stage_bytes);
+        const uint32_t b = smem_u32(smem + s * stage_bytes);
 #pragma unroll
         for (int kk = 0; kk < BLOCK_K / 16; ++kk)
-          umma_a_tmem(tmem, tmem_a + half * A_COLUMNS + kk * 8, umma_desc(b + (kk >> 2) * (x_bytes / 2) + (kk & 3) * 32), idesc, i > 0 || kk > 0);
+          umma_a_tmem(tmem, tmem_a + group * A_COLUMNS + kk * 8, umma_desc(b + (kk >> 2) * (x_bytes / 2) + (kk & 3) * 32), idesc, i > 0 || kk > 0);
         tc_commit(&empty[s]);
-        tc_commit(&a_empty[half]);
+        tc_commit(&a_empty[group]);
+        if (++s == stages) s = 0, phase ^= 1;
+        if (++group == a.groups) group = 0, turn ^= 1;
       }
       tc_commit(acc_full);
     }
   } else {
-    const int group = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;  // a warp reaches the 32 lanes of its number's rest by 4
-    const int out_row = min(n0 + row, p.N - 1);
-    const uint32_t* words = p.groups + out_row;
-    auto group_word = [&](int i, int u) {  // of sub-block u (32 k) of step i
-      return words[(size_t)min(((step_lo + i) * BLOCK_K + 32 * u) / p.group, p.n_groups - 1) * p.N];
-    };
-    uint32_t next[4] = {};
-    auto load_words = [&](int i) {
-      if (i >= k_steps) return;
-      next[0] = group_word(i, 0);
-      if (a.per >= 2) next[2] = group_word(i, 2);
-      if (a.per == 4) {
-        next[1] = group_word(i, 1);
-        next[3] = group_word(i, 3);
-      }
-    };
-    load_words(group);
-    for (int i = group; i < k_steps; i += 2) {
-      const int s = i % stages;
-      uint32_t g[4] = {next[0], a.per == 4 ? next[1] : next[0], a.per >= 2 ? next[2] : next[0], 0};
-      g[3] = a.per == 4 ? next[3] : g[2];
-      load_words(i + 2);
-      if (!warp_wait(&full[s], (i / stages) & 1, failed)) break;
-      const uint4* at = reinterpret_cast<const uint4*>(smem + (size_t)s * stage_bytes + x_bytes + row * 64);
-      uint4 piece[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) piece[c] = at[c ^ ((row >> 1) & 3)];
-      if (!warp_wait(&a_empty[group], ((i >> 1) & 1) ^ 1, failed)) break;
-      tc_fence_after();
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // 64 k: 32 columns
-        uint32_t col[32];
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const uint32_t gw = g[2 * h + v];
-          const __nv_bfloat162 zero = both(gw >> 16), scale = both(gw & 0xffffu);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t word = h == 0 ? (v == 0 ? piece[c].x : piece[c].y) : (v == 0 ? piece[c].z : piece[c].w);
-            unpack8(word, zero, col + v * 16 + c * 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&col[v * 16 + c * 4 + e]), scale);
-              col[v * 16 + c * 4 + e] = *reinterpret_cast<const uint32_t*>(&r);
-            }
-          }
-        }
-        tmem_store_pairs(tmem_a + group * A_COLUMNS + h * 32 + ((uint32_t)(quarter * 32) << 16), col);
-      }
-      asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-      tc_fence_before();
-      __syncwarp();
+    const int group = (warp - 2) >> 2;
+    int s = group;  // no more groups than stages
+    uint32_t phase = 0, turn = 1;
+    for (int i = group < a.groups ? group : k_steps; i < k_steps; i += a.groups) {
+      if (!warp_wait(&a_empty[group], turn, failed)) break;
+      if (!warp_wait(&full[s], phase, failed)) break;
+      unpack_row(smem + s * stage_bytes + x_bytes, bytes, p.per, warp & 3, lane, tmem_a + group * A_COLUMNS);
       if (lane == 0) mbar_arrive(&a_full[group]);
+      turn ^= 1;
+      s += a.groups;
+      if (s >= stages) s -= stages, phase ^= 1;
     }
   }
-  // This block's sums as float32 [128][n_tokens + 4] in shared memory, over the stages: every copy into them has landed and
-  // every instruction that read them is done once the accumulator is ready.
+  // The sums leave tensor memory as they are where a block has them whole; else they meet in shared memory, as float32
+  // [128][n_tokens + 4] over the stages (every copy into them has landed and every instruction that read them is done once the
+  // accumulator is ready).  Thread: a row of w, runs of 8 or 16 tokens.
   float* red = reinterpret_cast<float*>(smem);
   const int red_stride = a.n_tokens + 4;
-  if (warp >= 2 && warp < 6) {
-    pdl_wait();
-    const int quarter = warp & 3, row = quarter * 32 + lane;
+  if (warp >= 2) {
+    pdl_wait();  // y may be what the kernel before still reads
+    const int quarter = warp & 3, row = quarter * 32 + lane, col = n0 + row;
+    const bool live = col < p.N;
+    const float bias = live && p.bias ? __bfloat162float(p.bias[col]) : 0.f;
     const bool ok = warp_wait(acc_full, 0, failed);
     tc_fence_after();
-    for (int c0 = 0; c0 < a.n_tokens; c0 += 16) {
+    for (int c0 = 16 * ((warp - 2) >> 2); c0 < a.n_tokens; c0 += 16 * GROUPS) {
       float v[16];
       if (ok && k_steps > 0) {
         tmem_load_16(tmem + ((uint32_t)(quarter * 32) << 16) + c0, v);
@@ -461,75 +492,80 @@ __global__ void __launch_bounds__(ROWS_THREADS) int4_rows_kernel(const __grid_co
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] = 0.f;
       }
+      if (ks > 1) {
 #pragma unroll
-      for (int j = 0; j < 16; j += 4)
-        *reinterpret_cast<float4*>(red + row * red_stride + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        for (int j = 0; j < 16; j += 4)
+          *reinterpret_cast<float4*>(red + row * red_stride + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      } else if (ok && live) {
+        store_column<16>(p, v, c0, col, bias);
+      }
     }
     tc_fence_before();
   }
-  __syncthreads();
-  if (ks > 1) cluster_sync_all();
-  if (warp >= 2 && !*failed) {  // this block's share of the tokens, four at a time; a thread keeps its row of w
-    const int e = threadIdx.x - 64, i = e & 127, share = ((a.n_tokens + ks - 1) / ks + 3) / 4 * 4;
-    const int t_hi = min((rank + 1) * share, a.n_tokens), col = n0 + i;
-    const uint32_t at0 = smem_u32(red) + (uint32_t)(i * red_stride) * 4u;
-    const float bias = p.bias && col < p.N ? __bfloat162float(p.bias[col]) : 0.f;
-    for (int t = rank * share + 4 * (e >> 7); t < t_hi; t += 8) {
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-      float4 v[MAX_KS];
+  if (ks > 1) {
+    __syncthreads();
+    cluster_sync_all();
+    if (warp >= 2 && !*failed) {  // this block's share of the tokens, 8 at a time
+      const int e = threadIdx.x - 64, i = e & 127, col = n0 + i, share = ((a.n_tokens + ks - 1) / ks + 7) / 8 * 8;
+      const int t_hi = min((rank + 1) * share, a.n_tokens);
+      const bool live = col < p.N;
+      const float bias = live && p.bias ? __bfloat162float(p.bias[col]) : 0.f;
+      for (int t = rank * share + 8 * (e >> 7); t < t_hi; t += 8 * GROUPS) {
+        float4 v[MAX_KS][2];
+        const uint32_t at = smem_u32(red) + (uint32_t)(i * red_stride + t) * 4u;
 #pragma unroll
-      for (int r = 0; r < MAX_KS; ++r)
-        if (r < ks) v[r] = ks == 1 ? *reinterpret_cast<const float4*>(red + i * red_stride + t) : ld_cluster_f32x4(at0 + 4u * t, (uint32_t)r);
+        for (int r = 0; r < MAX_KS; ++r)  // all loads on their way before the first sum
+          if (r < ks) {
+            v[r][0] = ld_cluster_f32x4(at, (uint32_t)r);
+            v[r][1] = ld_cluster_f32x4(at + 16, (uint32_t)r);
+          }
+        float sum[8] = {};
 #pragma unroll
-      for (int r = 0; r < MAX_KS; ++r)
-        if (r < ks) {
-          sum[0] += v[r].x; sum[1] += v[r].y; sum[2] += v[r].z; sum[3] += v[r].w;
-        }
-      if (col >= p.N) continue;
+        for (int r = 0; r < MAX_KS; ++r)
+          if (r < ks) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int m = m0 + t + j;
-        if (m < p.M && FMS_IN((size_t)m * p.N + col, (size_t)p.M * p.N)) p.y[(size_t)m * p.N + col] = __float2bfloat16_rn(sum[j] + bias);
+            for (int h = 0; h < 2; ++h) {
+              sum[4 * h] += v[r][h].x; sum[4 * h + 1] += v[r][h].y; sum[4 * h + 2] += v[r][h].z; sum[4 * h + 3] += v[r][h].w;
+            }
+          }
+        if (live) store_column<8>(p, sum, t, col, bias);
       }
     }
+    cluster_sync_all();  // nobody leaves while another block still reads its shared memory
   }
-  if (ks > 1) cluster_sync_all();  // nobody leaves while another block still reads its shared memory
   __syncthreads();
   if (threadIdx.x == 0 && *failed && error_flag) atomicExch(error_flag, 4);
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, a.tmem_columns);
+    tmem_dealloc(tmem, 512);
   }
 }
 
+// A block that holds all of the tensor memory takes so much shared memory that no block that wants some fits beside it: one that
+// waits for it could be what this one waits for (the others of a cluster, the kernel before).
+constexpr size_t SMEM_LEAST = 200 * 1024, SMEM_MOST = 225 * 1024, EXTRA = 1024 /* alignment */ + 512 /* barriers */;
+
 int launch_rows(const Int4Args& p, int* error_flag, cudaStream_t stream) {
-  constexpr int MOST = 256, EXTRA = 1024 + 512;
   RowsArgs a = {};
   a.p = p;
-  a.n_tokens = p.M >= MOST ? MOST : (p.M + 15) / 16 * 16;
-  const int tiles = (p.N + TILE - 1) / TILE, chunks = (p.M + a.n_tokens - 1) / a.n_tokens;
-  if (tiles > 65535 || chunks > 65535) return fms_fail("gemm_int4: %d by %d tiles", tiles, chunks);
-  a.ks = 1;  // blocks that share a tile, as many as leave each 4 steps, up to two a multiprocessor
-  while (a.ks < MAX_KS && tiles * chunks * a.ks * 2 <= 320 && p.k_blocks / (a.ks * 2) >= 4) a.ks *= 2;
-  const int stage_bytes = a.n_tokens * BLOCK_K * 2 + TILE / BLOCK_ROWS * BLOCK_BYTES;
-  const int budget = (a.n_tokens <= 128 && tiles * chunks * a.ks > 148) ? 104 * 1024 : 222 * 1024;
-  const size_t red_bytes = (size_t)TILE * (a.n_tokens + 4) * sizeof(float);
-  a.stages = min(max(budget / stage_bytes, 2), MAX_STAGES);
-  while ((size_t)a.stages * stage_bytes < red_bytes) ++a.stages;
-  a.acc_columns = (a.n_tokens + 31) / 32 * 32;
-  a.tmem_columns = a.acc_columns + 2 * A_COLUMNS <= 256 ? 256 : 512;
-  a.per = (p.group % 128 == 0 || p.n_groups == 1) ? 1 : (p.group % 64 == 0 ? 2 : 4);
-  CUtensorMap map_x;
-  if (make_map(&map_x, p.x, p.M, p.K, a.n_tokens)) return 1;
+  a.n_tokens = (p.M + 15) / 16 * 16;
+  const int tiles = (p.N + TILE - 1) / TILE;
+  if (tiles > 65535) return fms_fail("gemm_int4: %d tiles of rows of w", tiles);
+  a.ks = 1;  // from the weights' shape alone, as many as fill most of the multiprocessors, each with 4 steps at least
+  while (a.ks < MAX_KS && tiles * a.ks < 120 && p.k_blocks / (a.ks * 2) >= 4) a.ks *= 2;
+  const int stage_bytes = (a.n_tokens * BLOCK_K * 2 + TILE / BLOCK_ROWS * p.block_bytes() + 1023) / 1024 * 1024;
+  a.stages = min((int)((SMEM_MOST - EXTRA) / stage_bytes), MAX_STAGES);
+  a.groups = min(GROUPS, a.stages);
+  const size_t stages_bytes = (size_t)a.stages * stage_bytes, red_bytes = a.ks > 1 ? (size_t)TILE * (a.n_tokens + 4) * sizeof(float) : 0;
+  if (a.stages < 2 || red_bytes > stages_bytes) return fms_fail("gemm_int4: no room for %d tokens", a.n_tokens);
+  CUtensorMap map_x, map_w;
+  if (make_map(&map_x, p.x, p.M, p.K, a.n_tokens) || make_block_map(&map_w, p)) return 1;
   static uint64_t allowed = 0;
-  if (allow_smem("gemm_int4", int4_rows_kernel, 225 * 1024, &allowed)) return 1;
+  if (allow_smem(int4_rows_kernel, (int)SMEM_MOST, &allowed)) return 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.ks, tiles, chunks);
+  cfg.gridDim = dim3(a.ks, tiles);
   cfg.blockDim = dim3(ROWS_THREADS);
-  // No more blocks on a multiprocessor than its 512 columns of tensor memory serve: one that waited for columns could be what
-  // the holder's cluster waits for.
-  const size_t least = a.tmem_columns == 512 ? 200 * 1024 : 78 * 1024, smem = (size_t)a.stages * stage_bytes + EXTRA;
-  cfg.dynamicSmemBytes = smem < least ? least : smem;
+  cfg.dynamicSmemBytes = stages_bytes + EXTRA < SMEM_LEAST ? SMEM_LEAST : stages_bytes + EXTRA;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -540,42 +576,229 @@ int launch_rows(const Int4Args& p, int* error_flag, cudaStream_t stream) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = fms_pdl_enabled() ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, int4_rows_kernel, map_x, a, error_flag);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, int4_rows_kernel, map_x, map_w, a, error_flag);
   if (e != cudaSuccess) return fms_fail("gemm_int4: launch failed: %s", cudaGetErrorString(e));
+  return fms_launch_status("gemm_int4");
+}
+
+// ---- more rows (prefill) ------------------------------------------------------------------------------------------------
+// Persistent pairs of thread blocks (a cluster of two, cta_group::2): a pair owns a tile of 256 rows of w by up to 256 tokens.  Each
+// block unpacks its own 128 rows of w into its own tensor memory and brings half of the tokens, so a multiprocessor takes in
+// 128 rows of x and 128 half-bytes a k for 2 * 128 * 256 operations.  The accumulator takes half of the 512 columns and four stages
+// of the operand the other half: a stage goes round in some 2,400 cycles (barriers, unpacking, the instructions), so that two of
+// them, which left room for two accumulators of 192 columns, kept the tensor cores waiting (2,048 x 28,672 x 4,096 454 us).
+// The next tile's first four steps are unpacked under the epilogue.
+//   warp 0      per step of 128 k: two 64-k boxes of x, counted on block 0's barrier, and one of eight blocks of w, counted on its own
+//   warp 1      (of block 0) issues 8 instructions (256 x tokens x 16) a step
+//   warps 2-17  four groups of four unpack every fourth step each: a thread a row of w
+//   warps 18-25 the epilogue, a warp a row's 32 lanes and every second 16 tokens
+constexpr int PAIR_EPILOGUE = 8, PAIR_THREADS = 64 + 32 * (UNPACK_WARPS + PAIR_EPILOGUE), PAIR_TOKENS = 256;
+
+__device__ __forceinline__ void umma_pair_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
+  const uint32_t acc = accumulate ? 1u : 0u, zero = 0u;
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(zero)
+      : "memory");
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+    int4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, RowsArgs a,
+                     int* __restrict__ error_flag) {
+  extern __shared__ unsigned char smem_unaligned[];
+  unsigned char* smem = smem_unaligned + (-smem_u32(smem_unaligned) & 1023);
+  const Int4Args& p = a.p;
+  const int half_tokens = a.n_tokens / 2, bytes = p.block_bytes(), x_bytes = half_tokens * BLOCK_K * 2, stages = a.stages;
+  const int stage_bytes = (x_bytes + TILE / BLOCK_ROWS * bytes + 1023) / 1024 * 1024, k_steps = p.k_blocks;
+  uint64_t* x_full = reinterpret_cast<uint64_t*>(smem + stages * stage_bytes);
+  uint64_t* w_full = x_full + MAX_STAGES;
+  uint64_t* empty = w_full + MAX_STAGES;
+  uint64_t* a_full = empty + MAX_STAGES;  // [GROUPS]
+  uint64_t* a_empty = a_full + GROUPS;    // [GROUPS]
+  uint64_t* acc_full = a_empty + GROUPS;
+  uint64_t* acc_empty = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  __shared__ int failed_flag;
+  volatile int* failed = &failed_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int tiles_m = (p.M + a.n_tokens - 1) / a.n_tokens, n_tiles = tiles_m * ((p.N + 2 * TILE - 1) / (2 * TILE));
+  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    failed_flag = 0;
+    for (int s = 0; s < MAX_STAGES; ++s) {
+      mbar_init(&x_full[s], 1);
+      mbar_init(&w_full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < GROUPS; ++i) {
+      mbar_init(&a_full[i], 8);  // the warps of a group, of either block (used in block 0)
+      mbar_init(&a_empty[i], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 2 * PAIR_EPILOGUE);  // of either block (used in block 0)
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the partner's barriers exist before anything is sent to them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, tmem_a = tmem + A_FIRST;
+  pdl_launch_dependents();  // now: a block of the next kernel must not take the tensor memory that this one still needs
+  pdl_wait();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int it = 0;
+      for (int tile = pair; tile < n_tiles && !*failed; tile += pairs) {
+        const int m0 = (tile % tiles_m) * a.n_tokens + (int)rank * half_tokens;
+        const int block0 = ((tile / tiles_m) * 2 + (int)rank) * (TILE / BLOCK_ROWS);
+        for (int i = 0; i < k_steps; ++i, ++it) {
+          const int s = it % stages;
+          if (!wait_or_abort(&empty[s], ((it / stages) & 1) ^ 1, failed)) break;
+          unsigned char* to = smem + s * stage_bytes;
+          mbar_arrive_expect_tx(&w_full[s], TILE / BLOCK_ROWS * bytes);
+          tma_load_3d(to + x_bytes, &map_w, 0, i, block0, &w_full[s]);
+          if (leader) mbar_arrive_expect_tx(&x_full[s], 2 * x_bytes);  // the bytes of both blocks
+          tma_load_2d_pair(to, &map_x, i * BLOCK_K, m0, &x_full[s]);
+          tma_load_2d_pair(to + x_bytes / 2, &map_x, i * BLOCK_K + 64, m0, &x_full[s]);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (leader && elect_one()) {
+      const uint32_t idesc = umma_idesc(2 * TILE, a.n_tokens);
+      int j = 0, s = 0, group = 0;
+      uint32_t phase = 0, turn = 0;
+      for (int tile = pair; tile < n_tiles && !*failed; tile += pairs, ++j) {
+        if (!wait_or_abort(acc_empty, (j & 1) ^ 1, failed)) break;  // both epilogues have read the tile before
+        for (int i = 0; i < k_steps; ++i) {
+          if (!wait_or_abort(&x_full[s], phase, failed)) break;
+          if (!wait_or_abort(&a_full[group], turn, failed)) break;
+          tc_fence_after();
+          const uint32_t b = smem_u32(smem + s * stage_bytes);
+#pragma unroll
+          for (int kk = 0; kk < BLOCK_K / 16; ++kk)
+            umma_pair_a_tmem(tmem, tmem_a + group * A_COLUMNS + kk * 8, umma_desc(b + (kk >> 2) * (x_bytes / 2) + (kk & 3) * 32), idesc,
+                             i > 0 || kk > 0);
+          tc_commit_pair(&empty[s]);
+          tc_commit_pair(&a_empty[group]);
+          if (++s == stages) s = 0, phase ^= 1;
+          if (++group == GROUPS) group = 0, turn ^= 1;
+        }
+        tc_commit_pair(acc_full);
+      }
+    }
+  } else if (warp < 2 + UNPACK_WARPS) {
+    const int group = (warp - 2) >> 2;
+    int left = 0;  // steps, over all tiles
+    for (int tile = pair; tile < n_tiles; tile += pairs) left += k_steps;
+    int s = group;  // there are no fewer stages than groups
+    uint32_t phase = 0, turn = 1;
+    for (int it = group; it < left; it += GROUPS) {
+      // its columns first: see the kernel above
+      if (!warp_wait(&a_empty[group], turn, failed)) break;
+      if (!warp_wait(&w_full[s], phase, failed)) break;
+      unpack_row(smem + s * stage_bytes + x_bytes, bytes, p.per, warp & 3, lane, tmem_a + group * A_COLUMNS);
+      if (lane == 0) {
+        if (leader) mbar_arrive(&a_full[group]);
+        else mbar_arrive_remote(&a_full[group], 0);
+      }
+      turn ^= 1;
+      s += GROUPS;
+      if (s >= stages) s -= stages, phase ^= 1;
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2 - UNPACK_WARPS) >> 2;
+    int j = 0;
+    for (int tile = pair; tile < n_tiles; tile += pairs, ++j) {
+      const int m0 = (tile % tiles_m) * a.n_tokens, col = ((tile / tiles_m) * 2 + (int)rank) * TILE + quarter * 32 + lane;
+      const float bias = p.bias && col < p.N ? __bfloat162float(p.bias[col]) : 0.f;
+      if (!warp_wait(acc_full, j & 1, failed)) break;
+      tc_fence_after();
+      for (int c0 = 16 * half; c0 < a.n_tokens; c0 += 32) {
+        float v[16];
+        tmem_load_16(tmem + ((uint32_t)(quarter * 32) << 16) + c0, v);
+        if (col < p.N) store_column<16>(p, v, m0 + c0, col, bias);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (leader) mbar_arrive(acc_empty);
+        else mbar_arrive_remote(acc_empty, 0);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // nothing is sent to a block that has left
+  if (threadIdx.x == 0 && *failed && error_flag) atomicExch(error_flag, 4);
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+int launch_pair(const Int4Args& p, int* error_flag, cudaStream_t stream) {
+  RowsArgs a = {};
+  a.p = p;
+  // the width whose tiles cost least in whole rounds of the pairs; below some 144 tokens a step takes what unpacking takes
+  const int pairs = max(multiprocessors() / 2, 1), tiles_n = (p.N + 2 * TILE - 1) / (2 * TILE);
+  long best = -1;
+  for (int tn = PAIR_TOKENS; tn >= 64; tn -= 16) {
+    const long tiles = (long)tiles_n * ((p.M + tn - 1) / tn), cost = (tiles + pairs - 1) / pairs * (max(tn, 144) + 24);
+    if (best < 0 || cost < best) {
+      best = cost;
+      a.n_tokens = tn;
+    }
+  }
+  const long tiles = (long)tiles_n * ((p.M + a.n_tokens - 1) / a.n_tokens);
+  if (tiles > 0x7fffffffL) return fms_fail("gemm_int4: %ld tiles", tiles);
+  const int stage_bytes = (a.n_tokens * BLOCK_K + TILE / BLOCK_ROWS * p.block_bytes() + 1023) / 1024 * 1024;
+  a.stages = min((int)((SMEM_MOST - EXTRA) / stage_bytes), MAX_STAGES);
+  CUtensorMap map_x, map_w;
+  if (make_map(&map_x, p.x, p.M, p.K, a.n_tokens / 2) || make_block_map(&map_w, p)) return 1;
+  static uint64_t allowed = 0;
+  if (allow_smem(int4_pair_kernel, (int)SMEM_MOST, &allowed)) return 1;
+  const size_t smem = (size_t)a.stages * stage_bytes + EXTRA;
+  fms_launch(int4_pair_kernel, dim3(2 * (int)(tiles < pairs ? tiles : pairs)), dim3(PAIR_THREADS), smem < SMEM_LEAST ? SMEM_LEAST : smem,
+             stream, map_x, map_w, a, error_flag);
   return fms_launch_status("gemm_int4");
 }
 
 int check(const Int4Args& p) {
   if (p.K <= 0 || p.K % 8) return fms_fail("gemm_int4: %d input channels, a multiple of 8 is wanted", p.K);
   if (p.k_blocks != (p.K + BLOCK_K - 1) / BLOCK_K) return fms_fail("gemm_int4: %d blocks for %d input channels", p.k_blocks, p.K);
-  if (p.group <= 0 || p.n_groups != (p.K + p.group - 1) / p.group || (p.n_groups > 1 && p.group % 32))
-    return fms_fail("gemm_int4: %d groups of %d for %d input channels", p.n_groups, p.group, p.K);
+  if (p.per != 1 && p.per != 2 && p.per != 4) return fms_fail("gemm_int4: %d scales a block of 128 input channels", p.per);
   if (((uintptr_t)p.x | (uintptr_t)p.w) & 15) return fms_fail("gemm_int4: operands must be 16-byte aligned");
   return 0;
 }
-constexpr int FEW_ROWS = 16;  // rows of x up to which mma.sync takes the product
+constexpr int SOME_ROWS = 256;  // rows of x up to which the second kernel takes the product
 }  // namespace
 
-// The most rows of fms_glu_int4.
-FMS_API int fms_int4_few_rows() { return FEW_ROWS; }
-
-// y [M, N] bfloat16 of x [M, K] bfloat16, w packed, groups [n_groups, N], bias [N] bfloat16 or null.
-FMS_API int fms_linear_int4(const void* x, const void* w, const void* groups, const void* bias, void* y, int M, int N, int K,
-                            int k_blocks, int n_groups, int group, int* error_flag, cudaStream_t stream) {
+// y [M, N] bfloat16 of x [M, K] bfloat16, w packed with `per` scales a block, bias [N] bfloat16 or null.
+FMS_API int fms_linear_int4(const void* x, const void* w, const void* bias, void* y, int M, int N, int K, int k_blocks, int per,
+                            int* error_flag, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
-  const Int4Args p = {(const __nv_bfloat16*)x, (const unsigned char*)w, (const uint32_t*)groups, (const __nv_bfloat16*)bias,
-                      (__nv_bfloat16*)y, M, N, K, k_blocks, n_groups, group, N, 0};
+  const Int4Args p = {(const __nv_bfloat16*)x, (const unsigned char*)w, (const __nv_bfloat16*)bias, (__nv_bfloat16*)y,
+                      M, N, K, k_blocks, per, N, 0};
   if (check(p)) return 1;
-  return M <= FEW_ROWS ? few<false>(p, stream) : launch_rows(p, error_flag, stream);
+  return M <= FEW_ROWS ? few<false>(p, stream) : (M <= SOME_ROWS ? launch_rows(p, error_flag, stream) : launch_pair(p, error_flag, stream));
 }
 
-// y [M, hidden] = act(gate) * up for w = [gate; up] of 2 hidden rows, up to FEW_ROWS rows of x.
-FMS_API int fms_glu_int4(const void* x, const void* w, const void* groups, const void* bias, void* y, int M, int hidden, int K,
-                         int k_blocks, int n_groups, int group, int act, cudaStream_t stream) {
+// y [M, hidden] = act(gate) * up for w = [gate; up] of 2 hidden rows, hidden a multiple of 16, up to 8 rows of x.
+FMS_API int fms_glu_int4(const void* x, const void* w, const void* bias, void* y, int M, int hidden, int K, int k_blocks, int per,
+                         int act, cudaStream_t stream) {
   if (M <= 0 || hidden <= 0) return 0;
-  if (M > FEW_ROWS || act < 0 || act > 3) return fms_fail("glu_int4: %d rows of x, activation %d", M, act);
-  const Int4Args p = {(const __nv_bfloat16*)x, (const unsigned char*)w, (const uint32_t*)groups, (const __nv_bfloat16*)bias,
-                      (__nv_bfloat16*)y, M, 2 * hidden, K, k_blocks, n_groups, group, hidden, act};
+  if (M > FEW_ROWS || hidden % BLOCK_ROWS || act < 0 || act > 3)
+    return fms_fail("glu_int4: %d rows of x, %d hidden values, activation %d", M, hidden, act);
+  const Int4Args p = {(const __nv_bfloat16*)x, (const unsigned char*)w, (const __nv_bfloat16*)bias, (__nv_bfloat16*)y,
+                      M, 2 * hidden, K, k_blocks, per, hidden, act};
   if (check(p)) return 1;
   return few<true>(p, stream);
 }

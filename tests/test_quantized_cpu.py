@@ -28,13 +28,18 @@ def test_packed_weights_stand_for_what_was_given(out, dim, group, zeros):
 
 
 def test_the_layout_of_a_block():
-    """Value k of row r: word 16 r' + 4 place + k // 32, place = (k // 8 % 4) ^ (r // 2 % 4), bits 4 (k % 8 // 2) + 16 (k % 2)."""
+    """Value k of row r: word 16 r + 4 place + k // 32 of its block, place = (k // 8 % 4) ^ (r // 2 % 4), bits 4 (k % 8 // 2) + 16 (k % 2);
+    behind the 256 words a block's scales and zero points, 16 rows at a time."""
     q = torch.randint(0, 16, (32, 256), generator=gen(0), dtype=torch.uint8)
-    w = ops.pack_int4(q, torch.ones(32, 2), None, 128)
+    scales = torch.arange(1, 129).view(32, 4).float()
+    w = ops.pack_int4(q, scales, None, 64)
+    assert w.per == 2 and w.blocks.shape == (2, 2, 256 + 32)
     for r, k in ((0, 0), (0, 1), (3, 13), (17, 200), (31, 255), (9, 127), (14, 64)):
-        word = int(w.blocks[r // 16, k // 128, r % 16, (k // 8 % 4) ^ (r // 2 % 4), k % 128 // 32])
+        word = int(w.blocks[r // 16, k // 128, r % 16 * 16 + ((k // 8 % 4) ^ (r // 2 % 4)) * 4 + k % 128 // 32])
         assert (word >> (4 * (k % 8 // 2) + 16 * (k % 2))) & 15 == int(q[r, k])
-    assert int(w.groups[1, 5]) & 0xFFFF == 0x3F80 and (int(w.groups[1, 5]) >> 16) & 0xFFFF == 0x4308  # bfloat16 1 and 136
+        group = int(w.blocks[r // 16, k // 128, 256 + k % 128 // 64 * 16 + r % 16])
+        assert (group >> 16) & 0xFFFF == 0x4308  # bfloat16 136
+        assert torch.tensor([group << 16], dtype=torch.int64).to(torch.int32).view(torch.float32).item() == float(scales[r, k // 64])
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, BF16])
