@@ -7,7 +7,7 @@ turn prompts into ids, generate, print.
 Kept from the reference: --device_type, --architecture, --variant, --model_path, --model_source,
 --tokenizer, --default_dtype, --batch_input (run all prompts as one batch), --context_file, --deterministic
 (here: greedy).  Added: --prompt (repeatable), --prompt_ids, --max_new_tokens, --do_sample, --temperature,
---top_k, --seed, --eos_token_id, --timing.  Dropped, with what they selected gone: --no_use_cache,
+--top_k, --seed, --eos_token_id, --timing, --linear_type and --linear_group_size (the reference's ``linear_config``).  Dropped, with what they selected gone: --no_use_cache,
 --unfuse_weights, --compile, --compile_mode, --distributed, --attn_name.  --min_pad_length is kept with its
 meaning: the prompts go through ``pad_input_ids`` and come back out of their padding, which changes no token.
 """
@@ -30,6 +30,9 @@ def build_parser() -> argparse.ArgumentParser:
                    help='"char_tokenizer" or a folder with a tokenizer.json; without one give --prompt_ids')
     p.add_argument("--default_dtype", type=str, default=None, choices=["bf16", "fp32"],
                    help="Compute dtype; fp32 uses no reduced-precision product")
+    p.add_argument("--linear_type", type=str, default="torch_linear", choices=["torch_linear", "fp8", "int4"],
+                   help="How a Llama model keeps its layers' matrices: as stored, in 8 bits (rows too) or in 4 bits")
+    p.add_argument("--linear_group_size", type=int, default=128, help="Input channels that share a scale (int4)")
     p.add_argument("--batch_input", action="store_true", help="Run all prompts as one batch")
     p.add_argument("--min_pad_length", type=int, default=0,
                    help="Pad inputs to a minimum length. If any prompt is longer, padding will be determined by "
@@ -81,9 +84,14 @@ def main(argv=None) -> int:
 
     if args.variant is None and args.model_path is None:
         args.variant = "micro"
+    linear = {}
+    if args.linear_type != "torch_linear":
+        linear["linear_config"] = {"linear_type": args.linear_type}
+        if args.linear_type == "int4":
+            linear["linear_config"]["group_size"] = args.linear_group_size
     print("loading model", file=sys.stderr)
     model = get_model(args.architecture, args.variant, model_path=args.model_path, source=args.model_source,
-                      device_type=args.device_type, data_type=args.default_dtype, seed=args.seed)
+                      device_type=args.device_type, data_type=args.default_dtype, seed=args.seed, **linear)
     eos = args.eos_token_id if args.eos_token_id is not None else (tokenizer.eos_token_id if tokenizer else None)
     do_sample = args.do_sample and not args.deterministic
     groups = [prompts] if args.batch_input else [[p] for p in prompts]

@@ -87,7 +87,9 @@ def get_model(architecture: str, variant: Optional[str] = None, model_path: Opti
         fms/modules/attention.py:689-692; fms/modules/feedforward.py:269-283; gains 1).
     distributed_strategy, checkpoint_sharding, group: the reference's parameters for several devices
         (fms/models/__init__.py:298-308); this library runs on one GPU and refuses anything but None.
-    kwargs: overrides of configuration fields, as in the reference.
+    kwargs: overrides of configuration fields, as in the reference.  ``linear_config`` (Llama) quantises the layers' matrices
+        as they are loaded: {"linear_type": "fp8"} (8-bit weights and rows) or {"linear_type": "int4", "group_size": 128}
+        (4-bit weights); bfloat16 models only.
     """
     if distributed_strategy is not None or checkpoint_sharding is not None or group is not None:
         raise NotImplementedError("this library runs a model on one GPU: distributed_strategy, checkpoint_sharding "
@@ -119,7 +121,12 @@ def get_model(architecture: str, variant: Optional[str] = None, model_path: Opti
                            f'`models.list_variants("{architecture}")` for available variants.')
         model = _models[architecture][variant](**kwargs)
 
+    from ..parts.linear import linear_options
     from ..weights.loader import checkpoint_dtype
+
+    quantised = linear_options(kwargs.get("linear_config"))
+    if quantised and not hasattr(model.config, "linear_config"):
+        raise ValueError(f"{architecture} has no quantised linear layers: linear_config {dict(kwargs['linear_config'])}")
 
     device = torch.device(device_type)
     if model_path is not None:
@@ -130,6 +137,8 @@ def get_model(architecture: str, variant: Optional[str] = None, model_path: Opti
         src = RandomSource(model.checkpoint_layout(), seed, dtype=torch.bfloat16, device=device, init=init)
         source = model.default_source
         dtype = torch.bfloat16 if data_type is None else _dtype(data_type)
+    if quantised and dtype != torch.bfloat16:
+        raise ValueError(f"quantised linear layers compute in bfloat16, not {dtype}: pass data_type=\"bf16\" or no linear_config")
     return model.load(src, source, device, dtype)
 
 

@@ -12,12 +12,13 @@ from __future__ import annotations
 
 import dataclasses
 import re
-from typing import Any, Dict, List, Optional
+from typing import Any, Dict, List, Mapping, Optional
 
 import torch
 
 from ..config.model_config import ModelConfig
 from ..config.specs import (BlockSpec, DecoderSpec, FeedForwardSpec, LayerCall, MixerSpec, NormSpec, PositionSpec)
+from ..parts.linear import linear_options
 from ..weights.adapters import register_adapter, register_adapter_step
 from ..weights.sources import TensorLayout
 from . import register_architecture, register_model
@@ -48,8 +49,12 @@ class LLaMAConfig(ModelConfig):
     rope_theta: float = 10_000.0
     rope_scaling: dict = dataclasses.field(default_factory=dict)
     hidden_dim: Optional[int] = None
+    # how the layers' matrices are kept (fms/modules/linear.py:11-156): {"linear_type": "torch_linear" | "fp8" | "int4",
+    # "group_size": a multiple of 32, "int4" only}; embedding and head stay as they are stored
+    linear_config: Optional[Mapping[str, Any]] = dataclasses.field(default_factory=lambda: {"linear_type": "torch_linear"})
 
     def __post_init__(self) -> None:
+        linear_options(self.linear_config)
         if self.nheads <= 0 or self.emb_dim % self.nheads:
             raise ValueError(f"emb_dim {self.emb_dim} must be a multiple of nheads {self.nheads}")
         kv = self.kvheads or self.nheads
@@ -146,11 +151,12 @@ class LLaMA(Model):
         position = PositionSpec("rope", head_dim=c.head_dim, theta=float(c.rope_theta),
                                 max_positions=c.max_expected_seq_len, scaling=tuple(sorted(c.rope_scaling.items())))
         norm = NormSpec("rmsnorm", c.emb_dim, float(c.norm_eps))
+        options = linear_options(c.linear_config)
         block = BlockSpec(
             mixer=MixerSpec("attention", dim=c.emb_dim, nheads=c.nheads, kvheads=c.n_kvheads, head_dim=c.head_dim,
-                            bias=c.attn_bias, window=0, scale=None, position=position),
+                            bias=c.attn_bias, window=0, scale=None, position=position, options=options),
             feed_forward=FeedForwardSpec("glu", dim=c.emb_dim, hidden=c.ffn_hidden, activation=c.activation_fn,
-                                         bias=c.mlp_bias),
+                                         bias=c.mlp_bias, options=options),
             mixer_norm=norm, feed_forward_norm=norm, arrangement="pre_norm",
             names=("ln", "attn", "ff_ln", "ff_sub_layer"),
         )

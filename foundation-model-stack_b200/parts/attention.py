@@ -14,7 +14,8 @@ sequence was cut into steps.
 Interface of a mixer (what a block calls):
 
     cache_request() -> KVRequest | StateRequest | None
-    forward(x, batch, cache_view, writes_cache) -> y       x, y: [tokens, dim] in the compute dtype
+    forward(x, batch, cache_view, writes_cache) -> y       x, y: [tokens, dim] in the compute dtype; where
+        ``takes_quantized_rows`` is set, x may be ``ops.QuantizedRows``
 """
 from __future__ import annotations
 
@@ -43,8 +44,8 @@ class MultiHeadAttention(Part):
         self.window = int(spec.window)
         qkv_rows = (spec.nheads + 2 * spec.kvheads) * spec.head_dim
         in_proj = self.add("in_proj", Part())
-        self.qkv = in_proj.add("qkv_fused", Linear(spec.dim, qkv_rows, spec.bias))
-        self.dense = self.add("dense", Linear(spec.nheads * spec.head_dim, spec.dim, spec.bias))
+        self.qkv = in_proj.add("qkv_fused", Linear(spec.dim, qkv_rows, spec.bias, spec.options))
+        self.dense = self.add("dense", Linear(spec.nheads * spec.head_dim, spec.dim, spec.bias, spec.options))
         # not a child: the encoding has no checkpoint tensors of its own and may be shared
         self.position = build_position(spec.position)
         if self.position.score_bias() is not None:
@@ -54,6 +55,10 @@ class MultiHeadAttention(Part):
     def finalize(self, device, dtype) -> None:
         super().finalize(device, dtype)
         self.position.finalize(device, dtype)
+
+    @property
+    def takes_quantized_rows(self) -> bool:
+        return self.qkv.takes_quantized_rows
 
     def cache_request(self):
         return KVRequest(self.kvheads, self.head_dim, self.window)

@@ -69,7 +69,15 @@ class Part:
         yield from walk(self, prefix)
 
     def state_dict(self) -> Dict[str, torch.Tensor]:
-        return {q: owner._tensors[n] for q, owner, n, _ in self.named_decls() if n in owner._tensors}
+        """Every tensor by its qualified name; of a quantised weight those that it is made of, under its name."""
+        out: Dict[str, torch.Tensor] = {}
+        for q, owner, n, _ in self.named_decls():
+            t = owner._tensors.get(n)
+            if isinstance(t, torch.Tensor):
+                out[q] = t
+            elif t is not None:
+                out.update({f"{q}.{k}": v for k, v in t.tensors().items()})
+        return out
 
     def finalize(self, device: torch.device, dtype: torch.dtype) -> None:
         """Called once after all tensors are set: build derived tables on the device."""

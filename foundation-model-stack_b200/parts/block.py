@@ -48,6 +48,13 @@ from .streams import HyperConnection, StreamMix, StreamSet
 from .token_side import TokenSide
 
 
+def normed_for(sublayer, norm, residual, pending, dtype):
+    """The normed stream as a sublayer takes it: where it multiplies rows of 8 bits, the norm leaves them in the same pass."""
+    if getattr(sublayer, "takes_quantized_rows", False) and hasattr(norm, "apply_quantized"):
+        return norm.apply_quantized(residual, pending, dtype)
+    return norm.apply(residual, pending, dtype)
+
+
 class PreNormBlock(Part):
     def __init__(self, spec: BlockSpec) -> None:
         super().__init__()
@@ -61,9 +68,9 @@ class PreNormBlock(Part):
         return self.mixer.cache_request()
 
     def forward(self, residual, pending, batch, cache_view, writes_cache, dtype):
-        h = self.mixer_norm.apply(residual, pending, dtype)
+        h = normed_for(self.mixer, self.mixer_norm, residual, pending, dtype)
         a = self.mixer.forward(h, batch, cache_view, writes_cache)
-        h = self.feed_forward_norm.apply(residual, a, dtype)
+        h = normed_for(self.feed_forward, self.feed_forward_norm, residual, a, dtype)
         return feed_forward_of(self.feed_forward, h, batch)
 
 

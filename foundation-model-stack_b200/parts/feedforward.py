@@ -9,6 +9,8 @@ Interface of a feed-forward (what a block calls):
     forward(x, sequences)    where ``takes_sequences`` is set: with the step's ``Batch``, or how many rows each sequence has, by which
                              large float32 products choose their kernel (None, or left out: every row stands alone)
 
+Where ``takes_quantized_rows`` is set, x may be ``ops.QuantizedRows``.
+
 A feed-forward with routing implements the same call and keeps router and experts inside.
 
 ``ProjectedUnit`` ("projected_unit"): the hidden values of a feed-forward whose two products a block makes together with
@@ -44,10 +46,14 @@ class GatedLinearUnit(Part):
             raise ValueError(f"activation {spec.activation!r} is not supported; supported: {sorted(ACTIVATIONS)}")
         self.activation = ACTIVATIONS[act]
         self.hidden = spec.hidden
-        self.gate_up = self.add("wg1_fused", Linear(spec.dim, 2 * spec.hidden, spec.bias))
-        self.down = self.add("w2", Linear(spec.hidden, spec.dim, spec.bias))
+        self.gate_up = self.add("wg1_fused", Linear(spec.dim, 2 * spec.hidden, spec.bias, spec.options))
+        self.down = self.add("w2", Linear(spec.hidden, spec.dim, spec.bias, spec.options))
 
     takes_sequences = True
+
+    @property
+    def takes_quantized_rows(self) -> bool:
+        return self.gate_up.takes_quantized_rows
 
     def forward(self, x, sequences=None):
         product = (x, self.gate_up.tensor("weight"), self.gate_up.tensor("bias"), self.activation)

@@ -117,6 +117,12 @@ class RMSNorm(Part):
             return ops.normed_add_rmsnorm(residual, delta.delta, delta.norm.gain(), self.gain(), out_dtype, rows)
         return ops.add_rmsnorm(residual, delta, self.gain_vector(), self.eps, out_dtype, rows)
 
+    def apply_quantized(self, residual, delta, out_dtype, rows=None):
+        """``apply`` whose result leaves as e4m3 rows (``ops.QuantizedRows``), for a product with 8-bit weights."""
+        if isinstance(residual, StreamSet) or isinstance(delta, NormedDelta):
+            return ops.quantize_rows(self.apply(residual, delta, out_dtype, rows))
+        return ops.add_rmsnorm_quantized(residual, None if isinstance(delta, StreamCopy) else delta, self.gain_vector(), self.eps, rows)
+
     def apply_after_sum(self, residual, alpha, parts, out_dtype):
         """residual = norm(alpha * residual + sum of factor * delta over ``parts``), in place; returns the new rows in
         the compute dtype (the stream itself where that is float32)."""

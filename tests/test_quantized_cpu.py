@@ -98,3 +98,56 @@ def test_refusals():
     ):
         with pytest.raises(E):
             call()
+
+
+# ---- a model's configuration -------------------------------------------------------------------------------------------
+def test_linear_config_of_a_model():
+    from fms_b200.models import get_model
+    from fms_b200.models.llama import LLaMA, LLaMAConfig
+    from fms_b200.parts.linear import Linear, linear_options
+
+    assert linear_options(None) == linear_options({"linear_type": "torch_linear"}) == ()
+    assert LLaMA(LLaMAConfig(nlayers=1)).decoder_spec().layers[0].mixer.options == ()
+    spec = LLaMA(LLaMAConfig(nlayers=1), linear_config={"linear_type": "int4", "group_size": 64}).decoder_spec()
+    assert dict(spec.layers[0].mixer.options) == dict(spec.layers[0].feed_forward.options) == {"linear_type": "int4", "group_size": 64}
+    for bad in ({"linear_type": "gptq"}, {"linear_type": "int4", "group_size": 48}, {"linear_type": "fp8", "group_size": 64}, {"linear_type": "int4", "bits": 3}):
+        with pytest.raises(ValueError):
+            LLaMAConfig(linear_config=bad)
+        with pytest.raises(ValueError):
+            get_model("llama", "micro", device_type="cpu", linear_config=bad)
+    with pytest.raises(ValueError, match="bfloat16"):
+        get_model("llama", "tiny-a", device_type="cpu", data_type="fp32", linear_config={"linear_type": "int4"})
+    with pytest.raises(ValueError, match="no quantised"):
+        get_model("goletar", "tiny", device_type="cpu", linear_config={"linear_type": "fp8"})
+    with pytest.raises(ValueError, match="multiple of 8"):
+        Linear(12, 8, options=(("linear_type", "int4"),))
+    with pytest.raises(ValueError):
+        Linear(16, 8, options=(("linear_type", "int3"),))
+
+
+def test_a_layer_quantises_what_it_is_given():
+    from fms_b200.parts.base import Part
+    from fms_b200.parts.linear import Linear
+
+    layer = Linear(72, 40, bias=True, options=(("linear_type", "int4"), ("group_size", 32)))
+    w = torch.randn(40, 72, generator=gen(3)).to(BF16)
+    layer.set_tensor("weight", w)
+    layer.set_tensor("bias", torch.zeros(40, dtype=BF16))
+    want = ops.quantize_int4(w, 32)
+    assert isinstance(layer.tensor("weight"), ops.Int4Weight) and torch.equal(layer.tensor("weight").blocks, want.blocks)
+    assert layer.kernel_libraries(BF16) == ["gemm_int4"] and not layer.by_sequence() and not layer.takes_quantized_rows
+    root = Part()
+    root.add("layer", layer)
+    assert sorted(root.state_dict()) == ["layer.bias", "layer.weight.blocks"]
+    with pytest.raises(ValueError, match="bfloat16"):
+        layer.finalize("cpu", torch.float32)
+    with pytest.raises(ValueError):
+        layer.set_tensor("weight", w[:, :64])
+
+
+def test_the_plain_rounding_to_four_bits_is_the_same():
+    import plain_quantized as pq
+
+    w = (torch.randn(37, 200, generator=gen(4)) * 0.02).to(BF16)
+    for group in (32, 64, 128, 256):
+        assert torch.equal(ops.quantize_int4(w, group).dequantize().double(), pq.int4_of(w, group))
