@@ -17,27 +17,10 @@ constexpr int THREADS = 320, EPILOGUE_WARPS = 8;
 constexpr int BOX_BYTES = TILE * TILE_K;  // 128 rows of an operand for one step
 
 #include "tcgen05.cuh"
+#include "umma_issue.cuh"
 
 // instruction descriptor of kind::f8f6f4: float32 accumulator, e4m3 a and b, both K-major; the shape M x N
 __host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
-__device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
-  const uint32_t acc = accumulate ? 1u : 0u, zero = 0u;
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(tmem_d),
-      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(zero)
-      : "memory");
-}
-// 256 x N x 32 over a pair of blocks: A 128 rows from each block's shared memory, B N/2 rows from each
-__device__ __forceinline__ void umma_e4m3_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
-  const uint32_t acc = accumulate ? 1u : 0u, zero = 0u;
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n}\n" ::"r"(tmem_d),
-      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(zero)
-      : "memory");
-}
-
 // by a whole warp, which gives up as one
 __device__ __forceinline__ bool warp_wait(void* bar, uint32_t parity, volatile int* failed) {
   return __all_sync(0xffffffffu, wait_or_abort(bar, parity, failed));
@@ -203,20 +186,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   } else if (warp == 1) {
     if (leader && elect_one()) {
       const uint32_t idesc = idesc_e4m3(2 * TILE, ep.tile_n);
-      int it = 0, j = 0;
+      const MatrixDesc base(smem_u32(smem));
+      int j = 0, s = 0;
+      uint32_t phase = 0;
       for (int tile = pair; tile < n_tiles && !*failed; tile += pairs, ++j) {
         const int acc = j & 1;
         if (!wait_or_abort(&acc_empty[acc], ((j >> 1) & 1) ^ 1, failed)) break;  // both epilogues have read this buffer
         tc_fence_after();
-        for (int i = 0; i < k_steps; ++i, ++it) {
-          const int s = it % stages;
-          if (!wait_or_abort(&full[s], (it / stages) & 1, failed)) break;
+        for (int i = 0; i < k_steps; ++i) {
+          if (!quick_wait(&full[s], phase, failed)) break;
           tc_fence_after();
-          const uint32_t a = smem_u32(smem + (size_t)s * stage_bytes), b = a + BOX_BYTES;
+          const uint32_t x = base.lo + (uint32_t)(s * stage_bytes >> 4), w = x + (BOX_BYTES >> 4);
 #pragma unroll
           for (int kk = 0; kk < TILE_K / UMMA_K; ++kk)
-            umma_e4m3_pair(tmem + acc * 256, umma_desc(a + kk * UMMA_K), umma_desc(b + kk * UMMA_K), idesc, i > 0 || kk > 0);
+            issue_e4m3_pair(tmem + acc * 256, x + kk * (UMMA_K >> 4), base.hi, w + kk * (UMMA_K >> 4), idesc, kk > 0 ? 1u : i > 0);
           tc_commit_pair(&empty[s]);
+          if (++s == stages) s = 0, phase ^= 1;
         }
         tc_commit_pair(&acc_full[acc]);
       }
@@ -357,15 +342,18 @@ __global__ void __launch_bounds__(THREADS, 2) e4m3_rows_kernel(const __grid_cons
   } else if (warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = idesc_e4m3(TILE, ep.n_tokens);
+      const MatrixDesc base(smem_u32(smem));
+      int s = 0;
+      uint32_t phase = 0;
       for (int i = 0; i < k_steps; ++i) {
-        const int s = i % stages;
-        if (!wait_or_abort(&full[s], (i / stages) & 1, failed)) break;
+        if (!quick_wait(&full[s], phase, failed)) break;
         tc_fence_after();
-        const uint32_t a = smem_u32(smem + (size_t)s * stage_bytes), b = a + BOX_BYTES;
+        const uint32_t w = base.lo + (uint32_t)(s * stage_bytes >> 4), x = w + (BOX_BYTES >> 4);
 #pragma unroll
         for (int kk = 0; kk < TILE_K / UMMA_K; ++kk)
-          umma_e4m3(tmem, umma_desc(a + kk * UMMA_K), umma_desc(b + kk * UMMA_K), idesc, i > 0 || kk > 0);
+          issue_e4m3(tmem, w + kk * (UMMA_K >> 4), base.hi, x + kk * (UMMA_K >> 4), idesc, kk > 0 ? 1u : i > 0);
         tc_commit(&empty[s]);
+        if (++s == stages) s = 0, phase ^= 1;
       }
       tc_commit(acc_full);  // arrives when everything issued so far is done (at once if there was nothing)
     }

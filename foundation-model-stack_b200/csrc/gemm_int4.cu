@@ -20,6 +20,7 @@
 
 namespace {
 #include "tcgen05.cuh"
+#include "umma_issue.cuh"
 
 constexpr int BLOCK_ROWS = 16, BLOCK_K = 128, WEIGHT_BYTES = 1024;
 
@@ -277,15 +278,6 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
 __device__ __forceinline__ bool warp_wait(void* bar, uint32_t parity, volatile int* failed) {
   return __all_sync(0xffffffffu, wait_or_abort(bar, parity, failed));
 }
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t local_addr, uint32_t rank) {
-  float4 v;
-  asm volatile(
-      "{\n.reg .b32 remote;\nmapa.shared::cluster.u32 remote, %4, %5;\nld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [remote];\n}\n"
-      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-      : "r"(local_addr), "r"(rank)
-      : "memory");
-  return v;
-}
 // 32 columns of 32 bits of this thread's lane of tensor memory, written; not waited for
 __device__ __forceinline__ void tmem_store_pairs(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -356,21 +348,31 @@ template <int N> __device__ __forceinline__ void store_column(const Int4Args& p,
     if (row0 + j < p.M && FMS_IN(at + j * pitch, (size_t)p.M * pitch)) p.y[at + j * pitch] = __float2bfloat16_rn(v[j] + bias);
 }
 
-// ---- 9 to 256 rows -----------------------------------------------------------------------------------------------------
-//   warp 0      per step of 128 k: two 64-k boxes of x and one of the eight blocks of w, into one of up to 8 stages
+// ---- 9 to 256 rows ------------------------------------------------------------------------------------------------------
+// One thread block a multiprocessor; each takes an equal run of the steps of all tiles, a step being 128 rows of w by 128 k, so that
+// no multiprocessor waits for another's second tile (28,672 rows are 224 tiles for 148).  Where a tile's steps fall to several
+// blocks, each leaves its sums in a slot of its own in scratch memory, and a second kernel adds them in the order of k.  The
+// cut depends on the weights' shape alone, so a row's result does not depend on the rest of the batch.
+//   warp 0      per step: two 64-k boxes of x and one of the eight blocks of w, into one of up to 8 stages
 //   warp 1      one lane issues 8 instructions (128 x tokens x 16) a step
-//   warps 2-17  up to four groups of four unpack every fourth step each, a thread a row of w, into the group's quarter of the
-//               operand's 256 columns (two groups took 2,500 cycles a step, most of it waiting for one another); then they
-//               read the accumulator.  A group waits for its columns before it waits for a step's copies: the steps up to its last
-//               one are used up then, and with no more groups than stages the copies' barrier cannot be a phase behind.  The ks blocks of a tile (a cluster) add their sums through distributed shared memory.
-// Every wait on an mbarrier is bounded: on a time-out the block records error 4, skips the rest of its work and still meets
-// the cluster's barriers and frees its tensor memory.
-constexpr int GROUPS = 4, UNPACK_WARPS = 4 * GROUPS, ROWS_THREADS = 64 + 32 * UNPACK_WARPS, MAX_STAGES = 8, MAX_KS = 4, A_FIRST = 256;
+//   warps 2-17  up to four groups of four unpack every fourth step each, a thread a row of w, into the next of up to 7 stages of the
+//               operand, 64 columns each: what the accumulators leave of the 512 (with a stage a group, a group waited for its
+//               own step's products before it went on: 800 cycles a step).  A group waits for its columns before it waits for a
+//               step's copies: the steps up to `a_stages` before are used up then, and with no fewer copies' stages and no more
+//               groups than that, neither barrier can be a phase behind.
+//   warps 18-21 the epilogue; two accumulators up to 64 tokens, so that it runs under the next tile's steps
+// Every wait on an mbarrier is bounded: on a time-out the block records error 4, skips the rest of its work and still frees its
+// tensor memory.
+constexpr int GROUPS = 4, UNPACK_WARPS = 4 * GROUPS, ROWS_THREADS = 64 + 32 * (UNPACK_WARPS + 4), MAX_STAGES = 8, A_FIRST = 256, MAX_A = 7;
 
 struct RowsArgs {
   Int4Args p;
-  int n_tokens, stages, ks, groups;
+  int n_tokens, stages, groups, a_stages, accs, acc_columns;
+  float* scratch;  // [2 blocks][n_tokens][128]: a block's first tile, then its last, where it has not all of it
 };
+// The run of steps of block b of `blocks`: [first_step(b), first_step(b + 1)); and the block of a step
+__host__ __device__ inline int first_step(int b, int blocks, int steps) { return (int)((long)b * steps / blocks); }
+__device__ __forceinline__ int block_of_step(int step, int blocks, int steps) { return (int)((((long)step + 1) * blocks - 1) / steps); }
 
 __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid_constant__ CUtensorMap map_x,
                                                                     const __grid_constant__ CUtensorMap map_w, RowsArgs a,
@@ -378,22 +380,21 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = smem_unaligned + (-smem_u32(smem_unaligned) & 1023);
   const Int4Args& p = a.p;
-  const int bytes = p.block_bytes(), x_bytes = a.n_tokens * BLOCK_K * 2, stages = a.stages, ks = a.ks;
+  const int bytes = p.block_bytes(), x_bytes = a.n_tokens * BLOCK_K * 2, stages = a.stages;
   const int stage_bytes = (x_bytes + TILE / BLOCK_ROWS * bytes + 1023) / 1024 * 1024;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + stages * stage_bytes);
   uint64_t* empty = full + MAX_STAGES;
-  uint64_t* a_full = empty + MAX_STAGES;  // [GROUPS]
-  uint64_t* a_empty = a_full + GROUPS;    // [GROUPS]
-  uint64_t* acc_full = a_empty + GROUPS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  uint64_t* a_full = empty + MAX_STAGES;  // [MAX_A]
+  uint64_t* a_empty = a_full + MAX_A;     // [MAX_A]
+  uint64_t* acc_full = a_empty + MAX_A;   // [2]
+  uint64_t* acc_empty = acc_full + 2;     // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   __shared__ int failed_flag;
   volatile int* failed = &failed_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = ks > 1 ? (int)cluster_rank() : 0;
-  const int n0 = blockIdx.y * TILE;
-  const int each = (p.k_blocks + ks - 1) / ks;
-  const int step_lo = min(rank * each, p.k_blocks), k_steps = min(step_lo + each, p.k_blocks) - step_lo;  // may be 0
+  const int all = (p.N + TILE - 1) / TILE * p.k_blocks;
+  const int lo = first_step(blockIdx.x, gridDim.x, all), hi = first_step(blockIdx.x + 1, gridDim.x, all);
 
   if (threadIdx.x == 0) {
     failed_flag = 0;
@@ -401,138 +402,123 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int i = 0; i < GROUPS; ++i) {
+    for (int i = 0; i < MAX_A; ++i) {
       mbar_init(&a_full[i], 4);  // the warps of a group
       mbar_init(&a_empty[i], 1);
     }
-    mbar_init(acc_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4);  // the warps of the epilogue
+    }
     mbar_fence_init();
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot, tmem_a = tmem + A_FIRST;
+  const uint32_t tmem = *tmem_slot, tmem_a = tmem + a.accs * a.acc_columns;
   pdl_launch_dependents();  // now: a block of the next kernel must not take the tensor memory that this one still needs
 
   if (warp == 0) {
     if (elect_one()) {
-      auto load_w = [&](int i) {
-        const int s = i % stages;
-        mbar_arrive_expect_tx(&full[s], x_bytes + TILE / BLOCK_ROWS * bytes);
-        tma_load_3d(smem + s * stage_bytes + x_bytes, &map_w, 0, step_lo + i, n0 / BLOCK_ROWS, &full[s]);
+      int tile = lo / p.k_blocks, k = lo - tile * p.k_blocks, s = 0;
+      auto load_w = [&](int to, int t, int kb) {
+        mbar_arrive_expect_tx(&full[to], x_bytes + TILE / BLOCK_ROWS * bytes);
+        tma_load_3d(smem + to * stage_bytes + x_bytes, &map_w, 0, kb, t * (TILE / BLOCK_ROWS), &full[to]);
       };
-      auto load_x = [&](int i) {
-        const int s = i % stages;
-        unsigned char* to = smem + s * stage_bytes;
-        tma_load_2d(to, &map_x, (step_lo + i) * BLOCK_K, 0, &full[s]);
-        tma_load_2d(to + x_bytes / 2, &map_x, (step_lo + i) * BLOCK_K + 64, 0, &full[s]);
+      auto load_x = [&](int to, int kb) {
+        tma_load_2d(smem + to * stage_bytes, &map_x, kb * BLOCK_K, 0, &full[to]);
+        tma_load_2d(smem + to * stage_bytes + x_bytes / 2, &map_x, kb * BLOCK_K + 64, 0, &full[to]);
       };
-      const int early = min(stages, k_steps);
-      for (int i = 0; i < early; ++i) load_w(i);  // weights do not depend on the kernel before
+      const int early = min(stages, hi - lo);
+      for (int i = 0, t = tile, kb = k; i < early; ++i) {  // weights do not depend on the kernel before
+        load_w(i, t, kb);
+        if (++kb == p.k_blocks) kb = 0, ++t;
+      }
       pdl_wait();
-      for (int i = 0; i < early; ++i) load_x(i);
-      for (int i = early; i < k_steps && !*failed; ++i) {
-        if (!wait_or_abort(&empty[i % stages], ((i / stages) & 1) ^ 1, failed)) break;
-        load_w(i);
-        load_x(i);
+      uint32_t phase = 1;
+      for (int i = lo; i < hi && !*failed; ++i) {
+        if (i - lo >= early) {
+          if (!wait_or_abort(&empty[s], phase, failed)) break;
+          load_w(s, tile, k);
+        }
+        load_x(s, k);
+        if (++k == p.k_blocks) k = 0, ++tile;
+        if (++s == stages) s = 0, phase ^= 1;
       }
     }
   } else if (warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = umma_idesc(TILE, a.n_tokens);
-      int s = 0, group = 0;
-      uint32_t phase = 0, turn = 0;
-      for (int i = 0; i < k_steps; ++i) {
-        if (!wait_or_abort(&full[s], phase, failed)) break;
-        if (!wait_or_abort(&a_full[group], turn, failed)) break;
+      const MatrixDesc base(smem_u32(smem));
+      const uint32_t box = (uint32_t)x_bytes / 2 >> 4;
+      int k = lo % p.k_blocks, s = 0, stage = 0, acc = 0;
+      uint32_t phase = 0, turn = 0, acc_phase = 1;
+      for (int i = lo; i < hi; ++i) {
+        const bool first = i == lo || k == 0;
+        if (first && !wait_or_abort(&acc_empty[acc], acc_phase, failed)) break;
+        if (!quick_wait(&full[s], phase, failed) || !quick_wait(&a_full[stage], turn, failed)) break;
         tc_fence_after();
-        const uint32_t b = smem_u32(smem + s * stage_bytes);
+        const uint32_t d = tmem + acc * a.acc_columns, ta = tmem_a + stage * A_COLUMNS, b = base.lo + (uint32_t)(s * stage_bytes >> 4);
 #pragma unroll
-        for (int kk = 0; kk < BLOCK_K / 16; ++kk)
-          umma_a_tmem(tmem, tmem_a + group * A_COLUMNS + kk * 8, umma_desc(b + (kk >> 2) * (x_bytes / 2) + (kk & 3) * 32), idesc, i > 0 || kk > 0);
+        for (int kk = 0; kk < BLOCK_K / 16; ++kk)  // 64 k a box of x, 32 bytes of its rows an instruction
+          issue_a_tmem(d, ta + kk * 8, b + (kk & 3) * 2 + (kk < 4 ? 0 : box), base.hi, idesc, kk > 0 ? 1u : !first);
         tc_commit(&empty[s]);
-        tc_commit(&a_empty[group]);
+        tc_commit(&a_empty[stage]);
+        if (++k == p.k_blocks) k = 0;
+        if (k == 0 || i + 1 == hi) {
+          tc_commit(&acc_full[acc]);
+          if (++acc == a.accs) acc = 0, acc_phase ^= 1;
+        }
         if (++s == stages) s = 0, phase ^= 1;
-        if (++group == a.groups) group = 0, turn ^= 1;
+        if (++stage == a.a_stages) stage = 0, turn ^= 1;
       }
-      tc_commit(acc_full);
     }
-  } else {
+  } else if (warp < 2 + UNPACK_WARPS) {
     const int group = (warp - 2) >> 2;
-    int s = group;  // no more groups than stages
+    int s = group, stage = group;  // groups <= a_stages <= stages
     uint32_t phase = 0, turn = 1;
-    for (int i = group < a.groups ? group : k_steps; i < k_steps; i += a.groups) {
-      if (!warp_wait(&a_empty[group], turn, failed)) break;
+    for (int i = group < a.groups ? lo + group : hi; i < hi; i += a.groups) {
+      if (!warp_wait(&a_empty[stage], turn, failed)) break;
       if (!warp_wait(&full[s], phase, failed)) break;
-      unpack_row(smem + s * stage_bytes + x_bytes, bytes, p.per, warp & 3, lane, tmem_a + group * A_COLUMNS);
-      if (lane == 0) mbar_arrive(&a_full[group]);
-      turn ^= 1;
+      unpack_row(smem + s * stage_bytes + x_bytes, bytes, p.per, warp & 3, lane, tmem_a + stage * A_COLUMNS);
+      if (lane == 0) mbar_arrive(&a_full[stage]);
       s += a.groups;
       if (s >= stages) s -= stages, phase ^= 1;
+      stage += a.groups;
+      if (stage >= a.a_stages) stage -= a.a_stages, turn ^= 1;
+    }
+  } else {
+    pdl_wait();  // y and the scratch memory may be what the kernel before still uses
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int i = lo; i < hi;) {
+      const int tile = i / p.k_blocks, k_lo = i - tile * p.k_blocks, k_hi = min(p.k_blocks, hi - tile * p.k_blocks);
+      const int col = tile * TILE + row;
+      const bool whole = k_lo == 0 && k_hi == p.k_blocks;
+      float* slot = a.scratch + ((size_t)(2 * blockIdx.x + (i == lo ? 0 : 1)) * a.n_tokens) * TILE + row;
+      const float bias = whole && p.bias && col < p.N ? __bfloat162float(p.bias[col]) : 0.f;
+      if (!warp_wait(&acc_full[acc], acc_phase, failed)) break;
+      tc_fence_after();
+      for (int c0 = 0; c0 < a.n_tokens; c0 += 16) {
+        float v[16];
+        tmem_load_16(tmem + acc * a.acc_columns + ((uint32_t)(quarter * 32) << 16) + c0, v);
+        if (whole) {
+          if (col < p.N) store_column<16>(p, v, c0, col, bias);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) slot[(size_t)(c0 + j) * TILE] = v[j];
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[acc]);
+      if (++acc == a.accs) acc = 0, acc_phase ^= 1;
+      i += k_hi - k_lo;
     }
   }
-  // The sums leave tensor memory as they are where a block has them whole; else they meet in shared memory, as float32
-  // [128][n_tokens + 4] over the stages (every copy into them has landed and every instruction that read them is done once the
-  // accumulator is ready).  Thread: a row of w, runs of 8 or 16 tokens.
-  float* red = reinterpret_cast<float*>(smem);
-  const int red_stride = a.n_tokens + 4;
-  if (warp >= 2) {
-    pdl_wait();  // y may be what the kernel before still reads
-    const int quarter = warp & 3, row = quarter * 32 + lane, col = n0 + row;
-    const bool live = col < p.N;
-    const float bias = live && p.bias ? __bfloat162float(p.bias[col]) : 0.f;
-    const bool ok = warp_wait(acc_full, 0, failed);
-    tc_fence_after();
-    for (int c0 = 16 * ((warp - 2) >> 2); c0 < a.n_tokens; c0 += 16 * GROUPS) {
-      float v[16];
-      if (ok && k_steps > 0) {
-        tmem_load_16(tmem + ((uint32_t)(quarter * 32) << 16) + c0, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = 0.f;
-      }
-      if (ks > 1) {
-#pragma unroll
-        for (int j = 0; j < 16; j += 4)
-          *reinterpret_cast<float4*>(red + row * red_stride + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-      } else if (ok && live) {
-        store_column<16>(p, v, c0, col, bias);
-      }
-    }
-    tc_fence_before();
-  }
-  if (ks > 1) {
-    __syncthreads();
-    cluster_sync_all();
-    if (warp >= 2 && !*failed) {  // this block's share of the tokens, 8 at a time
-      const int e = threadIdx.x - 64, i = e & 127, col = n0 + i, share = ((a.n_tokens + ks - 1) / ks + 7) / 8 * 8;
-      const int t_hi = min((rank + 1) * share, a.n_tokens);
-      const bool live = col < p.N;
-      const float bias = live && p.bias ? __bfloat162float(p.bias[col]) : 0.f;
-      for (int t = rank * share + 8 * (e >> 7); t < t_hi; t += 8 * GROUPS) {
-        float4 v[MAX_KS][2];
-        const uint32_t at = smem_u32(red) + (uint32_t)(i * red_stride + t) * 4u;
-#pragma unroll
-        for (int r = 0; r < MAX_KS; ++r)  // all loads on their way before the first sum
-          if (r < ks) {
-            v[r][0] = ld_cluster_f32x4(at, (uint32_t)r);
-            v[r][1] = ld_cluster_f32x4(at + 16, (uint32_t)r);
-          }
-        float sum[8] = {};
-#pragma unroll
-        for (int r = 0; r < MAX_KS; ++r)
-          if (r < ks) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              sum[4 * h] += v[r][h].x; sum[4 * h + 1] += v[r][h].y; sum[4 * h + 2] += v[r][h].z; sum[4 * h + 3] += v[r][h].w;
-            }
-          }
-        if (live) store_column<8>(p, sum, t, col, bias);
-      }
-    }
-    cluster_sync_all();  // nobody leaves while another block still reads its shared memory
-  }
+  tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *failed && error_flag) atomicExch(error_flag, 4);
   if (warp == 1) {
@@ -541,44 +527,74 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid
   }
 }
 
+// y of the tiles that several blocks share: their sums in the order of k, + bias.  Block: a tile's 128 columns of y by 4 tokens; the
+// slots of four blocks are on their way at a time (one after another they took 9 us of 23).
+__global__ void __launch_bounds__(TILE) int4_join_kernel(RowsArgs a, int blocks) {
+  pdl_launch_dependents();
+  const Int4Args& p = a.p;
+  const int all = (p.N + TILE - 1) / TILE * p.k_blocks, tile = blockIdx.x, start = tile * p.k_blocks;
+  const int from = block_of_step(start, blocks, all), to = block_of_step(start + p.k_blocks - 1, blocks, all);
+  const int col = tile * TILE + (int)threadIdx.x, t0 = blockIdx.y * 4;
+  if (from == to || col >= p.N || t0 >= p.M) return;  // some block of some tile goes on, and waits
+  const float bias = p.bias ? __bfloat162float(p.bias[col]) : 0.f;
+  // only the first block of a tile can have begun with an earlier one
+  const int head = first_step(from, blocks, all) / p.k_blocks == tile ? 0 : 1;
+  const float* slots = a.scratch + (size_t)t0 * TILE + threadIdx.x;
+  const size_t pitch = (size_t)a.n_tokens * TILE;
+  pdl_wait();
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int b = from; b <= to; b += 4) {
+    float v[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = b + i <= to ? __ldcg(slots + (2 * (b + i) + (b + i == from ? head : 0)) * pitch + j * TILE) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] += v[i][j];
+  }
+  store_column<4>(p, sum, t0, col, bias);
+}
+
 // A block that holds all of the tensor memory takes so much shared memory that no block that wants some fits beside it: one that
 // waits for it could be what this one waits for (the others of a cluster, the kernel before).
 constexpr size_t SMEM_LEAST = 200 * 1024, SMEM_MOST = 225 * 1024, EXTRA = 1024 /* alignment */ + 512 /* barriers */;
 
-int launch_rows(const Int4Args& p, int* error_flag, cudaStream_t stream) {
+constexpr int ROWS_MOST = 256;  // rows of x
+int rows_blocks(int N, int K) {
+  const long steps = (long)((N + TILE - 1) / TILE) * ((K + BLOCK_K - 1) / BLOCK_K);
+  const int sms = multiprocessors();
+  return steps < sms ? (int)steps : sms;
+}
+long rows_scratch(int M, int N, int K) { return 2L * rows_blocks(N, K) * ((M + 15) / 16 * 16) * TILE; }
+
+int launch_rows(const Int4Args& p, float* scratch, long scratch_floats, int* error_flag, cudaStream_t stream) {
   RowsArgs a = {};
   a.p = p;
   a.n_tokens = (p.M + 15) / 16 * 16;
-  const int tiles = (p.N + TILE - 1) / TILE;
-  if (tiles > 65535) return fms_fail("gemm_int4: %d tiles of rows of w", tiles);
-  a.ks = 1;  // from the weights' shape alone, as many as fill most of the multiprocessors, each with 4 steps at least
-  while (a.ks < MAX_KS && tiles * a.ks < 120 && p.k_blocks / (a.ks * 2) >= 4) a.ks *= 2;
+  a.scratch = scratch;
+  const int tiles = (p.N + TILE - 1) / TILE, blocks = rows_blocks(p.N, p.K);
+  if ((long)tiles * p.k_blocks > 0x3fffffffL) return fms_fail("gemm_int4: %d tiles of %d blocks", tiles, p.k_blocks);
+  if (scratch_floats < rows_scratch(p.M, p.N, p.K)) return fms_fail("gemm_int4: %ld floats of scratch memory, %ld are wanted", scratch_floats, rows_scratch(p.M, p.N, p.K));
   const int stage_bytes = (a.n_tokens * BLOCK_K * 2 + TILE / BLOCK_ROWS * p.block_bytes() + 1023) / 1024 * 1024;
   a.stages = min((int)((SMEM_MOST - EXTRA) / stage_bytes), MAX_STAGES);
-  a.groups = min(GROUPS, a.stages);
-  const size_t stages_bytes = (size_t)a.stages * stage_bytes, red_bytes = a.ks > 1 ? (size_t)TILE * (a.n_tokens + 4) * sizeof(float) : 0;
-  if (a.stages < 2 || red_bytes > stages_bytes) return fms_fail("gemm_int4: no room for %d tokens", a.n_tokens);
+  a.acc_columns = (a.n_tokens + 31) / 32 * 32;
+  a.accs = a.n_tokens <= 64 ? 2 : 1;
+  a.a_stages = min(min(MAX_A, (512 - a.accs * a.acc_columns) / A_COLUMNS), a.stages);
+  a.groups = min(GROUPS, a.a_stages);
   CUtensorMap map_x, map_w;
   if (make_map(&map_x, p.x, p.M, p.K, a.n_tokens) || make_block_map(&map_w, p)) return 1;
   static uint64_t allowed = 0;
   if (allow_smem(int4_rows_kernel, (int)SMEM_MOST, &allowed)) return 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.ks, tiles);
-  cfg.blockDim = dim3(ROWS_THREADS);
-  cfg.dynamicSmemBytes = stages_bytes + EXTRA < SMEM_LEAST ? SMEM_LEAST : stages_bytes + EXTRA;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = a.ks;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = fms_pdl_enabled() ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, int4_rows_kernel, map_x, map_w, a, error_flag);
-  if (e != cudaSuccess) return fms_fail("gemm_int4: launch failed: %s", cudaGetErrorString(e));
-  return fms_launch_status("gemm_int4");
+  const size_t smem = (size_t)a.stages * stage_bytes + EXTRA;
+  fms_launch(int4_rows_kernel, dim3(blocks), dim3(ROWS_THREADS), smem < SMEM_LEAST ? SMEM_LEAST : smem, stream, map_x, map_w, a, error_flag);
+  if (fms_launch_status("gemm_int4")) return 1;
+  bool shared = false;  // whether any tile's steps fall to two blocks
+  for (int b = 1; b < blocks && !shared; ++b) shared = first_step(b, blocks, tiles * p.k_blocks) % p.k_blocks != 0;
+  if (!shared) return 0;
+  fms_launch(int4_join_kernel, dim3(tiles, a.n_tokens / 4), dim3(TILE), 0, stream, a, blocks);
+  return fms_launch_status("gemm_int4_join");
 }
 
 // ---- more rows (prefill) ------------------------------------------------------------------------------------------------
@@ -593,15 +609,6 @@ int launch_rows(const Int4Args& p, int* error_flag, cudaStream_t stream) {
 //   warps 2-17  four groups of four unpack every fourth step each: a thread a row of w
 //   warps 18-25 the epilogue, a warp a row's 32 lanes and every second 16 tokens
 constexpr int PAIR_EPILOGUE = 8, PAIR_THREADS = 64 + 32 * (UNPACK_WARPS + PAIR_EPILOGUE), PAIR_TOKENS = 256;
-
-__device__ __forceinline__ void umma_pair_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, bool accumulate) {
-  const uint32_t acc = accumulate ? 1u : 0u, zero = 0u;
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(acc), "r"(zero)
-      : "memory");
-}
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     int4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, RowsArgs a,
@@ -673,19 +680,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   } else if (warp == 1) {
     if (leader && elect_one()) {
       const uint32_t idesc = umma_idesc(2 * TILE, a.n_tokens);
+      const MatrixDesc base(smem_u32(smem));
+      const uint32_t box = (uint32_t)x_bytes / 2 >> 4;
       int j = 0, s = 0, group = 0;
       uint32_t phase = 0, turn = 0;
       for (int tile = pair; tile < n_tiles && !*failed; tile += pairs, ++j) {
         if (!wait_or_abort(acc_empty, (j & 1) ^ 1, failed)) break;  // both epilogues have read the tile before
         for (int i = 0; i < k_steps; ++i) {
-          if (!wait_or_abort(&x_full[s], phase, failed)) break;
-          if (!wait_or_abort(&a_full[group], turn, failed)) break;
+          if (!quick_wait(&x_full[s], phase, failed) || !quick_wait(&a_full[group], turn, failed)) break;
           tc_fence_after();
-          const uint32_t b = smem_u32(smem + s * stage_bytes);
+          const uint32_t ta = tmem_a + group * A_COLUMNS, b = base.lo + (uint32_t)(s * stage_bytes >> 4);
 #pragma unroll
           for (int kk = 0; kk < BLOCK_K / 16; ++kk)
-            umma_pair_a_tmem(tmem, tmem_a + group * A_COLUMNS + kk * 8, umma_desc(b + (kk >> 2) * (x_bytes / 2) + (kk & 3) * 32), idesc,
-                             i > 0 || kk > 0);
+            issue_a_tmem_pair(tmem, ta + kk * 8, b + (kk & 3) * 2 + (kk < 4 ? 0 : box), base.hi, idesc, kk > 0 ? 1u : i > 0);
           tc_commit_pair(&empty[s]);
           tc_commit_pair(&a_empty[group]);
           if (++s == stages) s = 0, phase ^= 1;
@@ -778,17 +785,20 @@ int check(const Int4Args& p) {
   if (((uintptr_t)p.x | (uintptr_t)p.w) & 15) return fms_fail("gemm_int4: operands must be 16-byte aligned");
   return 0;
 }
-constexpr int SOME_ROWS = 256;  // rows of x up to which the second kernel takes the product
 }  // namespace
+
+// Floats of scratch memory that fms_linear_int4 wants.
+FMS_API long fms_linear_int4_scratch(int M, int N, int K) { return M <= FEW_ROWS || M > ROWS_MOST || N <= 0 || K <= 0 ? 0 : rows_scratch(M, N, K); }
 
 // y [M, N] bfloat16 of x [M, K] bfloat16, w packed with `per` scales a block, bias [N] bfloat16 or null.
 FMS_API int fms_linear_int4(const void* x, const void* w, const void* bias, void* y, int M, int N, int K, int k_blocks, int per,
-                            int* error_flag, cudaStream_t stream) {
+                            float* scratch, long scratch_floats, int* error_flag, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
   const Int4Args p = {(const __nv_bfloat16*)x, (const unsigned char*)w, (const __nv_bfloat16*)bias, (__nv_bfloat16*)y,
                       M, N, K, k_blocks, per, N, 0};
   if (check(p)) return 1;
-  return M <= FEW_ROWS ? few<false>(p, stream) : (M <= SOME_ROWS ? launch_rows(p, error_flag, stream) : launch_pair(p, error_flag, stream));
+  return M <= FEW_ROWS ? few<false>(p, stream)
+                       : (M <= ROWS_MOST ? launch_rows(p, scratch, scratch_floats, error_flag, stream) : launch_pair(p, error_flag, stream));
 }
 
 // y [M, hidden] = act(gate) * up for w = [gate; up] of 2 hidden rows, hidden a multiple of 16, up to 8 rows of x.

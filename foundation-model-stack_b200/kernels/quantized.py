@@ -14,6 +14,7 @@ refused.  ``linear``, ``gated_linear`` and ``activated_linear`` (kernels/ops.py)
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
@@ -342,9 +343,28 @@ def linear_int4(x: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor
     bias = _int4_checked("linear_int4", x, weight, bias)
     (n, k), blocks = weight.shape, weight.blocks
     y = torch.empty_strided((x.shape[0], n), (n, 1), dtype=torch.bfloat16, device=x.device)
-    ops._call("gemm_int4", "fms_linear_int4", x, blocks, bias, y, x.shape[0], n, k, blocks.shape[1], weight.per,
+    floats = _int4_scratch(x.shape[0], n, k)
+    # for sums that several thread blocks share: of this call alone, so that calls at once and captured graphs do not meet in it
+    scratch = torch.empty_strided((floats,), (1,), dtype=torch.float32, device=x.device) if floats else None
+    ops._call("gemm_int4", "fms_linear_int4", x, blocks, bias, y, x.shape[0], n, k, blocks.shape[1], weight.per, scratch, floats,
               ops.error_flag(x.device), ops._stream())
     return y
+
+
+def _int4_scratch(rows: int, n: int, k: int) -> int:
+    if rows <= INT4_FEW_ROWS:
+        return 0
+    f = _int4_scratch_of.get(ops._device())
+    if f is None:
+        from .build import load_library
+
+        f = load_library("gemm_int4").fms_linear_int4_scratch
+        f.restype, f.argtypes = ctypes.c_long, [ctypes.c_int] * 3
+        _int4_scratch_of[ops._device()] = f
+    return f(rows, n, k)
+
+
+_int4_scratch_of = {}  # by device
 
 
 def gated_linear_int4(x: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor], activation: int) -> torch.Tensor:
