@@ -348,7 +348,7 @@ template <int N> __device__ __forceinline__ void store_column(const Int4Args& p,
     if (row0 + j < p.M && FMS_IN(at + j * pitch, (size_t)p.M * pitch)) p.y[at + j * pitch] = __float2bfloat16_rn(v[j] + bias);
 }
 
-// ---- 9 to 256 rows ------------------------------------------------------------------------------------------------------
+// ---- 9 to 112 or 256 rows ------------------------------------------------------------------------------------------------------
 // One thread block a multiprocessor; each takes an equal run of the steps of all tiles, a step being 128 rows of w by 128 k, so that
 // no multiprocessor waits for another's second tile (28,672 rows are 224 tiles for 148).  Where a tile's steps fall to several
 // blocks, each leaves its sums in a slot of its own in scratch memory, and a second kernel adds them in the order of k.  The
@@ -561,7 +561,10 @@ __global__ void __launch_bounds__(TILE) int4_join_kernel(RowsArgs a, int blocks)
 // waits for it could be what this one waits for (the others of a cluster, the kernel before).
 constexpr size_t SMEM_LEAST = 200 * 1024, SMEM_MOST = 225 * 1024, EXTRA = 1024 /* alignment */ + 512 /* barriers */;
 
-constexpr int ROWS_MOST = 256;  // rows of x
+// The most rows of x that this kernel takes: 256, but 112 where the pairs of the kernel below have a tile each.  This one / that one in
+// us, by rows: 28,672 x 4,096 96 31.8 / 32.3, 128 38.7 / 32.4, 256 72.2 / 60.6; 6,144 x 4,096 128 13.0 / 16.3, 256 19.5 / 17.3; 4,096 x
+// 14,336 128 19.9 / 42.9, 256 29.7 / 44.7.
+int rows_most(int N) { return (long)N >= 2L * TILE * (multiprocessors() / 2) ? 112 : 256; }
 int rows_blocks(int N, int K) {
   const long steps = (long)((N + TILE - 1) / TILE) * ((K + BLOCK_K - 1) / BLOCK_K);
   const int sms = multiprocessors();
@@ -754,11 +757,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 int launch_pair(const Int4Args& p, int* error_flag, cudaStream_t stream) {
   RowsArgs a = {};
   a.p = p;
-  // the width whose tiles cost least in whole rounds of the pairs; below some 144 tokens a step takes what unpacking takes
+  // the width whose tiles cost least in whole rounds of the pairs; below some 100 tokens a step takes what unpacking takes
   const int pairs = max(multiprocessors() / 2, 1), tiles_n = (p.N + 2 * TILE - 1) / (2 * TILE);
   long best = -1;
   for (int tn = PAIR_TOKENS; tn >= 64; tn -= 16) {
-    const long tiles = (long)tiles_n * ((p.M + tn - 1) / tn), cost = (tiles + pairs - 1) / pairs * (max(tn, 144) + 24);
+    const long tiles = (long)tiles_n * ((p.M + tn - 1) / tn), cost = (tiles + pairs - 1) / pairs * (max(tn, 100) + 24);
     if (best < 0 || cost < best) {
       best = cost;
       a.n_tokens = tn;
@@ -788,7 +791,7 @@ int check(const Int4Args& p) {
 }  // namespace
 
 // Floats of scratch memory that fms_linear_int4 wants.
-FMS_API long fms_linear_int4_scratch(int M, int N, int K) { return M <= FEW_ROWS || M > ROWS_MOST || N <= 0 || K <= 0 ? 0 : rows_scratch(M, N, K); }
+FMS_API long fms_linear_int4_scratch(int M, int N, int K) { return M <= FEW_ROWS || N <= 0 || K <= 0 || M > rows_most(N) ? 0 : rows_scratch(M, N, K); }
 
 // y [M, N] bfloat16 of x [M, K] bfloat16, w packed with `per` scales a block, bias [N] bfloat16 or null.
 FMS_API int fms_linear_int4(const void* x, const void* w, const void* bias, void* y, int M, int N, int K, int k_blocks, int per,
@@ -798,7 +801,7 @@ FMS_API int fms_linear_int4(const void* x, const void* w, const void* bias, void
                       M, N, K, k_blocks, per, N, 0};
   if (check(p)) return 1;
   return M <= FEW_ROWS ? few<false>(p, stream)
-                       : (M <= ROWS_MOST ? launch_rows(p, scratch, scratch_floats, error_flag, stream) : launch_pair(p, error_flag, stream));
+                       : (M <= rows_most(N) ? launch_rows(p, scratch, scratch_floats, error_flag, stream) : launch_pair(p, error_flag, stream));
 }
 
 // y [M, hidden] = act(gate) * up for w = [gate; up] of 2 hidden rows, hidden a multiple of 16, up to 8 rows of x.

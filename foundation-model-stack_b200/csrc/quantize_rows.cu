@@ -10,9 +10,11 @@
 //
 // Both are bound by memory: a value is read once (2 or 4 bytes, behind the norm 4 and 2 or 4), the stream written (4) and
 // one byte stored.  A thread block owns a row and keeps it in registers, as it was loaded, between the maximum and the rounding,
-// so that nothing is read twice.  A thread owns runs of 8 neighbours, 16-byte loads and 8-byte stores; where an array's rows do
-// not begin on 16 bytes, 8 values a whole block apart, so that a warp's single loads and stores are neighbours.  Rows of q are
-// `pitch` bytes apart, dim rounded up to 16 with zeros behind the last value, as the products' copies want them.
+// so that nothing is read twice.  A thread owns runs of 8 neighbours, 16-byte loads and 8-byte stores.  Rows of a width that is no
+// multiple of 8 begin anywhere: their runs are moved forward by up to 3 values to where the rows' own loads are aligned, and a
+// warp's lanes hand one another the bytes that make aligned stores (1,100 x 5,001 bfloat16 7.7 us, and behind the norm, float32,
+// 22.9; 11.4 and 25.1 with single loads and stores).  Rows of q are `pitch` bytes apart, dim rounded up to 16 with zeros behind the last value, as the products'
+// copies want them.
 //
 // q is what the exact quotient rounds to.  Of bfloat16 rows it is often a tie, and otherwise, a ratio of numbers of 11 and 8 bits,
 // at least 2^-13 away from one, so one step of Newton's, whose remainder x * 448 - q0 * max |x| is exact in a fused
@@ -47,6 +49,8 @@ template <> struct Run<float> {
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
+  static __device__ __forceinline__ bool aligned(const float* p) { return ((uintptr_t)p & 15) == 0; }
+  __device__ __forceinline__ void load_halves(const float* p) { load(p); }
 };
 template <> struct Run<__nv_bfloat16> {
   static constexpr bool EXACT = true;
@@ -60,22 +64,31 @@ template <> struct Run<__nv_bfloat16> {
     const uint4 t = *reinterpret_cast<const uint4*>(p);
     w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
   }
+  static __device__ __forceinline__ bool aligned(const __nv_bfloat16* p) { return ((uintptr_t)p & 7) == 0; }
+  __device__ __forceinline__ void load_halves(const __nv_bfloat16* p) {
+    const uint2 a = reinterpret_cast<const uint2*>(p)[0], b = reinterpret_cast<const uint2*>(p)[1];
+    w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y;
+  }
 };
-// The place in the row of value e of this thread's run j
-template <bool NEIGHBOURS> __device__ __forceinline__ int place(int j, int e) {
-  return NEIGHBOURS ? 8 * (threadIdx.x + j * blockDim.x) + e : (8 * j + e) * blockDim.x + threadIdx.x;
-}
-// zeros beyond the row's end; neighbours: dim is a multiple of 8 then
-template <bool NEIGHBOURS, typename T> __device__ __forceinline__ void load_run(Run<T>& run, const T* row, int j, int dim) {
+// The place in the row of the first value of this thread's run j, moved forward by `shift` (0 where a run's 8 are NEIGHBOURS that
+// begin on a multiple of 8, as dim does)
+__device__ __forceinline__ int place(int j, int shift) { return 8 * (int)(threadIdx.x + j * blockDim.x) - shift; }
+// the values by which the runs of a row are moved so that 4 of them lie aligned
+template <typename T> __device__ __forceinline__ int shift_of(const T* row) { return (int)((uintptr_t)row / sizeof(T)) & 3; }
+// zeros outside the row
+template <bool NEIGHBOURS, typename T> __device__ __forceinline__ void load_run(Run<T>& run, const T* row, int j, int shift, int dim) {
+  const int c0 = place(j, NEIGHBOURS ? 0 : shift);
   if (NEIGHBOURS) {
-    const int c0 = place<true>(j, 0);
     if (c0 < dim) {
       run.load(row + c0);
       return;
     }
+  } else if (c0 >= 0 && c0 + 8 <= dim && Run<T>::aligned(row + c0)) {  // (taking the others as three aligned loads and picking was slower)
+    run.load_halves(row + c0);
+    return;
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) run.set(e, !NEIGHBOURS && place<false>(j, e) < dim ? row[place<false>(j, e)] : T(0.f));
+  for (int e = 0; e < 8; ++e) run.set(e, !NEIGHBOURS && c0 + e >= 0 && c0 + e < dim ? row[c0 + e] : T(0.f));
 }
 // 8 values as e4m3, nearest and ties to even, beyond 448 to 448
 __device__ __forceinline__ uint2 to_e4m3(const float* v) {
@@ -86,11 +99,11 @@ __device__ __forceinline__ uint2 to_e4m3(const float* v) {
   return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
 
-// zeros where the row has ended, where zeros times what is not finite are not
-template <bool NEIGHBOURS> __device__ __forceinline__ float* ended(float* q, int j, int dim) {
-  if (!NEIGHBOURS || place<true>(j, 0) >= dim) {
+// zeros outside the row, where zeros times what is not finite are not
+template <bool NEIGHBOURS> __device__ __forceinline__ float* ended(float* q, int c0, int dim) {
+  if (c0 < 0 || c0 + 8 > dim) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = place<NEIGHBOURS>(j, e) < dim ? q[e] : 0.f;
+    for (int e = 0; e < 8; ++e) q[e] = c0 + e >= 0 && c0 + e < dim ? q[e] : 0.f;
   }
   return q;
 }
@@ -98,7 +111,7 @@ template <bool NEIGHBOURS> __device__ __forceinline__ float* ended(float* q, int
 // 8 quotients t * 448 / most, t = x (* g), to e4m3 as exact quotients would be, zeros where the row has ended; inv = 448 / most.
 // The float32 quotient, three or four roundings away, is off by less than 4 units of its last place.
 template <bool NEIGHBOURS, bool GAIN, typename X, typename G>
-__device__ __forceinline__ uint2 quotients(const X& x, const G& g, float inv, double most, int j, int dim) {
+__device__ __forceinline__ uint2 quotients(const X& x, const G& g, float inv, double most, int c0, int dim) {
   float q[8];
   if (!GAIN && X::EXACT) {  // inv = 448 / most is 0.875 / part, and neither 0.875 x nor part is rounded or out of range
     const float part = (float)most * 0x1p-9f;
@@ -107,7 +120,7 @@ __device__ __forceinline__ uint2 quotients(const X& x, const G& g, float inv, do
       const float q0 = x[e] * inv;
       q[e] = fmaf(fmaf(-q0, part, x[e] * 0.875f), inv * (1.f / 0.875f), q0);
     }
-    return to_e4m3(ended<NEIGHBOURS>(q, j, dim));
+    return to_e4m3(ended<NEIGHBOURS>(q, c0, dim));
   }
   // From 2^-6 on a value is beside a middle where its last 20 bits are within 8 of 2^19; below, the middles are the odd
   // multiples of 2^-10, which 2^-6 more puts where the same test finds them.
@@ -130,16 +143,26 @@ __device__ __forceinline__ uint2 quotients(const X& x, const G& g, float inv, do
       q[e] = copysignf(r, q[e]);
     }
   }
-  return to_e4m3(ended<NEIGHBOURS>(q, j, dim));
+  return to_e4m3(ended<NEIGHBOURS>(q, c0, dim));
 }
-template <bool NEIGHBOURS> __device__ __forceinline__ void store_run(uint8_t* row, uint2 q, int j, int pitch) {
-  if (NEIGHBOURS) {
-    if (place<true>(j, 0) < pitch) *reinterpret_cast<uint2*>(row + place<true>(j, 0)) = q;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (place<false>(j, e) < pitch) row[place<false>(j, e)] = (uint8_t)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
+// By a whole warp.  A run that is moved by `shift` holds the last bytes of its aligned 8 first: the next lane has the others.
+template <bool NEIGHBOURS> __device__ __forceinline__ void store_run(uint8_t* row, uint2 q, int j, int shift, int pitch) {
+  const int at = place(j, 0);
+  if (NEIGHBOURS || shift == 0) {
+    if (at < pitch) *reinterpret_cast<uint2*>(row + at) = q;
+    return;
   }
+  const uint64_t own = ((uint64_t)q.y << 32) | q.x, next = __shfl_down_sync(0xffffffffu, own, 1);
+  const int lane = threadIdx.x & 31, bits = 8 * shift;
+  if (lane < 31) {
+    if (at < pitch) *reinterpret_cast<uint64_t*>(row + at) = (own >> bits) | (next << (64 - bits));
+  } else {
+    for (int e = shift; e < 8; ++e)
+      if (at + e - shift < pitch) row[at + e - shift] = (uint8_t)(own >> (8 * e));
+  }
+  if (lane == 0 && at > 0)  // what the warp before could not store
+    for (int e = 0; e < shift; ++e)
+      if (at + e - shift < pitch) row[at + e - shift] = (uint8_t)(own >> (8 * e));
 }
 
 __device__ __forceinline__ float block_max(float v, float* scratch) {
@@ -179,15 +202,15 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && RUNS != 
   const T* row = x + (size_t)blockIdx.x * dim;
   uint8_t* out = q + (size_t)blockIdx.x * pitch;
   constexpr int KEPT = RUNS > 0 ? RUNS : 1;
-  const int runs = RUNS > 0 ? RUNS : (pitch / 8 + blockDim.x - 1) / blockDim.x;
+  const int runs = RUNS > 0 ? RUNS : (pitch / 8 + !NEIGHBOURS + blockDim.x - 1) / blockDim.x, shift = NEIGHBOURS ? 0 : shift_of(row);
   Run<T> v[KEPT];
   float most = 0.f;
 #pragma unroll
   for (int j = 0; j < KEPT; ++j)
-    if (RUNS > 0) load_run<NEIGHBOURS>(v[j], row, j, dim);
+    if (RUNS > 0) load_run<NEIGHBOURS>(v[j], row, j, shift, dim);
 #pragma unroll KEPT
   for (int j = 0; j < runs; ++j) {
-    if (RUNS == 0) load_run<NEIGHBOURS>(v[0], row, j, dim);
+    if (RUNS == 0) load_run<NEIGHBOURS>(v[0], row, j, shift, dim);
     most = max_nan(most, largest(v[RUNS > 0 ? j : 0]));
   }
   most = block_max(most, scratch);
@@ -196,9 +219,9 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && RUNS != 
   const float inv = none ? 0.f : E4M3_MAX / most;
 #pragma unroll KEPT
   for (int j = 0; j < runs; ++j) {
-    if (RUNS == 0) load_run<NEIGHBOURS>(v[0], row, j, dim);
+    if (RUNS == 0) load_run<NEIGHBOURS>(v[0], row, j, shift, dim);
     const Run<T>& u = v[RUNS > 0 ? j : 0];
-    store_run<NEIGHBOURS>(out, quotients<NEIGHBOURS, false>(u, u, inv, most, j, dim), j, pitch);
+    store_run<NEIGHBOURS>(out, quotients<NEIGHBOURS, false>(u, u, inv, most, place(j, shift), dim), j, shift, pitch);
   }
   if (threadIdx.x == 0) scales[blockIdx.x] = none ? 0.f : s;
 }
@@ -217,17 +240,25 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && (RUNS ==
                                                                      int residual_rows) {
   __shared__ float scratch[3][32];
   constexpr int KEPT = RUNS > 0 ? RUNS : 1;
-  const int runs = RUNS > 0 ? RUNS : (pitch / 8 + blockDim.x - 1) / blockDim.x;
+  const int runs = RUNS > 0 ? RUNS : (pitch / 8 + !NEIGHBOURS + blockDim.x - 1) / blockDim.x;
   Run<float> x[KEPT];
   Run<TG> g[KEPT];
   pdl_launch_dependents();
+  int shift = 0;
+  auto load_gain = [&]() {
 #pragma unroll
-  for (int j = 0; j < KEPT; ++j)  // the gain is a weight: it can be read before the kernel before this one is done
-    if (RUNS > 0) load_run<NEIGHBOURS>(g[j], gain, j, dim);
+    for (int j = 0; j < KEPT; ++j)
+      if (RUNS > 0) load_run<NEIGHBOURS>(g[j], gain, j, shift, dim);
+  };
+  if (NEIGHBOURS) load_gain();  // a weight: it can be read before the kernel before this one is done
   pdl_wait();
   const int src = rows ? rows[blockIdx.x] : blockIdx.x;
   if (!FMS_IN(src, residual_rows)) return;  // the whole block alike
   float* res = residual + (size_t)src * dim;
+  if (!NEIGHBOURS) {
+    shift = shift_of(res);
+    load_gain();
+  }
   const T* del = delta ? delta + (size_t)src * dim : nullptr;
   const bool writes = del && rows == nullptr;
   auto add = [&](Run<float>& v, const Run<T>& d) {
@@ -237,10 +268,10 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && (RUNS ==
   if (RUNS > 0) {
     Run<T> d[KEPT];
 #pragma unroll
-    for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(x[j], res, j, dim);
+    for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(x[j], res, j, shift, dim);
     if (del) {
 #pragma unroll
-      for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(d[j], del, j, dim);
+      for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(d[j], del, j, shift, dim);
 #pragma unroll
       for (int j = 0; j < KEPT; ++j) add(x[j], d[j]);
     }
@@ -252,25 +283,24 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && (RUNS ==
     Run<float>& xs = x[RUNS > 0 ? j : 0];
     Run<TG>& gs = g[RUNS > 0 ? j : 0];
     if (RUNS == 0) {
-      load_run<NEIGHBOURS>(xs, res, j, dim);
-      load_run<NEIGHBOURS>(gs, gain, j, dim);
+      load_run<NEIGHBOURS>(xs, res, j, shift, dim);
+      load_run<NEIGHBOURS>(gs, gain, j, shift, dim);
       if (del) {
         Run<T> d;
-        load_run<NEIGHBOURS>(d, del, j, dim);
+        load_run<NEIGHBOURS>(d, del, j, shift, dim);
         add(xs, d);
       }
     }
     if (writes) {
-      if (NEIGHBOURS) {
-        if (place<true>(j, 0) < dim) {
-          float4* to = reinterpret_cast<float4*>(res + place<true>(j, 0));
-          to[0] = make_float4(xs.v[0], xs.v[1], xs.v[2], xs.v[3]);
-          to[1] = make_float4(xs.v[4], xs.v[5], xs.v[6], xs.v[7]);
-        }
-      } else {
+      const int c0 = place(j, shift);
+      if (c0 >= 0 && c0 + 8 <= dim) {
+        float4* to = reinterpret_cast<float4*>(res + c0);
+        to[0] = make_float4(xs.v[0], xs.v[1], xs.v[2], xs.v[3]);
+        to[1] = make_float4(xs.v[4], xs.v[5], xs.v[6], xs.v[7]);
+      } else if (!NEIGHBOURS) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (place<false>(j, e) < dim) res[place<false>(j, e)] = xs.v[e];
+          if (c0 + e >= 0 && c0 + e < dim) res[c0 + e] = xs.v[e];
       }
     }
 #pragma unroll
@@ -309,15 +339,15 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && (RUNS ==
     Run<float>& xs = x[RUNS > 0 ? j : 0];
     Run<TG>& gs = g[RUNS > 0 ? j : 0];
     if (RUNS == 0) {
-      load_run<NEIGHBOURS>(xs, res, j, dim);  // the sum, where this thread has stored it
-      load_run<NEIGHBOURS>(gs, gain, j, dim);
+      load_run<NEIGHBOURS>(xs, res, j, shift, dim);  // the sum, where this thread has stored it
+      load_run<NEIGHBOURS>(gs, gain, j, shift, dim);
       if (del && !writes) {
         Run<T> d;
-        load_run<NEIGHBOURS>(d, del, j, dim);
+        load_run<NEIGHBOURS>(d, del, j, shift, dim);
         add(xs, d);
       }
     }
-    store_run<NEIGHBOURS>(q + (size_t)blockIdx.x * pitch, quotients<NEIGHBOURS, true>(xs, gs, inv, exact, j, dim), j, pitch);
+    store_run<NEIGHBOURS>(q + (size_t)blockIdx.x * pitch, quotients<NEIGHBOURS, true>(xs, gs, inv, exact, place(j, shift), dim), j, shift, pitch);
   }
   if (threadIdx.x == 0) scales[blockIdx.x] = none ? 0.f : s;
 }
@@ -336,16 +366,16 @@ int kept_for(int runs, int n_rows, int many, int most_kept, int* threads) {
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <typename T, int RUNS>
-void launch_rows(int threads, const void* x, uint8_t* q, float* scales, int n_rows, int dim, int pitch, cudaStream_t stream) {
-  const bool neighbours = dim % 8 == 0 && aligned16(x);
+void launch_rows(int threads, bool neighbours, const void* x, uint8_t* q, float* scales, int n_rows, int dim, int pitch, cudaStream_t stream) {
   fms_launch(neighbours ? quantize_rows_kernel<T, RUNS, true> : quantize_rows_kernel<T, RUNS, false>, dim3(n_rows), dim3(threads), 0,
              stream, (const T*)x, q, scales, n_rows, dim, pitch);
 }
 template <typename T> int quantize(const void* x, uint8_t* q, float* scales, int n_rows, int dim, int pitch, cudaStream_t stream) {
   int threads;
-  const int kept = kept_for(pitch / 8, n_rows, 4, 8, &threads);
+  const bool neighbours = dim % 8 == 0 && aligned16(x);
+  const int kept = kept_for(pitch / 8 + !neighbours, n_rows, 4, 8, &threads);  // a run more for rows that begin anywhere
   (kept == 1 ? launch_rows<T, 1> : kept == 2 ? launch_rows<T, 2> : kept == 4 ? launch_rows<T, 4> : kept == 8 ? launch_rows<T, 8> : launch_rows<T, 0>)(
-      threads, x, q, scales, n_rows, dim, pitch, stream);
+      threads, neighbours, x, q, scales, n_rows, dim, pitch, stream);
   return fms_launch_status("quantize_rows");
 }
 
@@ -358,16 +388,16 @@ struct NormArgs {
   const int* rows;
   int n_rows, dim, pitch, residual_rows;
 };
-template <typename T, typename TG, int RUNS> void launch_norm(int threads, const NormArgs& a, cudaStream_t stream) {
-  const bool neighbours = a.dim % 8 == 0 && aligned16(a.residual) && aligned16(a.delta) && aligned16(a.gain);
+template <typename T, typename TG, int RUNS> void launch_norm(int threads, bool neighbours, const NormArgs& a, cudaStream_t stream) {
   fms_launch(neighbours ? add_rmsnorm_quantized_kernel<T, TG, RUNS, true> : add_rmsnorm_quantized_kernel<T, TG, RUNS, false>, dim3(a.n_rows),
              dim3(threads), 0, stream, a.residual, (const T*)a.delta, (const TG*)a.gain, a.eps, a.q, a.scales, a.rows, a.dim, a.pitch,
              a.residual_rows);
 }
 template <typename T, typename TG> int norm(const NormArgs& a, cudaStream_t stream) {
   int threads;
-  const int kept = kept_for(a.pitch / 8, a.n_rows, 2, 4, &threads);
-  (kept == 1 ? launch_norm<T, TG, 1> : kept == 2 ? launch_norm<T, TG, 2> : kept == 4 ? launch_norm<T, TG, 4> : launch_norm<T, TG, 0>)(threads, a, stream);
+  const bool neighbours = a.dim % 8 == 0 && aligned16(a.residual) && aligned16(a.delta) && aligned16(a.gain);
+  const int kept = kept_for(a.pitch / 8 + !neighbours, a.n_rows, 2, 4, &threads);
+  (kept == 1 ? launch_norm<T, TG, 1> : kept == 2 ? launch_norm<T, TG, 2> : kept == 4 ? launch_norm<T, TG, 4> : launch_norm<T, TG, 0>)(threads, neighbours, a, stream);
   return fms_launch_status("add_rmsnorm_quantized");
 }
 }  // namespace

@@ -61,6 +61,24 @@ def test_quantize_rows(ops, dtype, rows, dim):
     assert bool(((back - x.float()).abs() <= x.float().abs() * 2.0 ** -4 * (1 + 2.0 ** -20) + scale[:, None] * 2.0 ** -10).all())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("off", [1, 2, 3, 5])
+@pytest.mark.parametrize("rows,dim", [(3, 64), (4, 517), (300, 1000), (5, 8193), (2, 33001)])
+def test_rows_that_begin_anywhere(ops, dtype, rows, dim, off):
+    g = gen(off + dim)
+    moved = lambda t: torch.cat((t.new_zeros(off), t.reshape(-1)))[off:].view(t.shape)  # noqa: E731
+    x, res, gain = normal(g, rows, dim).to(dtype), normal(g, rows, dim), (1 + normal(g, dim, std=0.1)).to(dtype)
+    a, b = ops.quantize_rows(x), ops.quantize_rows(moved(x))
+    assert torch.equal(a.values.view(torch.uint8), b.values.view(torch.uint8)) and torch.equal(a.scales, b.scales)
+    first, other = res.clone(), moved(res)
+    a = ops.add_rmsnorm_quantized(first, x, gain, 1e-5)
+    for b in (ops.add_rmsnorm_quantized(other, x, gain, 1e-5), ops.add_rmsnorm_quantized(res.clone(), moved(x), moved(gain), 1e-5)):
+        assert torch.equal(a.values.view(torch.uint8), b.values.view(torch.uint8))
+        # the same squares in another order: as far apart as either may be from the exact scale
+        torch.testing.assert_close(a.scales, b.scales, atol=0, rtol=2 * 2.0 ** -24 * (max(34, dim / 256) / 2 + 10))
+    assert torch.equal(first, other)
+
+
 def test_quantize_rows_of_zeros_tiny_and_not_finite(ops):
     x = normal(gen(1), 8, 70)
     x[1] = 0.0
