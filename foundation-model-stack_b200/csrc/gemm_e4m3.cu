@@ -12,7 +12,7 @@
 #include "common.cuh"
 
 namespace {
-constexpr int TILE = 128, TILE_K = 128, UMMA_K = 32, MAX_STAGES = 12, MAX_KS = 4;
+constexpr int TILE = 128, TILE_K = 128, UMMA_K = 32, MAX_STAGES = 12;
 constexpr int THREADS = 320, EPILOGUE_WARPS = 8;
 constexpr int BOX_BYTES = TILE * TILE_K;  // 128 rows of an operand for one step
 
@@ -41,7 +41,9 @@ struct Epilogue {
   const float *sx, *sw;       // [M], [N]
   int out_f32, glu, act;
   int outputs;                // columns of y: N, or the hidden values of GLU (half of N)
-  int tile_n, stages, ks, n_tokens;
+  int tile_n, stages, n_tokens;
+  float* scratch;             // [blocks][slots][n_tokens][128], of the second kernel
+  int slots;                  // of a block in scratch, or 0: each takes one whole tile
 };
 
 // four sums times the scales of their row and columns (+ bias)
@@ -264,41 +266,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 
 // ---- up to 256 rows (decode) ---------------------------------------------------------------------------------------
 // The operands swapped: 128 rows of w fill the instruction's rows and the tokens are its columns (16 to 256), since a product
-// of this size is bound by reading w once.  A block owns 128 rows of w (GLU: 64 gate rows and the 64 up rows that belong to
-// them) for a slice of k; the ks blocks of a tile form a cluster and add their sums through distributed shared memory in the
-// order of their ranks.  ks depends on the weights' shape alone, so a row's result does not depend on the rest of the batch.
-// The first stages' boxes of w are asked for before griddepcontrol.wait: weights do not depend on the kernel before.
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t local_addr, uint32_t rank) {
-  float4 v;
-  asm volatile(
-      "{\n.reg .b32 remote;\nmapa.shared::cluster.u32 remote, %4, %5;\nld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [remote];\n}\n"
-      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-      : "r"(local_addr), "r"(rank)
-      : "memory");
-  return v;
-}
+// of this size is bound by reading w once.  A tile is 128 rows of w (GLU: 64 gate rows and the 64 up rows that belong to them),
+// a step of it 128 k.  Many tiles, or short ones: a block takes one whole tile, two blocks a multiprocessor, and stores y.  Few
+// tiles (cut_of): every multiprocessor takes an equal run of the steps of all tiles; where a tile's steps fall to several blocks,
+// each leaves its sums in a slot of its own in scratch memory, and a second kernel adds them in the order of k; under GLU all
+// tiles of such a cut go that way, since a gate and its up value lie in different lanes.  (Clusters that shared a tile and added
+// their sums through distributed shared memory: 6,144 x 4,096 by 64 rows 11.8 us, 4,096 x 14,336 17.7 us; so 10.0 and 15.1.)  The
+// cut depends on the weights' shape alone, so a row's result does not depend on the rest of the batch.  The first stages'
+// boxes of w are asked for before griddepcontrol.wait: weights do not depend on the kernel before.
+//   warp 0 TMA, warp 1 the instructions, warps 2-9 the epilogue, under the next tile's steps up to 128 tokens
+__host__ __device__ inline int first_step(int b, int blocks, int steps) { return (int)((long)b * steps / blocks); }
+__device__ __forceinline__ int block_of_step(int step, int blocks, int steps) { return (int)((((long)step + 1) * blocks - 1) / steps); }
 
 __global__ void __launch_bounds__(THREADS, 2) e4m3_rows_kernel(const __grid_constant__ CUtensorMap map_x,
-                                                            const __grid_constant__ CUtensorMap map_w, Epilogue ep, int M,
-                                                            int k_steps_all, int* __restrict__ error_flag) {
+                                                               const __grid_constant__ CUtensorMap map_w, Epilogue ep, int M,
+                                                               int tiles, int k_steps, int* __restrict__ error_flag) {
   extern __shared__ unsigned char smem_unaligned[];
   unsigned char* smem = smem_unaligned + (-smem_u32(smem_unaligned) & 1023);
-  const int stage_bytes = BOX_BYTES + ep.n_tokens * TILE_K, stages = ep.stages, ks = ep.ks;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)stages * stage_bytes);
+  const int stage_bytes = BOX_BYTES + ep.n_tokens * TILE_K, stages = ep.stages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + stages * stage_bytes);
   uint64_t* empty = full + MAX_STAGES;
-  uint64_t* acc_full = empty + MAX_STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  uint64_t* acc_full = empty + MAX_STAGES;  // [2]
+  uint64_t* acc_empty = acc_full + 2;       // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   __shared__ int failed_flag;
-  __shared__ float row_scales[256];  // of x: read from global memory they would be waited for four tokens at a time
+  __shared__ float row_scales[256];  // of x: read from global memory they would be waited for at every run of tokens
   volatile int* failed = &failed_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = ks > 1 ? (int)cluster_rank() : 0;
-  const int n0 = blockIdx.y * (ep.glu ? TILE / 2 : TILE);
-  const int per = (k_steps_all + ks - 1) / ks;
-  const int step_lo = min(rank * per, k_steps_all), k_steps = min(step_lo + per, k_steps_all) - step_lo;  // may be 0
-  uint32_t tmem_cols = 32;
-  while ((int)tmem_cols < ep.n_tokens) tmem_cols *= 2;
+  const int all = tiles * k_steps, row_step = ep.glu ? TILE / 2 : TILE;
+  const int lo = first_step(blockIdx.x, gridDim.x, all), hi = first_step(blockIdx.x + 1, gridDim.x, all);
+  const int accs = ep.n_tokens <= 128 ? 2 : 1;
 
   if (threadIdx.x == 0) {
     failed_flag = 0;
@@ -306,10 +304,13 @@ __global__ void __launch_bounds__(THREADS, 2) e4m3_rows_kernel(const __grid_cons
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(acc_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], EPILOGUE_WARPS);
+    }
     mbar_fence_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, tmem_cols);
+  if (warp == 1) tmem_alloc(tmem_slot, 256);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -318,136 +319,170 @@ __global__ void __launch_bounds__(THREADS, 2) e4m3_rows_kernel(const __grid_cons
 
   if (warp == 0) {
     if (elect_one()) {
-      auto load_w = [&](int i) {
-        const int s = i % stages;
-        unsigned char* a = smem + (size_t)s * stage_bytes;
+      auto load_w = [&](int s, int tile, int k) {
+        unsigned char* to = smem + s * stage_bytes;
         mbar_arrive_expect_tx(&full[s], stage_bytes);
-        tma_load_2d(a, &map_w, (step_lo + i) * TILE_K, n0, &full[s]);
-        if (ep.glu) tma_load_2d(a + BOX_BYTES / 2, &map_w, (step_lo + i) * TILE_K, ep.outputs + n0, &full[s]);
+        tma_load_2d(to, &map_w, k * TILE_K, tile * row_step, &full[s]);
+        if (ep.glu) tma_load_2d(to + BOX_BYTES / 2, &map_w, k * TILE_K, ep.outputs + tile * row_step, &full[s]);
       };
-      auto load_x = [&](int i) {
-        const int s = i % stages;
-        tma_load_2d(smem + (size_t)s * stage_bytes + BOX_BYTES, &map_x, (step_lo + i) * TILE_K, 0, &full[s]);
-      };
-      const int early = min(stages, k_steps);
-      for (int i = 0; i < early; ++i) load_w(i);
+      int tile = lo / k_steps, k = lo - tile * k_steps, s = 0;
+      const int early = min(stages, hi - lo);
+      for (int i = 0, t = tile, kk = k; i < early; ++i) {
+        load_w(i, t, kk);
+        if (++kk == k_steps) kk = 0, ++t;
+      }
       pdl_wait();  // x is what the kernel before wrote
-      for (int i = 0; i < early; ++i) load_x(i);
-      for (int i = early; i < k_steps && !*failed; ++i) {
-        if (!wait_or_abort(&empty[i % stages], ((i / stages) & 1) ^ 1, failed)) break;
-        load_w(i);
-        load_x(i);
+      uint32_t phase = 1;
+      for (int i = lo; i < hi && !*failed; ++i) {
+        if (i - lo >= early) {
+          if (!wait_or_abort(&empty[s], phase, failed)) break;
+          load_w(s, tile, k);
+        }
+        tma_load_2d(smem + s * stage_bytes + BOX_BYTES, &map_x, k * TILE_K, 0, &full[s]);
+        if (++k == k_steps) k = 0, ++tile;
+        if (++s == stages) s = 0, phase ^= 1;
       }
     }
   } else if (warp == 1) {
     if (elect_one()) {
       const uint32_t idesc = idesc_e4m3(TILE, ep.n_tokens);
       const MatrixDesc base(smem_u32(smem));
-      int s = 0;
-      uint32_t phase = 0;
-      for (int i = 0; i < k_steps; ++i) {
+      int k = lo % k_steps, s = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 1;
+      for (int i = lo; i < hi; ++i) {
+        const bool first = i == lo || k == 0;
+        if (first && !quick_wait(&acc_empty[acc], acc_phase, failed)) break;
         if (!quick_wait(&full[s], phase, failed)) break;
         tc_fence_after();
         const uint32_t w = base.lo + (uint32_t)(s * stage_bytes >> 4), x = w + (BOX_BYTES >> 4);
 #pragma unroll
         for (int kk = 0; kk < TILE_K / UMMA_K; ++kk)
-          issue_e4m3(tmem, w + kk * (UMMA_K >> 4), base.hi, x + kk * (UMMA_K >> 4), idesc, kk > 0 ? 1u : i > 0);
+          issue_e4m3(tmem + acc * 128, w + kk * (UMMA_K >> 4), base.hi, x + kk * (UMMA_K >> 4), idesc, kk > 0 ? 1u : !first);
         tc_commit(&empty[s]);
+        if (++k == k_steps) k = 0;
+        if (k == 0 || i + 1 == hi) {
+          tc_commit(&acc_full[acc]);
+          if (++acc == accs) acc = 0, acc_phase ^= 1;
+        }
         if (++s == stages) s = 0, phase ^= 1;
       }
-      tc_commit(acc_full);  // arrives when everything issued so far is done (at once if there was nothing)
     }
-  }
-  // The sums leave tensor memory as they are where a block has them whole and a thread's row of w is a column of y; else they meet
-  // in shared memory, as float32 [128][n_tokens + 4] over the stages (every copy into them has landed and every instruction
-  // that read them is done once the accumulator is ready).  Thread: a row of w, runs of 8 or 16 tokens.
-  float* red = reinterpret_cast<float*>(smem);
-  const int red_stride = ep.n_tokens + 4, part = (warp - 2) >> 2;
-  const bool direct = ks == 1 && !ep.glu;
-  const size_t pitch = ep.outputs;
-  if (warp >= 2) {
-    pdl_wait();  // these warps read and write what other kernels touch (scales, the error flag, y)
+  } else {
+    pdl_wait();  // these warps read and write what other kernels touch (scales, scratch memory, y)
     for (int t = threadIdx.x - 64; t < ep.n_tokens; t += 32 * EPILOGUE_WARPS) row_scales[t] = t < M ? ep.sx[t] : 0.f;
-    const int quarter = warp & 3, row = quarter * 32 + lane, col = n0 + row;
-    const bool live = col < ep.outputs;
-    const float sw = direct && live ? ep.sw[col] : 0.f, bias = direct && live && ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;
     asm volatile("bar.sync 1, %0;\n" ::"n"(32 * EPILOGUE_WARPS) : "memory");
-    const bool ok = warp_wait(acc_full, 0, failed);
-    tc_fence_after();
-    for (int c0 = 16 * part; c0 < ep.n_tokens; c0 += 32) {
-      float v[16];
-      if (ok && k_steps > 0) {
-        tmem_load_16(tmem + ((uint32_t)(quarter * 32) << 16) + c0, v);
-      } else {
+    const int quarter = warp & 3, part = (warp - 2) >> 2, row = quarter * 32 + lane;
+    // A block of one whole tile under GLU: the sums meet in shared memory, as float32 [128][n_tokens + 4] over the stages (every
+    // copy into them has landed and every instruction that read them is done once the accumulator is ready).
+    const bool exchange = ep.glu && ep.slots == 0;
+    float* sums = reinterpret_cast<float*>(smem);
+    const int sums_pitch = ep.n_tokens + 4;
+    int acc = 0, segment = 0;
+    uint32_t acc_phase = 0;
+    for (int i = lo; i < hi; ++segment) {
+      const int tile = i / k_steps, k_lo = i - tile * k_steps, k_hi = min(k_steps, hi - tile * k_steps), col = tile * TILE + row;
+      const bool whole = !ep.glu && k_lo == 0 && k_hi == k_steps, live = whole && col < ep.outputs;
+      const float sw = live ? ep.sw[col] : 0.f, bias = live && ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;
+      float* slot = ep.scratch + ((size_t)(ep.slots * blockIdx.x + segment) * ep.n_tokens) * TILE + row;
+      if (!warp_wait(&acc_full[acc], acc_phase, failed)) break;
+      tc_fence_after();
+      for (int c0 = 16 * part; c0 < ep.n_tokens; c0 += 32) {
+        float v[16];
+        tmem_load_16(tmem + acc * 128 + ((uint32_t)(quarter * 32) << 16) + c0, v);
+        if (exchange) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = 0.f;
-      }
-      if (!direct) {
+          for (int j = 0; j < 16; j += 4)
+            *reinterpret_cast<float4*>(sums + row * sums_pitch + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        } else if (!whole) {
 #pragma unroll
-        for (int j = 0; j < 16; j += 4)
-          *reinterpret_cast<float4*>(red + row * red_stride + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-      } else if (ok && live) {
+          for (int j = 0; j < 16; ++j) slot[(size_t)(c0 + j) * TILE] = v[j];
+        } else if (live) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = fmaf(v[j], row_scales[c0 + j] * sw, bias);
-        store_column<16>(ep, v, c0, col, M, pitch);
-      }
-    }
-    tc_fence_before();
-  }
-  if (!direct) {
-    __syncthreads();
-    if (ks > 1) cluster_sync_all();  // every block's sums are in its shared memory
-    if (warp >= 2 && !*failed) {     // this block's share of the tokens, 8 at a time
-      const int e = threadIdx.x - 64, i = ep.glu ? e & 63 : e & 127, col = n0 + i;
-      const int share = ((ep.n_tokens + ks - 1) / ks + 7) / 8 * 8, t_hi = min((rank + 1) * share, ep.n_tokens);
-      const bool live = col < ep.outputs;
-      const float sw = live ? ep.sw[col] : 0.f, su = live && ep.glu ? ep.sw[ep.outputs + col] : 0.f;
-      const float bias = live && ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;
-      const float bias_up = live && ep.glu && ep.bias ? __bfloat162float(ep.bias[ep.outputs + col]) : 0.f;
-      const uint32_t red_addr = smem_u32(red);
-      auto total8 = [&](int row, int t, float* out) {
-        float4 v[MAX_KS][2];
-        const uint32_t at = red_addr + (uint32_t)(row * red_stride + t) * 4u;
-#pragma unroll
-        for (int r = 0; r < MAX_KS; ++r)  // all loads on their way before the first sum
-          if (r < ks) {
-            v[r][0] = ld_cluster_f32x4(at, (uint32_t)r);
-            v[r][1] = ld_cluster_f32x4(at + 16, (uint32_t)r);
-          }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) out[j] = 0.f;
-#pragma unroll
-        for (int r = 0; r < MAX_KS; ++r)
-          if (r < ks) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              out[4 * h] += v[r][h].x; out[4 * h + 1] += v[r][h].y; out[4 * h + 2] += v[r][h].z; out[4 * h + 3] += v[r][h].w;
-            }
-          }
-      };
-      const int step = 32 * EPILOGUE_WARPS / (ep.glu ? 64 : 128) * 8;
-      for (int t = rank * share + 8 * (ep.glu ? e >> 6 : e >> 7); t < t_hi; t += step) {
-        float v[8], u[8];
-        total8(i, t, v);
-        if (ep.glu) total8(64 + i, t, u);
-        if (!live) continue;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float sx = row_scales[t + j];
-          v[j] = fmaf(v[j], sx * sw, bias);
-          if (ep.glu) v[j] = activate(v[j], ep.act) * fmaf(u[j], sx * su, bias_up);
+          for (int j = 0; j < 16; ++j) v[j] = fmaf(v[j], row_scales[c0 + j] * sw, bias);
+          store_column<16>(ep, v, c0, col, M, ep.outputs);
         }
-        store_column<8>(ep, v, t, col, M, pitch);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[acc]);
+      if (++acc == accs) acc = 0, acc_phase ^= 1;
+      i += k_hi - k_lo;
+    }
+    if (exchange) {
+      asm volatile("bar.sync 1, %0;\n" ::"n"(32 * EPILOGUE_WARPS) : "memory");
+      const int e = threadIdx.x - 64, r = e & 63, col = blockIdx.x * (TILE / 2) + r;
+      if (col < ep.outputs && !*failed) {
+        const float sw = ep.sw[col], su = ep.sw[ep.outputs + col];
+        const float bias = ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;
+        const float bias_up = ep.bias ? __bfloat162float(ep.bias[ep.outputs + col]) : 0.f;
+        for (int t = 4 * (e >> 6); t < ep.n_tokens; t += 16) {
+          const float4 g = *reinterpret_cast<const float4*>(sums + r * sums_pitch + t);
+          const float4 u = *reinterpret_cast<const float4*>(sums + (TILE / 2 + r) * sums_pitch + t);
+          float v[4] = {g.x, g.y, g.z, g.w}, up[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float sx = row_scales[t + j];
+            v[j] = activate(fmaf(v[j], sx * sw, bias), ep.act) * fmaf(up[j], sx * su, bias_up);
+          }
+          store_column<4>(ep, v, t, col, M, ep.outputs);
+        }
       }
     }
   }
-  if (ks > 1) cluster_sync_all();  // nobody leaves while another block still reads its shared memory
+  tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *failed && error_flag) atomicExch(error_flag, 4);
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, tmem_cols);
+    tmem_dealloc(tmem, 256);
   }
+}
+
+// y of the tiles that several blocks share (GLU: of all) in a cut of equal runs: their sums in the order of k, scales, bias,
+// activation.  Block: a tile's columns of y by 4 tokens (GLU: 64 by 8); the slots of four blocks are on their way at a time.
+__global__ void __launch_bounds__(TILE) e4m3_join_kernel(Epilogue ep, int M, int k_steps, int blocks, int tiles) {
+  pdl_launch_dependents();
+  const int all = tiles * k_steps, tile = blockIdx.x, start = tile * k_steps, row_step = ep.glu ? TILE / 2 : TILE;
+  const int from = block_of_step(start, blocks, all), to = block_of_step(start + k_steps - 1, blocks, all);
+  const int row = (int)threadIdx.x & (row_step - 1), col = tile * row_step + row;
+  const int t0 = (blockIdx.y * (TILE / row_step) + (int)threadIdx.x / row_step) * 4;
+  if ((!ep.glu && from == to) || col >= ep.outputs || t0 >= M) return;  // some block of some tile goes on, and waits
+  const float sw = ep.sw[col], bias = ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;
+  // only the first block of a tile can have begun with an earlier one
+  const int head = tile - first_step(from, blocks, all) / k_steps;
+  const size_t pitch = (size_t)ep.n_tokens * TILE;
+  pdl_wait();
+  float sx[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sx[j] = t0 + j < M ? ep.sx[t0 + j] : 0.f;
+  auto total = [&](int r, float* sum) {
+    const float* slots = ep.scratch + (size_t)t0 * TILE + r;
+    sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+    for (int b = from; b <= to; b += 4) {
+      float v[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[i][j] = b + i <= to ? __ldcg(slots + ((size_t)ep.slots * (b + i) + (b + i == from ? head : 0)) * pitch + j * TILE) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += v[i][j];
+    }
+  };
+  float y[4];
+  total(row, y);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = fmaf(y[j], sx[j] * sw, bias);
+  if (ep.glu) {
+    const float su = ep.sw[ep.outputs + col], bias_up = ep.bias ? __bfloat162float(ep.bias[ep.outputs + col]) : 0.f;
+    float up[4];
+    total(TILE / 2 + row, up);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = activate(y[j], ep.act) * fmaf(up[j], sx[j] * su, bias_up);
+  }
+  store_column<4>(ep, y, t0, col, M, ep.outputs);
 }
 
 // [rows, pitch] bytes in boxes of `box_rows` rows x 128 bytes with the 128-byte swizzle
@@ -491,11 +526,28 @@ int choose_tile_n(int tiles_m, int cols, bool glu, int pairs) {
   return best;
 }
 
-// Blocks that share a tile: from the weights' shape alone, as many as fill most of the multiprocessors, each with 4 steps at least
-int choose_ks(int tiles, int k_steps) {
-  int ks = 1;
-  while (ks < 4 && tiles * ks < 120 && k_steps / (ks * 2) >= 4) ks *= 2;
-  return ks;
+// How the second kernel cuts a product; slots 0: a block takes one whole tile, and there is nothing to join.  Equal runs cost the
+// second launch and a trip through scratch memory, about what 16 steps of a block cost, and more the more tiles there are.  By
+// 64 rows, equal runs against whole tiles, us: 4,096 x 4,096 8.1 : 11.4, 6,144 x 4,096 10.0 : 11.5, 8,192 x 4,096 11.0 : 11.7,
+// 6,144 x 2,560 8.3 : 8.3, 8,192 x 2,048 8.4 : 7.5, 12,288 x 4,096 14.1 : 12.6, 12,288 x 12,288 31.6 : 30.0,
+// 28,672 x 4,096 28.7 : 21.7.  A run is 4 steps or more: the sums of 32 blocks of one step each take longer to join than to make.
+struct Cut {
+  int tiles, k_steps, blocks, slots;
+};
+Cut cut_of(int outputs, bool glu, long pitch) {
+  Cut c;
+  const int row_step = glu ? TILE / 2 : TILE, sms = multiprocessors();
+  c.tiles = (outputs + row_step - 1) / row_step;
+  c.k_steps = (int)((pitch + TILE_K - 1) / TILE_K);
+  if (3L * c.tiles >= 2L * sms || (long)c.k_steps * (sms - c.tiles) <= 16L * sms) {
+    c.blocks = c.tiles;
+    c.slots = 0;
+  } else {  // 18 steps a tile or more, so that there are more blocks than tiles, and a run reaches into two tiles at most
+    const long runs = (long)c.tiles * c.k_steps / 4;
+    c.blocks = runs < sms ? (int)runs : sms;
+    c.slots = 2;
+  }
+  return c;
 }
 
 constexpr int ROWS_MOST = 256;  // rows of x that the second kernel takes
@@ -514,44 +566,32 @@ template <typename Kernel> int allow_smem(const char* what, Kernel kernel, int b
   return 0;
 }
 
-int launch(const void* x, const void* w, Epilogue ep, int M, int N, long pitch, int* error_flag, cudaStream_t stream) {
+int launch(const void* x, const void* w, Epilogue ep, int M, int N, long pitch, long scratch_floats, int* error_flag, cudaStream_t stream) {
   if (pitch <= 0 || pitch % 16 || pitch > 0x7fffff00L) return fms_fail("gemm_e4m3: rows of %ld bytes, a multiple of 16 is wanted", pitch);
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)ep.out) & 15) return fms_fail("gemm_e4m3: operands and result must be 16-byte aligned");
   const int k_steps = (int)((pitch + TILE_K - 1) / TILE_K);
   CUtensorMap map_x, map_w;
   static uint64_t rows_allowed = 0, pair_allowed = 0;
-  if (M <= ROWS_MOST ? allow_smem("gemm_e4m3", e4m3_rows_kernel, 225 * 1024, &rows_allowed)
+  if (M <= ROWS_MOST ? allow_smem("gemm_e4m3", e4m3_rows_kernel, (int)(PAIR_RING + EXTRA), &rows_allowed)
                      : allow_smem("gemm_e4m3", e4m3_pair_kernel, (int)(PAIR_RING + EXTRA), &pair_allowed))
     return 1;
   if (M <= ROWS_MOST) {
+    const Cut c = cut_of(ep.outputs, ep.glu != 0, pitch);
     ep.n_tokens = (M + 15) / 16 * 16;
-    const int row_step = ep.glu ? TILE / 2 : TILE, tiles = (ep.outputs + row_step - 1) / row_step;
-    if (tiles > 65535) return fms_fail("gemm_e4m3: %d tiles of rows of w", tiles);
-    ep.ks = choose_ks(tiles, k_steps);
-    const int stage_bytes = BOX_BYTES + ep.n_tokens * TILE_K;
-    // two blocks a multiprocessor; one where the tokens are many or the blocks few
-    const int budget = (ep.n_tokens <= 128 && tiles * ep.ks > 148) ? 104 * 1024 : 200 * 1024;
-    const size_t red_bytes = (size_t)TILE * (ep.n_tokens + 4) * sizeof(float);
-    ep.stages = min(max(budget / stage_bytes, 3), MAX_STAGES);
-    while ((size_t)ep.stages * stage_bytes < red_bytes) ++ep.stages;  // the sums go over the stages
-    if (make_byte_map(&map_x, x, M, pitch, ep.n_tokens) || make_byte_map(&map_w, w, N, pitch, row_step)) return 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ep.ks, tiles);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = (size_t)ep.stages * stage_bytes + EXTRA;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ep.ks;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = fms_pdl_enabled() ? 2 : 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, e4m3_rows_kernel, map_x, map_w, ep, M, k_steps, error_flag);
-    if (e != cudaSuccess) return fms_fail("gemm_e4m3: launch failed: %s", cudaGetErrorString(e));
-    return fms_launch_status("gemm_e4m3");
+    ep.slots = c.slots;
+    if ((long)c.tiles * c.k_steps > 0x3fffffffL) return fms_fail("gemm_e4m3: %d tiles of %d steps", c.tiles, c.k_steps);
+    const long wanted = (long)c.blocks * c.slots * ep.n_tokens * TILE;
+    if (scratch_floats < wanted) return fms_fail("gemm_e4m3: %ld floats of scratch memory, %ld are wanted", scratch_floats, wanted);
+    // room for two blocks on a multiprocessor where they are as many and the ring stays deep enough
+    const size_t ring = ep.n_tokens <= 128 && c.slots == 0 && c.blocks > multiprocessors() ? PAIR_RING / 2 : PAIR_RING;
+    ep.stages = min((int)(ring / (BOX_BYTES + ep.n_tokens * TILE_K)), MAX_STAGES);
+    if (make_byte_map(&map_x, x, M, pitch, ep.n_tokens) || make_byte_map(&map_w, w, N, pitch, ep.glu ? TILE / 2 : TILE)) return 1;
+    fms_launch(e4m3_rows_kernel, dim3(c.blocks), dim3(THREADS), ring + EXTRA, stream, map_x, map_w, ep, M, c.tiles, c.k_steps, error_flag);
+    if (fms_launch_status("gemm_e4m3")) return 1;
+    if (c.slots == 0) return 0;
+    const int each = ep.glu ? 8 : 4;
+    fms_launch(e4m3_join_kernel, dim3(c.tiles, (ep.n_tokens + each - 1) / each), dim3(TILE), 0, stream, ep, M, c.k_steps, c.blocks, c.tiles);
+    return fms_launch_status("gemm_e4m3_join");
   }
   const int pairs = max(multiprocessors() / 2, 1), tiles_m = (M + 2 * TILE - 1) / (2 * TILE);
   ep.tile_n = choose_tile_n(tiles_m, ep.outputs, ep.glu != 0, pairs);
@@ -567,10 +607,17 @@ int launch(const void* x, const void* w, Epilogue ep, int M, int N, long pitch, 
 }
 }  // namespace
 
+// Floats of scratch memory that the products of M rows with weights of N rows (glu 1: of N / 2 gate and N / 2 up rows) want.
+FMS_API long fms_e4m3_scratch(long M, long N, long pitch, long glu) {
+  if (M <= 0 || N <= 0 || pitch <= 0 || M > ROWS_MOST) return 0;
+  const Cut c = cut_of((int)(glu ? N / 2 : N), glu != 0, pitch);
+  return (long)c.blocks * c.slots * ((M + 15) / 16 * 16) * TILE;
+}
+
 // y [M, N] (bfloat16, or float32 with out_dtype FMS_F32) of x [M, pitch] and w [N, pitch], e4m3, with sx [M], sw [N] float32 and
 // bias [N] bfloat16 or null.
 FMS_API int fms_linear_e4m3(const void* x, const float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype,
-                            int M, int N, long pitch, int* error_flag, cudaStream_t stream) {
+                            int M, int N, long pitch, float* scratch, long scratch_floats, int* error_flag, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
   if (out_dtype != FMS_F32 && out_dtype != FMS_BF16) return fms_fail("linear_e4m3: out dtype %d", out_dtype);
   Epilogue ep = {};
@@ -580,12 +627,13 @@ FMS_API int fms_linear_e4m3(const void* x, const float* sx, const void* w, const
   ep.sw = sw;
   ep.out_f32 = out_dtype == FMS_F32;
   ep.outputs = N;
-  return launch(x, w, ep, M, N, pitch, error_flag, stream);
+  ep.scratch = scratch;
+  return launch(x, w, ep, M, N, pitch, scratch_floats, error_flag, stream);
 }
 
 // y [M, hidden] bfloat16 = act(gate) * up for w = [gate; up] of 2 hidden rows (sw and bias [2 hidden]).
 FMS_API int fms_glu_e4m3(const void* x, const float* sx, const void* w, const float* sw, const void* bias, void* y, int M, int hidden,
-                         long pitch, int act, int* error_flag, cudaStream_t stream) {
+                         long pitch, int act, float* scratch, long scratch_floats, int* error_flag, cudaStream_t stream) {
   if (M <= 0 || hidden <= 0) return 0;
   if (act < 0 || act > 3) return fms_fail("glu_e4m3: activation %d", act);
   Epilogue ep = {};
@@ -596,5 +644,6 @@ FMS_API int fms_glu_e4m3(const void* x, const float* sx, const void* w, const fl
   ep.glu = 1;
   ep.act = act;
   ep.outputs = hidden;
-  return launch(x, w, ep, M, 2 * hidden, pitch, error_flag, stream);
+  ep.scratch = scratch;
+  return launch(x, w, ep, M, 2 * hidden, pitch, scratch_floats, error_flag, stream);
 }

@@ -791,7 +791,7 @@ int check(const Int4Args& p) {
 }  // namespace
 
 // Floats of scratch memory that fms_linear_int4 wants.
-FMS_API long fms_linear_int4_scratch(int M, int N, int K) { return M <= FEW_ROWS || N <= 0 || K <= 0 || M > rows_most(N) ? 0 : rows_scratch(M, N, K); }
+FMS_API long fms_linear_int4_scratch(long M, long N, long K) { return M <= FEW_ROWS || N <= 0 || K <= 0 || M > rows_most(N) ? 0 : rows_scratch(M, N, K); }
 
 // y [M, N] bfloat16 of x [M, K] bfloat16, w packed with `per` scales a block, bias [N] bfloat16 or null.
 FMS_API int fms_linear_int4(const void* x, const void* w, const void* bias, void* y, int M, int N, int K, int k_blocks, int per,

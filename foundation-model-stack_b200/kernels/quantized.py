@@ -20,6 +20,7 @@ from typing import Optional
 import torch
 
 from . import ops
+from .build import load_library
 
 E4M3 = torch.float8_e4m3fn
 INT4_FEW_ROWS = 8  # rows up to which the 4-bit product runs on mma.sync and has a gated form (csrc/gemm_int4.cu)
@@ -296,6 +297,22 @@ def _rows_for(what: str, x, weight: E4M3Weight) -> QuantizedRows:
     return x
 
 
+_scratch_sizes = {}  # (entry, device, sizes) -> floats
+
+
+def _scratch(library: str, name: str, device, rows: int, *sizes):
+    """Scratch memory for the sums that several thread blocks share, and its floats: of one call alone, so that calls at once and
+    captured graphs do not meet in it."""
+    sizes = (min(rows, 257),) + sizes  # more than 256 rows want none
+    key = (name, device) + sizes
+    floats = _scratch_sizes.get(key)
+    if floats is None:
+        entry = getattr(load_library(library), name)
+        entry.restype, entry.argtypes = ctypes.c_long, [ctypes.c_long] * len(sizes)
+        floats = _scratch_sizes[key] = entry(*sizes)
+    return (torch.empty_strided((floats,), (1,), dtype=torch.float32, device=device) if floats else None), floats
+
+
 def linear_e4m3(x, weight: E4M3Weight, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """Rows ``x`` (``QuantizedRows``; a tensor is quantised first) times weight [out, in] transposed (+ bias), summed in float32,
     in bfloat16 or float32."""
@@ -305,8 +322,10 @@ def linear_e4m3(x, weight: E4M3Weight, bias: Optional[torch.Tensor] = None, out_
     _on_device("linear_e4m3", bias)
     code = ops._code(out_dtype)
     y = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=x.device)
+    pitch = x.values.shape[1]
+    scratch, floats = _scratch("gemm_e4m3", "fms_e4m3_scratch", x.device, m, n, pitch, 0)
     ops._call("gemm_e4m3", "fms_linear_e4m3", x.values, x.scales, weight.rows.values, weight.rows.scales, bias, y, code, m, n,
-              x.values.shape[1], ops.error_flag(x.device), ops._stream())
+              pitch, scratch, floats, ops.error_flag(x.device), ops._stream())
     return y
 
 
@@ -319,8 +338,10 @@ def gated_linear_e4m3(x, weight: E4M3Weight, bias: Optional[torch.Tensor], activ
     bias = _bias("gated_linear_e4m3", bias, n)
     _on_device("gated_linear_e4m3", bias)
     y = torch.empty((m, n // 2), dtype=torch.bfloat16, device=x.device)
+    pitch = x.values.shape[1]
+    scratch, floats = _scratch("gemm_e4m3", "fms_e4m3_scratch", x.device, m, n, pitch, 1)
     ops._call("gemm_e4m3", "fms_glu_e4m3", x.values, x.scales, weight.rows.values, weight.rows.scales, bias, y, m, n // 2,
-              x.values.shape[1], int(activation), ops.error_flag(x.device), ops._stream())
+              pitch, int(activation), scratch, floats, ops.error_flag(x.device), ops._stream())
     return y
 
 
@@ -343,28 +364,10 @@ def linear_int4(x: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor
     bias = _int4_checked("linear_int4", x, weight, bias)
     (n, k), blocks = weight.shape, weight.blocks
     y = torch.empty_strided((x.shape[0], n), (n, 1), dtype=torch.bfloat16, device=x.device)
-    floats = _int4_scratch(x.shape[0], n, k)
-    # for sums that several thread blocks share: of this call alone, so that calls at once and captured graphs do not meet in it
-    scratch = torch.empty_strided((floats,), (1,), dtype=torch.float32, device=x.device) if floats else None
+    scratch, floats = _scratch("gemm_int4", "fms_linear_int4_scratch", x.device, x.shape[0], n, k)
     ops._call("gemm_int4", "fms_linear_int4", x, blocks, bias, y, x.shape[0], n, k, blocks.shape[1], weight.per, scratch, floats,
               ops.error_flag(x.device), ops._stream())
     return y
-
-
-def _int4_scratch(rows: int, n: int, k: int) -> int:
-    if rows <= INT4_FEW_ROWS:
-        return 0
-    f = _int4_scratch_of.get(ops._device())
-    if f is None:
-        from .build import load_library
-
-        f = load_library("gemm_int4").fms_linear_int4_scratch
-        f.restype, f.argtypes = ctypes.c_long, [ctypes.c_int] * 3
-        _int4_scratch_of[ops._device()] = f
-    return f(rows, n, k)
-
-
-_int4_scratch_of = {}  # by device
 
 
 def gated_linear_int4(x: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor], activation: int) -> torch.Tensor:

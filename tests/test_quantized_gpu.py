@@ -162,7 +162,9 @@ def test_ties_go_to_the_even_value(ops, rows, dim):
 
 # ---- products of 8-bit rows and weights --------------------------------------------------------------------------------
 SHAPES = [(1, 1, 1), (1, 16, 16), (3, 37, 75), (8, 300, 128), (16, 129, 400), (17, 128, 256), (64, 200, 4096), (100, 72, 1000), (128, 130, 640),
-          (129, 65, 136), (200, 1000, 272), (256, 256, 2048), (257, 100, 96), (300, 520, 1040), (513, 264, 640), (1100, 1536, 512)]
+          (129, 65, 136), (200, 1000, 272), (256, 256, 2048), (257, 100, 96), (300, 520, 1040), (513, 264, 640), (1100, 1536, 512),
+          # equal runs of a multiprocessor's steps, joined by a second kernel; more tiles than multiprocessors
+          (5, 72, 2600), (130, 1000, 2500), (256, 2100, 4100), (33, 20000, 96), (200, 38000, 64)]
 
 
 def e4m3_case(m, n, k, seed, big=8):
@@ -197,10 +199,11 @@ def test_linear_e4m3(ops, m, n, k, out_dtype, biased):
     assert torch.equal(ops.linear(x, w, bias, out_dtype), y)
 
 
+@pytest.mark.parametrize("k", [1040, 2576])
 @pytest.mark.parametrize("m", [1, 7, 40, 256, 300])
-def test_a_row_of_linear_e4m3_does_not_depend_on_the_others(ops, m):
+def test_a_row_of_linear_e4m3_does_not_depend_on_the_others(ops, m, k):
     g = gen(m)
-    x, w = ops.quantize_rows(normal(g, m, 1040)), ops.quantize_e4m3(normal(g, 520, 1040, std=0.02))
+    x, w = ops.quantize_rows(normal(g, m, k)), ops.quantize_e4m3(normal(g, 520, k, std=0.02))
     y = ops.linear_e4m3(x, w, None, F32)
     x.values.view(torch.uint8)[: m - 1] = 0x7F  # NaN
     x.scales[: m - 1] = float("nan")
@@ -212,7 +215,8 @@ def test_a_row_of_linear_e4m3_does_not_depend_on_the_others(ops, m):
 
 
 @pytest.mark.parametrize("act", [0, 1, 2, 3])
-@pytest.mark.parametrize("m,hidden,k", [(1, 5, 40), (8, 200, 256), (33, 100, 512), (250, 72, 144), (300, 300, 512), (1100, 264, 256)])
+@pytest.mark.parametrize("m,hidden,k", [(1, 5, 40), (8, 200, 256), (33, 100, 512), (250, 72, 144), (300, 300, 512), (1100, 264, 256),
+                                        (7, 300, 2600), (256, 1000, 4100), (33, 9600, 144), (130, 19000, 64)])
 def test_gated_linear_e4m3(ops, act, m, hidden, k):
     g = gen(act + m)
     x, w = ops.quantize_rows(normal(g, m, k)), ops.quantize_e4m3(normal(g, 2 * hidden, k, std=k ** -0.5))
