@@ -83,14 +83,21 @@ int multiprocessors() {
   return sms;
 }
 
+// The run of steps of block b of `blocks`: [first_step(b), first_step(b + 1)); and the block of a step
+__host__ __device__ inline int first_step(int b, int blocks, int steps) { return (int)((long)b * steps / blocks); }
+__device__ __forceinline__ int block_of_step(int step, int blocks, int steps) { return (int)((((long)step + 1) * blocks - 1) / steps); }
+
 // ---- up to 8 rows -------------------------------------------------------------------------------------------------------
-// Bound by reading the weights once, and by the instructions that unpack them (some 190 for 16 rows x 128 k).  Persistent thread
-// blocks take 16 rows of w at a time (GLU: the gate rows and then the up rows that belong to them); their warps share the 128-k
-// blocks and add their sums in shared memory in a fixed order, into one of two buffers in turn, so that a tile costs one barrier
-// and the loads of the next go on across it.  A lane loads its pieces of two rows of a block straight into registers, AHEAD
-// blocks ahead; x comes from the first-level cache.  (28,672 x 4,096 by one row 17.0 us; with rings in shared memory fed by bulk
-// copies 22.7, which take 110 cycles a block, and by asynchronous copies of each lane's own 19.6, for the instructions they cost.)
-constexpr int FEW_ROWS = 8, AHEAD = 2;
+// Bound by reading the weights once, and by the instructions that unpack them.  A thread block, one or two a multiprocessor,
+// takes an equal run of tiles, 16 rows of w each (GLU: of gate rows and the up rows that belong to them), as many at a time as it
+// has warps; each warp takes an equal run of their 128-k blocks, whatever tiles these belong to, two at most, and leaves a sum of
+// each in shared memory; after the one barrier those of a tile are added in the order of k.  A lane loads its pieces of two rows
+// of a block straight into registers, AHEAD blocks ahead, as many as 64 registers hold (28,672 x 4,096 by one row with groups of
+// 128, 1 / 2 / 3 ahead 14.8 / 14.2 / 16.6 us; of 64, 1 / 2 ahead 15.2 / 17.1); x comes from the first-level cache.
+// 28,672 x 4,096 by one row 14.2 us, by eight 15.6, gated 16.0 (tiles shared by the warps of a block one after the other, with a
+// barrier each: 17.0, gated 23.5; rings in shared memory fed by bulk copies 22.7; without unpacking 12.6, without that and
+// the loads of x 11.2; with half the shifts as wide products 18.0; 16 warps 4 blocks ahead 17.6).
+constexpr int FEW_ROWS = 8, FEW_WARPS = 32;
 
 __device__ __forceinline__ void mma_bf16_first(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
@@ -114,138 +121,142 @@ __device__ __forceinline__ uint32_t load_once(const uint32_t* p) {
 }
 
 template <int PER, bool GLU>
-__global__ void __launch_bounds__(1024, 1) int4_few_rows_kernel(Int4Args p) {
-  constexpr int BYTES = WEIGHT_BYTES + 64 * PER;
-  extern __shared__ float4 red[];  // [2][warps][32]
+__global__ void __launch_bounds__(32 * FEW_WARPS, 1) int4_few_rows_kernel(Int4Args p, int log_warps, int at_once, int each, int more) {
+  constexpr int BYTES = WEIGHT_BYTES + 64 * PER, AHEAD = PER == 1 ? 2 : 1;
+  extern __shared__ float4 sums[][2][32];  // of a warp's first and second tile: lane l has rows l / 4 and + 8 by tokens 2 (l % 4) and + 1
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, c = lane & 3;
-  // GLU: tile 2 i is gate block i, tile 2 i + 1 the up block that belongs to it, both of this thread block
-  const int out_blocks = (p.outputs + BLOCK_ROWS - 1) / BLOCK_ROWS, up = p.outputs / BLOCK_ROWS;
-  const int mine = (out_blocks - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x * (GLU ? 2 : 1);
-  auto block_of = [&](int j) {  // the rows of tile j of this thread block
-    return GLU ? (int)(blockIdx.x + (j >> 1) * gridDim.x) + (j & 1) * up : (int)(blockIdx.x + j * gridDim.x);
-  };
-  // what this warp loads next: block `next_kb` of tile `next_j`, at the lane's pieces (those of rows g and g + 8 lie 512 bytes apart)
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int warps = 1 << log_warps, t_lo = blockIdx.x * each + min((int)blockIdx.x, more), t_hi = t_lo + each + ((int)blockIdx.x < more);
+  const int rounds = (t_hi - t_lo + at_once - 1) / at_once, per_round = rounds == 1 ? t_hi - t_lo : (t_hi - t_lo + rounds - 1) / rounds;
+  // the lane's pieces of a block (those of rows g and g + 8 lie 512 bytes apart)
   const int piece = g * 64 + (c ^ ((g >> 1) & 3)) * 16, word = WEIGHT_BYTES + g * 4 - piece;
-  int next_j = 0, next_kb = warp;
-  const unsigned char* next = p.w + ((size_t)block_of(0) * p.k_blocks + warp) * BYTES + piece;
-  uint4 w[AHEAD][2];
-  uint32_t gw[AHEAD][2 * PER];
-  auto load = [&](int at) {
-    if (next_j >= mine) return;
-    w[at][0] = load_once(reinterpret_cast<const uint4*>(next));
-    w[at][1] = load_once(reinterpret_cast<const uint4*>(next + 512));
-#pragma unroll
-    for (int u = 0; u < 2 * PER; ++u) gw[at][u] = load_once(reinterpret_cast<const uint32_t*>(next + word + u * 32));
-    next += (size_t)warps * BYTES;
-    next_kb += warps;
-    if (next_kb >= p.k_blocks) {
-      next_kb = warp;
-      if (++next_j < mine) next = p.w + ((size_t)block_of(next_j) * p.k_blocks + warp) * BYTES + piece;
-    }
-  };
-  const int n = warp < p.k_blocks ? (p.k_blocks - warp + warps - 1) / warps : 0;  // blocks of a tile for this warp
-  if (n == 0) next_j = mine;
-#pragma unroll
-  for (int q = 0; q < AHEAD; ++q) load(q);  // weights: before the wait for the kernel that makes x
+  const size_t to_up = (size_t)(p.outputs / BLOCK_ROWS) * p.k_blocks * BYTES;  // GLU: from a gate block to its up block
   // a lane without a row of x of its own reads the first: its sums are not stored
   const __nv_bfloat16* xp = p.x + (size_t)(g < p.M ? g : 0) * p.K + 8 * c;
-  pdl_wait();
 
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, gate = 0.f;
-  auto multiply = [&](const uint4* wq, const uint32_t* gq, int kb) {
-    uint4 b[4];
-    const int left = p.K - kb * BLOCK_K;  // K is a multiple of 8: a lane's 8 values are all inside or all outside
-    const uint4* xs = reinterpret_cast<const uint4*>(xp + (size_t)kb * BLOCK_K);
-    if (left >= BLOCK_K) {
+  for (int from = t_lo; from < t_hi; from += per_round) {
+    const int count = min(per_round, t_hi - from);
+    const int gates = count * p.k_blocks, units = GLU ? 2 * gates : gates;  // GLU: all gate blocks, then all up blocks
+    // warp w has units [run(w), run(w + 1)), fewer units than warps one each
+    auto run = [&](int w) { return units < warps ? min(w, units) : (int)((unsigned)(units * w) >> log_warps); };
+    auto warp_of = [&](int unit) { return units < warps ? unit : (int)((((unsigned)(unit + 1) << log_warps) - 1) / (unsigned)units); };
+    const int u = run(warp);
+    int todo = run(warp + 1) - u;
+    const unsigned char* next = p.w + ((size_t)from * p.k_blocks + u) * BYTES + piece;
+    if (GLU && u >= gates) next += to_up - (size_t)gates * BYTES;
+    int turn = GLU ? gates - u : 0;  // loads until the first of an up block
+    uint4 w[AHEAD][2];
+    uint32_t gw[AHEAD][2 * PER];
+    auto load = [&](int at) {
+      w[at][0] = load_once(reinterpret_cast<const uint4*>(next));
+      w[at][1] = load_once(reinterpret_cast<const uint4*>(next + 512));
 #pragma unroll
-      for (int u = 0; u < 4; ++u) b[u] = __ldg(xs + 4 * u);
-    } else {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) b[u] = left > 32 * u + 8 * c ? __ldg(xs + 4 * u) : make_uint4(0, 0, 0, 0);
-    }
-    const uint32_t wl[4] = {wq[0].x, wq[0].y, wq[0].z, wq[0].w}, wh[4] = {wq[1].x, wq[1].y, wq[1].z, wq[1].w};
-#pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const uint32_t gl = gq[2 * u], gh = gq[2 * u + 1];
-      const __nv_bfloat162 zl = zero_of(gl), zh = zero_of(gh);
-      float part[4];
-#pragma unroll
-      for (int v = u * (4 / PER); v < (u + 1) * (4 / PER); ++v) {
-        uint32_t a[4], d[4];
-        unpack8(wl[v], zl, a);
-        unpack8(wh[v], zh, d);
-        if (v == u * (4 / PER)) mma_bf16_first(part, a[0], d[0], a[1], d[1], b[v].x, b[v].y);
-        else mma_bf16(part, a[0], d[0], a[1], d[1], b[v].x, b[v].y);
-        mma_bf16(part, a[2], d[2], a[3], d[3], b[v].z, b[v].w);
-      }
-      const float sl = __uint_as_float(gl << 16), sh = __uint_as_float(gh << 16);
-      acc[0] = fmaf(part[0], sl, acc[0]);
-      acc[1] = fmaf(part[1], sl, acc[1]);
-      acc[2] = fmaf(part[2], sh, acc[2]);
-      acc[3] = fmaf(part[3], sh, acc[3]);
-    }
-  };
-  auto finish = [&](int j) {  // all warps have their sums of tile j
-    float4* sums = red + (size_t)(j & 1) * warps * 32;
-    sums[warp * 32 + lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
-    __syncthreads();
-    // thread: element e of lane l, which is (row l / 4 + 8 (e / 2) of the tile, row 2 (l % 4) + e % 2 of x)
-    for (int t = threadIdx.x; t < 128; t += blockDim.x) {
-      const int l = t >> 2, e = t & 3, m = 2 * (l & 3) + (e & 1), col = block_of(GLU ? j & ~1 : j) * BLOCK_ROWS + (l >> 2) + 8 * (e >> 1);
-      if (m >= p.M || col >= p.outputs) continue;
-      float v = p.bias ? __bfloat162float(p.bias[GLU && (j & 1) ? p.outputs + col : col]) : 0.f, total = 0.f;
-      for (int i = 0; i < warps; ++i) total += reinterpret_cast<const float*>(sums + i * 32)[t];
-      v += total;
-      if (GLU && !(j & 1)) {
-        gate = v;  // at least 128 threads: the same one finishes the up rows
-        continue;
-      }
-      if (GLU) v = activate(gate, p.act) * v;
-      if (FMS_IN((size_t)m * p.outputs + col, (size_t)p.M * p.outputs)) p.y[(size_t)m * p.outputs + col] = __float2bfloat16_rn(v);
-    }
-  };
-  int i = 0, j = 0;  // block of the tile, tile
-  if (n == 0) {
-    for (; j < mine; ++j) finish(j);
-    return;
-  }
-  while (j < mine) {
+      for (int i = 0; i < 2 * PER; ++i) gw[at][i] = load_once(reinterpret_cast<const uint32_t*>(next + word + i * 32));
+      next += BYTES;
+      if (GLU && --turn == 0) next += to_up - (size_t)gates * BYTES;
+    };
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q)
-      if (j < mine) {  // of the whole warp
-        multiply(w[q], gw[q], warp + i * warps);
-        load(q);
-        if (++i == n) {
-          i = 0;
-          finish(j++);
-        }
+      if (q < todo) load(q);  // weights: before the wait for the kernel that makes x
+    if (from == t_lo) pdl_wait();
+
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    int slot = 0, left = p.K - u % p.k_blocks * BLOCK_K;  // values of the tile from this block on
+    const uint4* xs = reinterpret_cast<const uint4*>(xp + (p.K - left));
+    auto multiply = [&](const uint4* wq, const uint32_t* gq) {
+      uint4 b[4];
+      if (left >= BLOCK_K) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) b[v] = __ldg(xs + 4 * v);
+      } else {  // K is a multiple of 8: a lane's 8 values are all inside or all outside
+#pragma unroll
+        for (int v = 0; v < 4; ++v) b[v] = left > 32 * v + 8 * c ? __ldg(xs + 4 * v) : make_uint4(0, 0, 0, 0);
       }
+      const uint32_t wl[4] = {wq[0].x, wq[0].y, wq[0].z, wq[0].w}, wh[4] = {wq[1].x, wq[1].y, wq[1].z, wq[1].w};
+#pragma unroll
+      for (int h = 0; h < PER; ++h) {
+        const uint32_t gl = gq[2 * h], gh = gq[2 * h + 1];
+        const __nv_bfloat162 zl = zero_of(gl), zh = zero_of(gh);
+        float part[4];
+#pragma unroll
+        for (int v = h * (4 / PER); v < (h + 1) * (4 / PER); ++v) {
+          uint32_t a[4], d[4];
+          unpack8(wl[v], zl, a);
+          unpack8(wh[v], zh, d);
+          if (v == h * (4 / PER)) mma_bf16_first(part, a[0], d[0], a[1], d[1], b[v].x, b[v].y);
+          else mma_bf16(part, a[0], d[0], a[1], d[1], b[v].x, b[v].y);
+          mma_bf16(part, a[2], d[2], a[3], d[3], b[v].z, b[v].w);
+        }
+        const float sl = __uint_as_float(gl << 16), sh = __uint_as_float(gh << 16);
+        acc[0] = fmaf(part[0], sl, acc[0]);
+        acc[1] = fmaf(part[1], sl, acc[1]);
+        acc[2] = fmaf(part[2], sh, acc[2]);
+        acc[3] = fmaf(part[3], sh, acc[3]);
+      }
+    };
+    while (todo > 0) {
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q)
+        if (todo > 0) {  // of the whole warp
+          multiply(w[q], gw[q]);
+          if (todo > AHEAD) load(q);
+          --todo;
+          left -= BLOCK_K;
+          xs += BLOCK_K / 8;
+          if (left <= 0 || todo == 0) {  // the tile's last block, or this warp's
+            sums[warp][slot++][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+            left = p.K;
+            xs = reinterpret_cast<const uint4*>(xp);
+          }
+        }
+    }
+    __syncthreads();
+    // thread: a row of x and a column of this round's
+    const int log_m = p.M > 4 ? 3 : (p.M > 2 ? 2 : p.M - 1), m = threadIdx.x & ((1 << log_m) - 1);
+    for (int local = threadIdx.x >> log_m; local < count * BLOCK_ROWS; local += 32 * warps >> log_m) {
+      const int tile = local >> 4, row = local & 15, col = from * BLOCK_ROWS + local;
+      if (m >= p.M || col >= p.outputs) continue;
+      const int at = ((row & 7) * 4 + (m >> 1)) * 4 + (row >> 3) * 2 + (m & 1);  // of 128
+      auto total = [&](int t) {
+        const int first = t * p.k_blocks, w_lo = warp_of(first), w_hi = warp_of(first + p.k_blocks - 1);
+        // only the first warp of a tile can have begun with an earlier one
+        float sum = reinterpret_cast<const float*>(sums[w_lo][run(w_lo) < first ? 1 : 0])[at];
+#pragma unroll 4
+        for (int i = w_lo + 1; i <= w_hi; ++i) sum += reinterpret_cast<const float*>(sums[i][0])[at];
+        return sum;
+      };
+      float v = total(tile);
+      if (p.bias) v += __bfloat162float(p.bias[col]);
+      if (GLU) {
+        float up = total(count + tile);
+        if (p.bias) up += __bfloat162float(p.bias[p.outputs + col]);
+        v = activate(v, p.act) * up;
+      }
+      if (FMS_IN((size_t)m * p.outputs + col, (size_t)p.M * p.outputs)) p.y[(size_t)m * p.outputs + col] = __float2bfloat16_rn(v);
+    }
+    if (rounds > 1) __syncthreads();
   }
 }
 
-template <int PER, bool GLU> int launch_few(const Int4Args& p, int warps, int grid, cudaStream_t stream) {
+template <int PER, bool GLU> int launch_few(const Int4Args& p, int warps, int tiles, int grid, cudaStream_t stream) {
   const int smem = 2 * warps * 32 * (int)sizeof(float4);  // 32 KB at most
-  fms_launch(int4_few_rows_kernel<PER, GLU>, dim3(grid), dim3(32 * warps), smem, stream, p);
+  fms_launch(int4_few_rows_kernel<PER, GLU>, dim3(grid), dim3(32 * warps), smem, stream, p, warps == 32 ? 5 : 4, GLU ? warps / 2 : warps, tiles / grid, tiles % grid);
   return fms_launch_status("gemm_int4");
 }
 template <bool GLU> int few(const Int4Args& p, cudaStream_t stream) {
-  // 32 warps a multiprocessor, as thread blocks of 8, 16 or 32: the cut whose rounds of tiles, each as long as its warps' blocks of k
-  // and a barrier, take least (8 / 16 / 32 warps in us: 28,672 x 4,096 17.1 / 17.6 / 20.6, 4,096 x 14,336 17.2 / 9.3 / 10.1,
-  // 6,144 x 4,096 6.3 / 6.0 / 5.8, 4,096 x 4,096 6.1 / 3.7 / 4.4)
+  // 32 warps a multiprocessor, as one thread block or two: by how many blocks of w a warp gets at most (16 : 32 warps in us:
+  // 28,672 x 4,096 14.5 : 14.2, 6,144 x 4,096 5.8 : 5.4, 512 x 16,384 7.8 : 6.0, 4,096 x 14,336 9.1 : 9.3, 4,096 x 4,096 4.1 : 4.5)
   const int sms = multiprocessors(), tiles = (p.outputs + BLOCK_ROWS - 1) / BLOCK_ROWS;
-  int best = 0, warps = 32;
-  for (int w = 8; w <= 32; w *= 2) {
-    const int slots = sms * (32 / w), cost = (tiles + slots - 1) / slots * (GLU ? 2 : 1) * ((p.k_blocks + w - 1) / w + 1);
-    if (best == 0 || cost < best) {
-      best = cost;
-      warps = w;
-    }
-  }
-  const int slots = sms * (32 / warps), grid = tiles < slots ? tiles : slots;
-  return p.per == 1 ? launch_few<1, GLU>(p, warps, grid, stream)
-                    : (p.per == 2 ? launch_few<2, GLU>(p, warps, grid, stream) : launch_few<4, GLU>(p, warps, grid, stream));
+  auto most = [&](int warps) {
+    const int slots = sms * (FEW_WARPS / warps);
+    return ((long)((tiles + slots - 1) / slots) * (GLU ? 2 : 1) * p.k_blocks + warps - 1) / warps;
+  };
+  const int warps = most(16) <= most(32) ? 16 : 32, slots = sms * (FEW_WARPS / warps), grid = tiles < slots ? tiles : slots;
+  // blocks of w that a thread block has in hand at once, times its warps, are counted in 32 bits
+  if (p.k_blocks > 0x3fffffff / (FEW_WARPS * FEW_WARPS)) return fms_fail("gemm_int4: %d blocks of k", p.k_blocks);
+  return p.per == 1 ? launch_few<1, GLU>(p, warps, tiles, grid, stream)
+                    : (p.per == 2 ? launch_few<2, GLU>(p, warps, tiles, grid, stream) : launch_few<4, GLU>(p, warps, tiles, grid, stream));
 }
 
 // ---- what the tcgen05 kernels share --------------------------------------------------------------------------------------
@@ -370,10 +381,6 @@ struct RowsArgs {
   int n_tokens, stages, groups, a_stages, accs, acc_columns;
   float* scratch;  // [2 blocks][n_tokens][128]: a block's first tile, then its last, where it has not all of it
 };
-// The run of steps of block b of `blocks`: [first_step(b), first_step(b + 1)); and the block of a step
-__host__ __device__ inline int first_step(int b, int blocks, int steps) { return (int)((long)b * steps / blocks); }
-__device__ __forceinline__ int block_of_step(int step, int blocks, int steps) { return (int)((((long)step + 1) * blocks - 1) / steps); }
-
 __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid_constant__ CUtensorMap map_x,
                                                                     const __grid_constant__ CUtensorMap map_w, RowsArgs a,
                                                                     int* __restrict__ error_flag) {

@@ -238,7 +238,9 @@ def test_gated_linear_e4m3(ops, act, m, hidden, k):
 # ---- products with 4-bit weights ---------------------------------------------------------------------------------------
 INT4_SHAPES = [(1, 1, 8, 32), (1, 40, 32, 32), (3, 37, 72, 64), (8, 300, 128, 128), (8, 129, 1000, 32), (9, 200, 640, 128), (16, 10000, 256, 64), (16, 72, 4096, 4096),
                (5, 9600, 384, 128), (17, 128, 256, 128), (33, 130, 640, 64), (64, 264, 4096, 128), (100, 72, 1000, 32), (112, 4096, 512, 96), (128, 2100, 384, 256),
-               (129, 65, 136, 1000), (256, 256, 2048, 128), (257, 100, 96, 32), (600, 264, 1160, 160)]
+               (129, 65, 136, 1000), (256, 256, 2048, 128), (257, 100, 96, 32), (600, 264, 1160, 160),
+               # runs of a warp that reach into the next tile, with odd ends; more tiles than a thread block has warps
+               (2, 4720, 1288, 128), (7, 7120, 648, 64), (3, 2400, 2056, 32), (4, 90000, 136, 128), (1, 80000, 32, 32)]
 
 
 def int4_case(m, n, k, group, zeros, seed):
@@ -291,7 +293,8 @@ def test_a_row_of_linear_int4_does_not_depend_on_the_others(ops, m):
 
 
 @pytest.mark.parametrize("act", [0, 1, 2, 3])
-@pytest.mark.parametrize("m,hidden,k,group", [(1, 5, 40, 32), (1, 16, 136, 32), (8, 208, 256, 128), (8, 4992, 256, 64), (16, 4800, 384, 32), (9, 80, 1040, 1040), (16, 72, 144, 144), (17, 200, 256, 128)])
+@pytest.mark.parametrize("m,hidden,k,group", [(1, 5, 40, 32), (1, 16, 136, 32), (8, 208, 256, 128), (8, 4992, 256, 64), (16, 4800, 384, 32), (9, 80, 1040, 1040), (16, 72, 144, 144), (17, 200, 256, 128),
+                                              (3, 4720, 1288, 128), (6, 2400, 648, 64), (2, 40000, 136, 128), (5, 39984, 72, 32)])
 def test_gated_linear_int4(ops, act, m, hidden, k, group):
     g = gen(act + m)
     w = ops.quantize_int4(normal(g, 2 * hidden, k, std=k ** -0.5), group)
