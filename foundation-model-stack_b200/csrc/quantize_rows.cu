@@ -13,7 +13,7 @@
 // so that nothing is read twice.  A thread owns runs of 8 neighbours, 16-byte loads and 8-byte stores.  Rows of a width that is no
 // multiple of 8 begin anywhere: their runs are moved forward by up to 3 values to where the rows' own loads are aligned, and a
 // warp's lanes hand one another the bytes that make aligned stores (1,100 x 5,001 bfloat16 7.7 us, and behind the norm, float32,
-// 22.9; 11.4 and 25.1 with single loads and stores).  Rows of q are `pitch` bytes apart, dim rounded up to 16 with zeros behind the last value, as the products'
+// 21.7; 11.4 and 25.1 with single loads and stores).  Rows of q are `pitch` bytes apart, dim rounded up to 16 with zeros behind the last value, as the products'
 // copies want them.
 //
 // q is what the exact quotient rounds to.  Of bfloat16 rows it is often a tie, and otherwise, a ratio of numbers of 11 and 8 bits,
@@ -192,9 +192,11 @@ __device__ __forceinline__ float largest(const Run<__nv_bfloat16>& r) {
 }
 
 // RUNS: runs of 8 values that a thread keeps; 0: any width, the row is read a second time.
+// What bounds many rows is how many of their bytes are on the way, so registers are kept few: three thread blocks of 448 for rows of
+// 14,336 (2,048 of them, bfloat16: 17.9 us, 4.9 TB/s; with two blocks 20.8, with four 19.2 for the registers that spill).
 template <typename T, int RUNS, bool NEIGHBOURS>
-__global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && RUNS != 1 && RUNS != 8 ? 2 : 1) quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales,
-                                                             int n_rows, int dim, int pitch) {
+__global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && RUNS == 4 && sizeof(T) == 2 ? 3 : (RUNS != 1 && RUNS != 8 ? 2 : 1))
+    quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales, int n_rows, int dim, int pitch) {
   __shared__ float scratch[32];
   pdl_launch_dependents();
   pdl_wait();
@@ -233,11 +235,10 @@ struct Pair {
 __device__ __forceinline__ Pair larger(Pair a, Pair b) { return b.hi > a.hi || (b.hi == a.hi && b.lo > a.lo) ? b : a; }
 
 template <typename T, typename TG, int RUNS, bool NEIGHBOURS>
-__global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && (RUNS == 0 || RUNS == 2) ? 2 : 1) add_rmsnorm_quantized_kernel(float* __restrict__ residual, const T* __restrict__ delta,
-                                                                     const TG* __restrict__ gain, float eps,
-                                                                     uint8_t* __restrict__ q, float* __restrict__ scales,
-                                                                     const int* __restrict__ rows, int dim, int pitch,
-                                                                     int residual_rows) {
+__global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2 ? 2 : 1)
+    add_rmsnorm_quantized_kernel(float* __restrict__ residual, const T* __restrict__ delta, const TG* __restrict__ gain, float eps,
+                                 uint8_t* __restrict__ q, float* __restrict__ scales, const int* __restrict__ rows, int dim, int pitch,
+                                 int residual_rows) {
   __shared__ float scratch[3][32];
   constexpr int KEPT = RUNS > 0 ? RUNS : 1;
   const int runs = RUNS > 0 ? RUNS : (pitch / 8 + !NEIGHBOURS + blockDim.x - 1) / blockDim.x;
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && (RUNS ==
 
 // The runs of 8 that a thread keeps (0: the row is too wide for registers) and the threads for a row of `runs` of them.  Few
 // rows: a thread a run as far as 1,024 go, since only latency counts.  Many: `many` runs a thread, so that more bytes a thread and
-// more rows a multiprocessor are on their way (8,192 x 4,096 bfloat16 to e4m3 with 1 / 2 / 4 / 8 runs: 27.5 / 22.8 / 18.2 / 19.8 us;
+// more rows a multiprocessor are on their way (8,192 x 4,096 bfloat16 to e4m3 with 1 / 2 / 4 / 8 runs: 27.5 / 22.8 / 16.9 / 19.8 us;
 // behind the norm, whose runs take 12 registers and more, 2,048 x 4,096 with 1 / 2 / 4: 22.4 / 17.3 / 18.4 us).
 int kept_for(int runs, int n_rows, int many, int most_kept, int* threads) {
   int kept = n_rows <= 296 ? (runs <= 1024 ? 1 : 4) : (runs <= 128 ? 1 : many);
