@@ -286,8 +286,8 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
                : "memory");
 }
 // by a whole warp, which gives up as one
-__device__ __forceinline__ bool warp_wait(void* bar, uint32_t parity, volatile int* failed) {
-  return __all_sync(0xffffffffu, wait_or_abort(bar, parity, failed));
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+  return __all_sync(0xffffffffu, quick_wait(bar, parity, failed));
 }
 // 32 columns of 32 bits of this thread's lane of tensor memory, written; not waited for
 __device__ __forceinline__ void tmem_store_pairs(uint32_t taddr, const uint32_t* r) {
@@ -363,22 +363,30 @@ template <int N> __device__ __forceinline__ void store_column(const Int4Args& p,
 // One thread block a multiprocessor; each takes an equal run of the steps of all tiles, a step being 128 rows of w by 128 k, so that
 // no multiprocessor waits for another's second tile (28,672 rows are 224 tiles for 148).  Where a tile's steps fall to several
 // blocks, each leaves its sums in a slot of its own in scratch memory, and a second kernel adds them in the order of k.  The
-// cut depends on the weights' shape alone, so a row's result does not depend on the rest of the batch.
-//   warp 0      per step: two 64-k boxes of x and one of the eight blocks of w, into one of up to 8 stages
-//   warp 1      one lane issues 8 instructions (128 x tokens x 16) a step
+// cut depends on the weights' shape alone, so among batches of up to 64 rows, and among larger ones, a row's result does not depend on
+// the rest of the batch.
+//   warp 0      per step one copy, the eight blocks of w, into one of up to 8 stages; warp 22 two 64-k boxes of x beside them
+//   warp 1      one lane issues 8 instructions (128 x tokens x 16) a step.  What a step costs is the instructions of these single
+//               threads more than the tensor cores (some 700 cycles against 260 at 64 tokens), so up to 64 tokens warp 23 takes every
+//               second step, into accumulators of its own that the epilogue adds, and a step's copies are waited for by those who unpack
+//               it alone: an issuer sees them by way of the operand's barrier.  (One issuer, one thread for all copies: 4,096 x 14,336
+//               by 16 rows 13.6 us, by 64 16.8, 28,672 x 4,096 22.7 and 26.5; so 11.6, 15.6, 19.6, 24.0.  Two issuers for
+//               128 tokens leave room for 4 stages of the operand and 4 of copies: 100 rows 18.7 -> 21.9 us.)
 //   warps 2-17  up to four groups of four unpack every fourth step each, a thread a row of w, into the next of up to 7 stages of the
-//               operand, 64 columns each: what the accumulators leave of the 512 (with a stage a group, a group waited for its
-//               own step's products before it went on: 800 cycles a step).  A group waits for its columns before it waits for a
-//               step's copies: the steps up to `a_stages` before are used up then, and with no fewer copies' stages and no more
-//               groups than that, neither barrier can be a phase behind.
-//   warps 18-21 the epilogue; two accumulators up to 64 tokens, so that it runs under the next tile's steps
+//               operand, 64 columns each
+//   warps 18-21 the epilogue; two accumulators (of each issuer) up to 64 tokens, so that it runs under the next tile's steps
+// No wait may meet a barrier that is a phase behind.  One issuer: steps are used up in order, a group waits for its stage of the operand
+// before it waits for a step's copies, and there are no fewer copies' stages than operand's stages and no fewer of these than groups.
+// Two: their numbers are multiples of the groups', so that the group of a step has itself waited for the last use of either stage,
+// and of the issuers', so that a stage of the operand is always the same issuer's.
 // Every wait on an mbarrier is bounded: on a time-out the block records error 4, skips the rest of its work and still frees its
 // tensor memory.
-constexpr int GROUPS = 4, UNPACK_WARPS = 4 * GROUPS, ROWS_THREADS = 64 + 32 * (UNPACK_WARPS + 4), MAX_STAGES = 8, A_FIRST = 256, MAX_A = 7;
+constexpr int GROUPS = 4, UNPACK_WARPS = 4 * GROUPS, X_WARP = 6 + UNPACK_WARPS, SECOND_ISSUER = 7 + UNPACK_WARPS,
+              ROWS_THREADS = 32 * (UNPACK_WARPS + 8), MAX_STAGES = 8, A_FIRST = 256, MAX_A = 7;
 
 struct RowsArgs {
   Int4Args p;
-  int n_tokens, stages, groups, a_stages, accs, acc_columns;
+  int n_tokens, stages, groups, a_stages, issuers, accs, acc_columns;
   float* scratch;  // [2 blocks][n_tokens][128]: a block's first tile, then its last, where it has not all of it
 };
 __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid_constant__ CUtensorMap map_x,
@@ -406,7 +414,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid
   if (threadIdx.x == 0) {
     failed_flag = 0;
     for (int s = 0; s < MAX_STAGES; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 2);
       mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < MAX_A; ++i) {
@@ -414,7 +422,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid
       mbar_init(&a_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_full[i], a.issuers);
       mbar_init(&acc_empty[i], 4);  // the warps of the epilogue
     }
     mbar_fence_init();
@@ -423,62 +431,67 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot, tmem_a = tmem + a.accs * a.acc_columns;
+  const uint32_t tmem = *tmem_slot, tmem_a = tmem + a.accs * a.issuers * a.acc_columns;
   pdl_launch_dependents();  // now: a block of the next kernel must not take the tensor memory that this one still needs
 
   if (warp == 0) {
-    if (elect_one()) {
+    if (elect_one()) {  // the weights, which do not depend on the kernel before
       int tile = lo / p.k_blocks, k = lo - tile * p.k_blocks, s = 0;
-      auto load_w = [&](int to, int t, int kb) {
-        mbar_arrive_expect_tx(&full[to], x_bytes + TILE / BLOCK_ROWS * bytes);
-        tma_load_3d(smem + to * stage_bytes + x_bytes, &map_w, 0, kb, t * (TILE / BLOCK_ROWS), &full[to]);
-      };
-      auto load_x = [&](int to, int kb) {
-        tma_load_2d(smem + to * stage_bytes, &map_x, kb * BLOCK_K, 0, &full[to]);
-        tma_load_2d(smem + to * stage_bytes + x_bytes / 2, &map_x, kb * BLOCK_K + 64, 0, &full[to]);
-      };
-      const int early = min(stages, hi - lo);
-      for (int i = 0, t = tile, kb = k; i < early; ++i) {  // weights do not depend on the kernel before
-        load_w(i, t, kb);
-        if (++kb == p.k_blocks) kb = 0, ++t;
-      }
-      pdl_wait();
+      const int w_bytes = TILE / BLOCK_ROWS * bytes;
       uint32_t phase = 1;
-      for (int i = lo; i < hi && !*failed; ++i) {
-        if (i - lo >= early) {
-          if (!wait_or_abort(&empty[s], phase, failed)) break;
-          load_w(s, tile, k);
-        }
-        load_x(s, k);
+      for (int i = lo; i < hi; ++i) {
+        if (!quick_wait(&empty[s], phase, failed)) break;
+        mbar_arrive_expect_tx(&full[s], w_bytes);
+        tma_load_3d(smem + s * stage_bytes + x_bytes, &map_w, 0, k, tile * (TILE / BLOCK_ROWS), &full[s]);
         if (++k == p.k_blocks) k = 0, ++tile;
         if (++s == stages) s = 0, phase ^= 1;
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == X_WARP) {
     if (elect_one()) {
-      const uint32_t idesc = umma_idesc(TILE, a.n_tokens);
-      const MatrixDesc base(smem_u32(smem));
-      const uint32_t box = (uint32_t)x_bytes / 2 >> 4;
-      int k = lo % p.k_blocks, s = 0, stage = 0, acc = 0;
-      uint32_t phase = 0, turn = 0, acc_phase = 1;
+      pdl_wait();
+      int k = lo % p.k_blocks, s = 0;
+      uint32_t phase = 1;
       for (int i = lo; i < hi; ++i) {
-        const bool first = i == lo || k == 0;
-        if (first && !wait_or_abort(&acc_empty[acc], acc_phase, failed)) break;
-        if (!quick_wait(&full[s], phase, failed) || !quick_wait(&a_full[stage], turn, failed)) break;
-        tc_fence_after();
-        const uint32_t d = tmem + acc * a.acc_columns, ta = tmem_a + stage * A_COLUMNS, b = base.lo + (uint32_t)(s * stage_bytes >> 4);
-#pragma unroll
-        for (int kk = 0; kk < BLOCK_K / 16; ++kk)  // 64 k a box of x, 32 bytes of its rows an instruction
-          issue_a_tmem(d, ta + kk * 8, b + (kk & 3) * 2 + (kk < 4 ? 0 : box), base.hi, idesc, kk > 0 ? 1u : !first);
-        tc_commit(&empty[s]);
-        tc_commit(&a_empty[stage]);
+        if (!quick_wait(&empty[s], phase, failed)) break;
+        mbar_arrive_expect_tx(&full[s], x_bytes);
+        tma_load_2d(smem + s * stage_bytes, &map_x, k * BLOCK_K, 0, &full[s]);
+        tma_load_2d(smem + s * stage_bytes + x_bytes / 2, &map_x, k * BLOCK_K + 64, 0, &full[s]);
         if (++k == p.k_blocks) k = 0;
-        if (k == 0 || i + 1 == hi) {
-          tc_commit(&acc_full[acc]);
-          if (++acc == a.accs) acc = 0, acc_phase ^= 1;
-        }
         if (++s == stages) s = 0, phase ^= 1;
-        if (++stage == a.a_stages) stage = 0, turn ^= 1;
+      }
+    }
+  } else if (warp == 1 || warp == SECOND_ISSUER) {
+    const int mine = warp == 1 ? 0 : 1;
+    if (mine < a.issuers && elect_one()) {
+      const uint32_t idesc = umma_idesc(TILE, a.n_tokens), box = (uint32_t)x_bytes / 2 >> 4;
+      const MatrixDesc base(smem_u32(smem));
+      int i = lo + mine, s = mine, stage = mine, acc = 0, from = lo;
+      uint32_t turn = 0, acc_phase = 1;
+      bool ok = true;
+      while (from < hi) {
+        const int to = min(from - from % p.k_blocks + p.k_blocks, hi);
+        const uint32_t d = tmem + (acc * a.issuers + mine) * a.acc_columns;
+        if (!quick_wait(&acc_empty[acc], acc_phase, failed)) break;
+        for (uint32_t more = 0; i < to; i += a.issuers, more = 1) {
+          // the group has seen the step's copies land, x among them
+          if (!(ok = quick_wait(&a_full[stage], turn, failed))) break;
+          tc_fence_after();
+          const uint32_t ta = tmem_a + stage * A_COLUMNS, b = base.lo + (uint32_t)(s * stage_bytes >> 4);
+#pragma unroll
+          for (int kk = 0; kk < BLOCK_K / 16; ++kk)  // 64 k a box of x, 32 bytes of its rows an instruction
+            issue_a_tmem(d, ta + kk * 8, b + (kk & 3) * 2 + (kk < 4 ? 0 : box), base.hi, idesc, kk > 0 ? 1u : more);
+          tc_commit(&empty[s]);
+          tc_commit(&a_empty[stage]);
+          s += a.issuers;
+          if (s >= stages) s -= stages;
+          stage += a.issuers;
+          if (stage >= a.a_stages) stage -= a.a_stages, turn ^= 1;
+        }
+        if (!ok) break;
+        tc_commit(&acc_full[acc]);
+        if (++acc == a.accs) acc = 0, acc_phase ^= 1;
+        from = to;
       }
     }
   } else if (warp < 2 + UNPACK_WARPS) {
@@ -510,7 +523,18 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid
       tc_fence_after();
       for (int c0 = 0; c0 < a.n_tokens; c0 += 16) {
         float v[16];
-        tmem_load_16(tmem + acc * a.acc_columns + ((uint32_t)(quarter * 32) << 16) + c0, v);
+        const uint32_t at = tmem + acc * a.issuers * a.acc_columns + ((uint32_t)(quarter * 32) << 16) + c0;
+        if (k_hi - k_lo == 1) {  // one accumulator alone has sums
+          tmem_load_16(at + (a.issuers == 2 && ((i - lo) & 1) ? a.acc_columns : 0), v);
+        } else {
+          tmem_load_16(at, v);
+          if (a.issuers == 2) {
+            float second[16];
+            tmem_load_16(at + a.acc_columns, second);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] += second[j];
+          }
+        }
         if (whole) {
           if (col < p.N) store_column<16>(p, v, c0, col, bias);
         } else {
@@ -569,8 +593,8 @@ __global__ void __launch_bounds__(TILE) int4_join_kernel(RowsArgs a, int blocks)
 constexpr size_t SMEM_LEAST = 200 * 1024, SMEM_MOST = 225 * 1024, EXTRA = 1024 /* alignment */ + 512 /* barriers */;
 
 // The most rows of x that this kernel takes: 256, but 112 where the pairs of the kernel below have a tile each.  This one / that one in
-// us, by rows: 28,672 x 4,096 96 31.8 / 32.3, 128 38.7 / 32.4, 256 72.2 / 60.6; 6,144 x 4,096 128 13.0 / 16.3, 256 19.5 / 17.3; 4,096 x
-// 14,336 128 19.9 / 42.9, 256 29.7 / 44.7.
+// us, by rows: 28,672 x 4,096 96 31.4 / 32.3, 128 38.7 / 32.4, 256 72.2 / 60.6; 6,144 x 4,096 128 13.5 / 16.3, 256 20.5 / 17.3; 4,096 x
+// 14,336 128 20.4 / 42.9, 256 30.9 / 44.7.
 int rows_most(int N) { return (long)N >= 2L * TILE * (multiprocessors() / 2) ? 112 : 256; }
 int rows_blocks(int N, int K) {
   const long steps = (long)((N + TILE - 1) / TILE) * ((K + BLOCK_K - 1) / BLOCK_K);
@@ -591,8 +615,14 @@ int launch_rows(const Int4Args& p, float* scratch, long scratch_floats, int* err
   a.stages = min((int)((SMEM_MOST - EXTRA) / stage_bytes), MAX_STAGES);
   a.acc_columns = (a.n_tokens + 31) / 32 * 32;
   a.accs = a.n_tokens <= 64 ? 2 : 1;
-  a.a_stages = min(min(MAX_A, (512 - a.accs * a.acc_columns) / A_COLUMNS), a.stages);
-  a.groups = min(GROUPS, a.a_stages);
+  a.issuers = a.n_tokens <= 64 ? 2 : 1;
+  if (a.issuers == 2) {  // 8 stages of copies, or 4
+    a.a_stages = a.groups = GROUPS;
+    a.stages = a.stages / GROUPS * GROUPS;
+  } else {
+    a.a_stages = min(min(MAX_A, (512 - a.accs * a.acc_columns) / A_COLUMNS), a.stages);
+    a.groups = min(GROUPS, a.a_stages);
+  }
   CUtensorMap map_x, map_w;
   if (make_map(&map_x, p.x, p.M, p.K, a.n_tokens) || make_block_map(&map_w, p)) return 1;
   static uint64_t allowed = 0;
