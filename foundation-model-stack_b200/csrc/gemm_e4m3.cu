@@ -166,8 +166,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   cluster_sync_all();  // the partner's barriers exist before anything is sent to them
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_launch_dependents();  // now: a block of the next kernel must not take the tensor memory that this one still needs
-  pdl_wait();
 
   if (warp == 0) {
     if (elect_one()) {
@@ -601,8 +599,9 @@ int launch(const void* x, const void* w, Epilogue ep, int M, int N, long pitch, 
   const long tiles = (long)((ep.outputs + out - 1) / out) * tiles_m;
   if (tiles > 0x7fffffffL) return fms_fail("gemm_e4m3: %ld tiles", tiles);
   const int busy = (int)(tiles < pairs ? tiles : pairs);
-  fms_launch(e4m3_pair_kernel, dim3(2 * busy), dim3(THREADS), PAIR_RING + EXTRA, stream, map_x, map_w, ep, M,
-             k_steps, error_flag);
+  // A plain launch: the pairs, which want all of the tensor memory, run beside no block of another kernel of the stream.  (Launched
+  // while the kernel before was still draining, a pair of blocks in a prompt of 8,192 tokens began and never got its tensor memory.)
+  e4m3_pair_kernel<<<dim3(2 * busy), dim3(THREADS), PAIR_RING + EXTRA, stream>>>(map_x, map_w, ep, M, k_steps, error_flag);
   return fms_launch_status("gemm_e4m3");
 }
 }  // namespace

@@ -696,8 +696,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   cluster_sync_all();  // the partner's barriers exist before anything is sent to them
   tc_fence_after();
   const uint32_t tmem = *tmem_slot, tmem_a = tmem + A_FIRST;
-  pdl_launch_dependents();  // now: a block of the next kernel must not take the tensor memory that this one still needs
-  pdl_wait();
 
   if (warp == 0) {
     if (elect_one()) {
@@ -813,8 +811,9 @@ int launch_pair(const Int4Args& p, int* error_flag, cudaStream_t stream) {
   static uint64_t allowed = 0;
   if (allow_smem(int4_pair_kernel, (int)SMEM_MOST, &allowed)) return 1;
   const size_t smem = (size_t)a.stages * stage_bytes + EXTRA;
-  fms_launch(int4_pair_kernel, dim3(2 * (int)(tiles < pairs ? tiles : pairs)), dim3(PAIR_THREADS), smem < SMEM_LEAST ? SMEM_LEAST : smem,
-             stream, map_x, map_w, a, error_flag);
+  // a plain launch: the pairs, which want all of the tensor memory, run beside no block of another kernel of the stream
+  int4_pair_kernel<<<dim3(2 * (int)(tiles < pairs ? tiles : pairs)), dim3(PAIR_THREADS), smem < SMEM_LEAST ? SMEM_LEAST : smem, stream>>>(
+      map_x, map_w, a, error_flag);
   return fms_launch_status("gemm_int4");
 }
 

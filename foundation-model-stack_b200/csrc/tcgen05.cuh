@@ -21,7 +21,9 @@ __device__ __forceinline__ void tmem_alloc(void* smem_result, uint32_t columns) 
                : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
 }
+// An instruction of a whole warp, which after a part that one lane ran alone comes together first.
 __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t columns) {
+  __syncwarp();
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(columns) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
@@ -134,6 +136,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 }
 // every thread of both blocks; a hardware barrier, not a spin
 __device__ __forceinline__ void cluster_sync_all() {
+  __syncwarp();  // a warp arrives as one
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 // by the same warp of both blocks, with the same address for the result
@@ -143,6 +146,7 @@ __device__ __forceinline__ void tmem_alloc_pair(void* smem_result, uint32_t colu
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
 }
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t columns) {
+  __syncwarp();
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(columns) : "memory");
 }
 // A box into this block's shared memory; the bytes are counted on the leader's mbarrier at the same offset (the

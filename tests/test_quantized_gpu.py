@@ -365,6 +365,63 @@ def test_a_run_of_them_captured_replayed_and_on_another_stream(ops, rows):
             assert torch.equal(y, want)
 
 
+def test_tensor_memory_is_given_back(ops):
+    """Blocks that share a multiprocessor's tensor memory, many times over, and then kernels that want all of it."""
+    g = gen(5)
+    many, few = ops.quantize_e4m3(normal(g, 28672, 512, std=0.04)), ops.quantize_e4m3(normal(g, 512, 2576, std=0.02))
+    int4, bf16 = ops.quantize_int4(normal(g, 512, 512, std=0.04)), normal(g, 512, 512).to(BF16)
+    x, long, wide = ops.quantize_rows(normal(g, 32, 512)), ops.quantize_rows(normal(g, 32, 2576)), ops.quantize_rows(normal(g, 600, 512))
+    xb, wideb = normal(g, 32, 512).to(BF16), normal(g, 600, 512).to(BF16)
+
+    def run():
+        return [ops.gated_linear_e4m3(x, many, None, 0), ops.linear_e4m3(x, many), ops.linear_e4m3(long, few), ops.linear_int4(xb, int4), ops.linear(xb, bf16)]
+
+    def whole():
+        return [ops.linear_e4m3(wide, many), ops.linear_int4(wideb, int4), ops.linear(wideb, bf16)]
+
+    first, all_of_it = run(), whole()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured = [y for _ in range(8) for y in run()]
+    for _ in range(25):
+        graph.replay()
+        again = whole()
+    for y, want in zip(captured + again, 8 * first + all_of_it):
+        assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int4"])
+def test_layers_of_long_prompts_back_to_back(ops, kind):
+    """Many layers' launches in the queue at once, those of the pairs of thread blocks among kernels of thousands of blocks."""
+    g = gen(6)
+    make = ops.quantize_e4m3 if kind == "e4m3" else ops.quantize_int4
+    qkv, dense = make(normal(g, 1536, 1024, std=0.03)), make(normal(g, 1024, 1024, std=0.03))
+    wide, down = make(normal(g, 4096, 1024, std=0.03)), make(normal(g, 1024, 2048, std=0.03))
+    head, gain = normal(g, 4000, 1024).to(BF16), torch.ones(1024, device="cuda", dtype=BF16)
+    start = normal(g, 8192, 1024)
+
+    def norm(residual, delta, rows=None):
+        if kind == "e4m3":
+            return ops.add_rmsnorm_quantized(residual, delta, gain, 1e-5, rows)
+        return ops.add_rmsnorm(residual, delta, gain, 1e-5, BF16, rows)
+
+    def run():
+        residual, delta = start.clone(), None
+        for _ in range(12):
+            a = ops.linear(norm(residual, delta), qkv)
+            delta = ops.linear(a[:, :1024].contiguous(), dense)
+            delta = ops.linear(ops.gated_linear(norm(residual, delta), wide, None, 0), down)
+        rows = torch.arange(31, 8192, 256, device="cuda", dtype=torch.int32)
+        last = ops.add_rmsnorm(residual, delta, gain, 1e-5, BF16, rows)
+        return ops.linear(last, head)
+
+    first = run()
+    for _ in range(6):
+        again = run()
+    assert bool(torch.isfinite(first).all()) and torch.equal(again, first)
+
+
 def test_weights_straight_after_what_makes_them(ops):
     """A product asks for its weights before the kernel in front of it is done; the weight's constructor has waited for them."""
     g = gen(9)
