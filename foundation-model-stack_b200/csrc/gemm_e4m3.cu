@@ -13,7 +13,7 @@
 
 namespace {
 constexpr int TILE = 128, TILE_K = 128, UMMA_K = 32, MAX_STAGES = 12;
-constexpr int THREADS = 320, EPILOGUE_WARPS = 8;
+constexpr int THREADS = 320, EPILOGUE_WARPS = 8, ROWS_THREADS = THREADS + 32;
 constexpr int BOX_BYTES = TILE * TILE_K;  // 128 rows of an operand for one step
 
 #include "tcgen05.cuh"
@@ -269,14 +269,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 // tiles (cut_of): every multiprocessor takes an equal run of the steps of all tiles; where a tile's steps fall to several blocks,
 // each leaves its sums in a slot of its own in scratch memory, and a second kernel adds them in the order of k; under GLU all
 // tiles of such a cut go that way, since a gate and its up value lie in different lanes.  (Clusters that shared a tile and added
-// their sums through distributed shared memory: 6,144 x 4,096 by 64 rows 11.8 us, 4,096 x 14,336 17.7 us; so 10.0 and 15.1.)  The
+// their sums through distributed shared memory: 6,144 x 4,096 by 64 rows 11.8 us, 4,096 x 14,336 17.7 us; so 9.0 and 14.4.)  The
 // cut depends on the weights' shape alone, so a row's result does not depend on the rest of the batch.  The first stages'
 // boxes of w are asked for before griddepcontrol.wait: weights do not depend on the kernel before.
-//   warp 0 TMA, warp 1 the instructions, warps 2-9 the epilogue, under the next tile's steps up to 128 tokens
+//   warp 0 the copies of w, warp 10 those of x (one thread for both: 4,096 x 14,336 by 8 rows 14.5 us, 6,144 x 4,096 by 64 10.2; so
+//   13.3 and 9.0), warp 1 the instructions, warps 2-9 the epilogue, under the next tile's steps up to 128 tokens
 __host__ __device__ inline int first_step(int b, int blocks, int steps) { return (int)((long)b * steps / blocks); }
 __device__ __forceinline__ int block_of_step(int step, int blocks, int steps) { return (int)((((long)step + 1) * blocks - 1) / steps); }
 
-__global__ void __launch_bounds__(THREADS, 2) e4m3_rows_kernel(const __grid_constant__ CUtensorMap map_x,
+__global__ void __launch_bounds__(ROWS_THREADS, 2) e4m3_rows_kernel(const __grid_constant__ CUtensorMap map_x,
                                                                const __grid_constant__ CUtensorMap map_w, Epilogue ep, int M,
                                                                int tiles, int k_steps, int* __restrict__ error_flag) {
   extern __shared__ unsigned char smem_unaligned[];
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, 2) e4m3_rows_kernel(const __grid_cons
   if (threadIdx.x == 0) {
     failed_flag = 0;
     for (int s = 0; s < MAX_STAGES; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 2);
       mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -316,28 +317,29 @@ __global__ void __launch_bounds__(THREADS, 2) e4m3_rows_kernel(const __grid_cons
   pdl_launch_dependents();  // now: a block of the next kernel must not take the tensor memory that this one still needs
 
   if (warp == 0) {
-    if (elect_one()) {
-      auto load_w = [&](int s, int tile, int k) {
+    if (elect_one()) {  // the weights, which do not depend on the kernel before
+      int tile = lo / k_steps, k = lo - tile * k_steps, s = 0;
+      uint32_t phase = 1;
+      for (int i = lo; i < hi; ++i) {
+        if (!quick_wait(&empty[s], phase, failed)) break;
         unsigned char* to = smem + s * stage_bytes;
-        mbar_arrive_expect_tx(&full[s], stage_bytes);
+        mbar_arrive_expect_tx(&full[s], BOX_BYTES);
         tma_load_2d(to, &map_w, k * TILE_K, tile * row_step, &full[s]);
         if (ep.glu) tma_load_2d(to + BOX_BYTES / 2, &map_w, k * TILE_K, ep.outputs + tile * row_step, &full[s]);
-      };
-      int tile = lo / k_steps, k = lo - tile * k_steps, s = 0;
-      const int early = min(stages, hi - lo);
-      for (int i = 0, t = tile, kk = k; i < early; ++i) {
-        load_w(i, t, kk);
-        if (++kk == k_steps) kk = 0, ++t;
-      }
-      pdl_wait();  // x is what the kernel before wrote
-      uint32_t phase = 1;
-      for (int i = lo; i < hi && !*failed; ++i) {
-        if (i - lo >= early) {
-          if (!wait_or_abort(&empty[s], phase, failed)) break;
-          load_w(s, tile, k);
-        }
-        tma_load_2d(smem + s * stage_bytes + BOX_BYTES, &map_x, k * TILE_K, 0, &full[s]);
         if (++k == k_steps) k = 0, ++tile;
+        if (++s == stages) s = 0, phase ^= 1;
+      }
+    }
+  } else if (warp == 2 + EPILOGUE_WARPS) {
+    if (elect_one()) {
+      pdl_wait();  // x is what the kernel before wrote
+      int k = lo % k_steps, s = 0;
+      uint32_t phase = 1;
+      for (int i = lo; i < hi; ++i) {
+        if (!quick_wait(&empty[s], phase, failed)) break;
+        mbar_arrive_expect_tx(&full[s], stage_bytes - BOX_BYTES);
+        tma_load_2d(smem + s * stage_bytes + BOX_BYTES, &map_x, k * TILE_K, 0, &full[s]);
+        if (++k == k_steps) k = 0;
         if (++s == stages) s = 0, phase ^= 1;
       }
     }
@@ -584,7 +586,7 @@ int launch(const void* x, const void* w, Epilogue ep, int M, int N, long pitch, 
     const size_t ring = ep.n_tokens <= 128 && c.slots == 0 && c.blocks > multiprocessors() ? PAIR_RING / 2 : PAIR_RING;
     ep.stages = min((int)(ring / (BOX_BYTES + ep.n_tokens * TILE_K)), MAX_STAGES);
     if (make_byte_map(&map_x, x, M, pitch, ep.n_tokens) || make_byte_map(&map_w, w, N, pitch, ep.glu ? TILE / 2 : TILE)) return 1;
-    fms_launch(e4m3_rows_kernel, dim3(c.blocks), dim3(THREADS), ring + EXTRA, stream, map_x, map_w, ep, M, c.tiles, c.k_steps, error_flag);
+    fms_launch(e4m3_rows_kernel, dim3(c.blocks), dim3(ROWS_THREADS), ring + EXTRA, stream, map_x, map_w, ep, M, c.tiles, c.k_steps, error_flag);
     if (fms_launch_status("gemm_e4m3")) return 1;
     if (c.slots == 0) return 0;
     const int each = ep.glu ? 8 : 4;
