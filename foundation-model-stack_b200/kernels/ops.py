@@ -19,6 +19,8 @@ The gated feed-forward product of 9 to 128 rows takes a tcgen05 kernel of this l
 instruction's rows and the activation in its epilogue (``gemm_bf16_mid.cu``); the same kernel can take the plain
 products and the fused projection up to 256 rows (clusters of blocks share a tile along K; projection + rotation
 + cache write in its epilogue; ``FMS_B200_MID_OPS``), where the library's product is still ahead of it.
+Weights of 8 and 4 bits (``E4M3Weight``, ``Int4Weight``) go through this library's own products for any number of rows
+(``gemm_e4m3.cu``, ``gemm_int4.cu``; kernels/quantized.py).
 """
 from __future__ import annotations
 
