@@ -296,6 +296,10 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) e4m3_rows_kernel(const __grid
   const int all = tiles * k_steps, row_step = ep.glu ? TILE / 2 : TILE;
   const int lo = first_step(blockIdx.x, gridDim.x, all), hi = first_step(blockIdx.x + 1, gridDim.x, all);
   const int accs = ep.n_tokens <= 128 ? 2 : 1;
+  // a block of one whole tile, beside which others fit, takes no more tensor memory than it needs
+  uint32_t tmem_cols = 32;
+  while ((int)tmem_cols < ep.n_tokens) tmem_cols *= 2;
+  if (ep.slots) tmem_cols = 256;
 
   if (threadIdx.x == 0) {
     failed_flag = 0;
@@ -309,7 +313,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) e4m3_rows_kernel(const __grid
     }
     mbar_fence_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 256);
+  if (warp == 1) tmem_alloc(tmem_slot, tmem_cols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -434,7 +438,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) e4m3_rows_kernel(const __grid
   if (threadIdx.x == 0 && *failed && error_flag) atomicExch(error_flag, 4);
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, tmem_cols);
   }
 }
 
