@@ -422,6 +422,28 @@ def test_layers_of_long_prompts_back_to_back(ops, kind):
     assert bool(torch.isfinite(first).all()) and torch.equal(again, first)
 
 
+def test_calls_on_two_streams_at_once(ops):
+    g = gen(8)
+    e4m3, int4 = ops.quantize_e4m3(normal(g, 6144, 2576, std=0.02)), ops.quantize_int4(normal(g, 6144, 2576, std=0.02))
+    xs = [normal(g, rows, 2576).to(BF16) for rows in (1, 8, 40, 200, 700)]
+
+    def run():
+        return [f for x in xs for f in (ops.linear_e4m3(x, e4m3), ops.gated_linear_e4m3(x, e4m3, None, 1), ops.linear_int4(x, int4),
+                                        ops.gated_linear_int4(x, int4, None, 1))]
+
+    want = run()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None, None]
+    for _ in range(10):
+        for i, stream in enumerate(streams):  # the one's launches run beside the other's
+            with torch.cuda.stream(stream):
+                got[i] = run()
+    torch.cuda.synchronize()
+    for ys in got:
+        for y, w in zip(ys, want):
+            assert torch.equal(y, w)
+
+
 def test_weights_straight_after_what_makes_them(ops):
     """A product asks for its weights before the kernel in front of it is done; the weight's constructor has waited for them."""
     g = gen(9)
