@@ -160,10 +160,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     mbar_fence_init();
   }
+  __syncthreads();
+  cluster_sync_all();  // the partner runs, and its barriers exist
   if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();  // the partner's barriers exist before anything is sent to them
+  cluster_sync_all();  // and it has its tensor memory
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 

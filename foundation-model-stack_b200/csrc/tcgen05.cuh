@@ -139,7 +139,9 @@ __device__ __forceinline__ void cluster_sync_all() {
   __syncwarp();  // a warp arrives as one
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
-// by the same warp of both blocks, with the same address for the result
+// By the same warp of both blocks, with the same address for the result.  The two blocks take their columns together, so each must
+// know that the other runs: after cluster_sync_all().  (A pair that was launched while the kernel before it drained, and asked ahead
+// of that barrier, once never got its columns.)
 __device__ __forceinline__ void tmem_alloc_pair(void* smem_result, uint32_t columns) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(smem_result)), "r"(columns)
                : "memory");
