@@ -74,7 +74,6 @@ __global__ void __launch_bounds__(FT_THREADS, 1) attn_prefill_f32_tc_kernel(Attn
   __shared__ float top[2][128], sums[2][128];
   volatile int* failed = &failed_flag;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, half = warp >> 2, row = (warp & 3) * 32 + lane;
-  pdl_launch_dependents();
   if (tid == 0) {
     failed_flag = 0;
     mbar_init(&done_s, 1);
@@ -85,6 +84,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) attn_prefill_f32_tc_kernel(Attn
   if (tid < 4) odd_keys[tid >> 1][tid & 1] = 0;
   if (warp == 0) tmem_alloc(&tmem_slot, 512);
   __syncthreads();
+  pdl_launch_dependents();  // a block of the next kernel must not take the tensor memory that this one still needs
   pdl_wait();
   const int pairs = a.nheads / 2, pair = blockIdx.x % pairs, tile = n_tiles - 1 - blockIdx.x / pairs;  // the longest tiles first
   const int seq = FMS_IN(tiles[2 * tile], n_seqs) ? tiles[2 * tile] : 0, r0 = tiles[2 * tile + 1];

@@ -79,7 +79,6 @@ __global__ void __launch_bounds__(192, 2) attn_prefill_tc_kernel(const __grid_co
   __shared__ float distance_table[DISTANCE ? 4 : 1][DISTANCE ? TC_DIST_FLOATS : 1];
   __shared__ float2 distance_factors[DISTANCE ? TC_DIST_HEADS : 1];
   volatile int* failed = &failed_flag;
-  pdl_launch_dependents();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.nheads / a.kvheads;
@@ -125,6 +124,7 @@ __global__ void __launch_bounds__(192, 2) attn_prefill_tc_kernel(const __grid_co
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t tmem_o = tmem, tmem_s = tmem + HD;  // S buffer b at tmem_s + 64 b
+  pdl_launch_dependents();  // a block of the next kernel must not take the tensor memory that this one still needs
   pdl_wait();
 
   if (warp == 0) {

@@ -120,8 +120,9 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 // ---- programmatic dependent launch ------------------------------------------------------------------
 // Kernels of a step are launched so that a kernel may start while the one before it is still draining.
 // Every kernel calls pdl_launch_dependents() early (the next kernel may be scheduled once all blocks of this
-// one have done so) and pdl_wait() before it reads what an earlier kernel wrote or writes anything at all;
-// only loads of constant data (weights) may come before pdl_wait().
+// one have done so; one that takes tensor memory does it when it has it, see tmem_alloc) and pdl_wait() before it
+// reads what an earlier kernel wrote or writes anything at all; only loads of constant data (weights) may come before
+// pdl_wait().
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 

@@ -104,7 +104,6 @@ __global__ void __launch_bounds__(THREADS) gemm_mid_kernel(const __grid_constant
   __shared__ int failed_flag;
   volatile int* failed = &failed_flag;
 
-  pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ks = p.ks, rank = ks > 1 ? (int)cluster_rank() : 0;
   const int tile = blockIdx.y;
@@ -131,6 +130,7 @@ __global__ void __launch_bounds__(THREADS) gemm_mid_kernel(const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();  // a block of the next kernel must not take the tensor memory that this one still needs
 
   if (warp == 0) {
     if (elect_one()) {

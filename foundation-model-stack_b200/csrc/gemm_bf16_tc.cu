@@ -207,7 +207,6 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_tc_kernel(const __grid_consta
   __shared__ int failed_flag;
   volatile int* failed = &failed_flag;
 
-  pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile_n = ep.glu ? ep.tile_n / 2 : ep.tile_n;  // output columns of a tile
   const int tiles_m = (M + TILE_M - 1) / TILE_M, tiles_n = (N + tile_n - 1) / tile_n;
@@ -231,6 +230,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_tc_kernel(const __grid_consta
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();  // a block of the next kernel must not take the tensor memory that this one still needs
   // everything above (barriers, tensor memory) overlaps the end of the kernel before; x may be read only now
   pdl_wait();
 
@@ -324,7 +324,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   __shared__ int failed_flag;
   volatile int* failed = &failed_flag;
 
-  pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
@@ -354,6 +353,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   cluster_sync_all();  // and it has its tensor memory
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();  // a block of the next kernel must not take the tensor memory that this one still needs
   pdl_wait();
 
   if (warp == 0) {

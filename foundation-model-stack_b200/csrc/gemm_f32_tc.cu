@@ -206,7 +206,6 @@ __global__ void __launch_bounds__(S::THREADS, 1) gemm_f32_split_kernel(const Pro
   const int k_begin = alone ? 0 : min(rank * p.run_len, p.K), k_end = alone ? p.K : min(k_begin + p.run_len, p.K);
   const int steps = (k_end - k_begin + S::STEP - 1) / S::STEP;
 
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     failed_flag = 0;
     whole_any = 0;
@@ -225,6 +224,7 @@ __global__ void __launch_bounds__(S::THREADS, 1) gemm_f32_split_kernel(const Pro
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  pdl_launch_dependents();  // a block of the next kernel must not take the tensor memory that this one still needs
 
   if (warp >= S::CONV_AT) {
     if constexpr (S::CONV_REGS > 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(S::CONV_REGS > 0 ? S::CONV_REGS : 24));

@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot, tmem_a = tmem + a.accs * a.issuers * a.acc_columns;
-  pdl_launch_dependents();  // now: a block of the next kernel must not take the tensor memory that this one still needs
+  pdl_launch_dependents();  // a block of the next kernel must not take the tensor memory that this one still needs
 
   if (warp == 0) {
     if (elect_one()) {  // the weights, which do not depend on the kernel before

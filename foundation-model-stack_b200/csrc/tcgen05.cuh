@@ -16,6 +16,10 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
                "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
                : "memory");
 }
+// The instruction waits for as long as it takes, without a limit.  That ends: a block asks once, for all that it needs, and lets the
+// next kernel of its stream in (pdl_launch_dependents) only behind the barrier after it.  So whoever holds tensor memory and
+// waits for an earlier kernel waits for one whose blocks all have theirs, and those of other streams end by themselves.  Blocks of a
+// cluster, which wait for one another, take so much shared memory that whatever fits beside them finds columns too.
 __device__ __forceinline__ void tmem_alloc(void* smem_result, uint32_t columns) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(smem_result)), "r"(columns)
                : "memory");

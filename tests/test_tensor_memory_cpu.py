@@ -46,3 +46,12 @@ def test_a_pair_takes_its_tensor_memory_when_both_blocks_run(body):
         at = body.index("tmem_alloc_pair(")
         assert "cluster_sync_all();" in body[:at]
         assert body[at:].index("cluster_sync_all();") < body[at:].index("elect_one()")  # and nothing is issued before both have theirs
+
+
+@pytest.mark.parametrize("body", KERNELS)
+def test_the_next_kernel_is_let_in_when_a_block_has_its_tensor_memory(body):
+    """A block of the next kernel takes tensor memory and waits for this kernel: had it come in earlier, it could hold what a block of
+    this kernel still waits for."""
+    if "pdl_launch_dependents" in body:
+        taken = body.rindex("tmem_alloc")
+        assert body.index("pdl_launch_dependents") > taken + body[taken:].index("__syncthreads();")
