@@ -58,6 +58,7 @@ __device__ __forceinline__ void scale4(float* v, float sx, const float* scales, 
 }
 // twice 16 columns of this thread's row (lane) of tensor memory: both loads are in flight before the one wait
 __device__ __forceinline__ void tmem_load_2x16(uint32_t taddr_a, uint32_t taddr_b, float* va, float* vb) {
+  __syncwarp();
   uint32_t r[32];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n"

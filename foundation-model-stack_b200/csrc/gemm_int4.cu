@@ -291,6 +291,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 }
 // 32 columns of 32 bits of this thread's lane of tensor memory, written; not waited for
 __device__ __forceinline__ void tmem_store_pairs(uint32_t taddr, const uint32_t* r) {
+  __syncwarp();
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
       "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(taddr),
@@ -300,7 +301,10 @@ __device__ __forceinline__ void tmem_store_pairs(uint32_t taddr, const uint32_t*
       "r"(r[31])
       : "memory");
 }
-__device__ __forceinline__ void tmem_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_stores() {
+  __syncwarp();
+  asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+}
 // 64 k of a row as 32 columns: words 2 h and 2 h + 1 of its four pieces, with the groups' words of either
 __device__ __forceinline__ void unpack64(const uint2* words, uint32_t group0, uint32_t group1, uint32_t* col) {
 #pragma unroll

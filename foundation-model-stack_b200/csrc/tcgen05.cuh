@@ -1,6 +1,8 @@
 // Helpers for the fifth-generation tensor cores of sm_100a and for TMA: tensor-memory allocation, tcgen05.mma
 // with shared-memory matrix descriptors, commits to mbarriers, tcgen05.ld, tiled TMA loads and their tensor maps.
 // Included inside the anonymous namespace of the kernels that use them, after common.cuh and <cuda.h>.
+// Instructions of a whole warp (.aligned) have a __syncwarp() ahead of them: behind a part that some lanes ran alone, or left early,
+// the compiler need not bring the lanes together by itself.
 #pragma once
 
 __device__ __forceinline__ bool elect_one() {
@@ -21,11 +23,11 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
 // waits for an earlier kernel waits for one whose blocks all have theirs, and those of other streams end by themselves.  Blocks of a
 // cluster, which wait for one another, take so much shared memory that whatever fits beside them finds columns too.
 __device__ __forceinline__ void tmem_alloc(void* smem_result, uint32_t columns) {
+  __syncwarp();
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(smem_result)), "r"(columns)
                : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
 }
-// An instruction of a whole warp, which after a part that one lane ran alone comes together first.
 __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t columns) {
   __syncwarp();
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(columns) : "memory");
@@ -68,6 +70,7 @@ __device__ __forceinline__ void umma_a_tmem(uint32_t tmem_d, uint32_t tmem_a, ui
 }
 // 32 consecutive float32 columns of this thread's row (lane) of tensor memory
 __device__ __forceinline__ void tmem_load_32(uint32_t taddr, float* v) {
+  __syncwarp();
   uint32_t r[32];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
@@ -84,6 +87,7 @@ __device__ __forceinline__ void tmem_load_32(uint32_t taddr, float* v) {
 
 // 16 consecutive float32 columns of this thread's row (lane) of tensor memory
 __device__ __forceinline__ void tmem_load_16(uint32_t taddr, float* v) {
+  __syncwarp();
   uint32_t r[16];
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
@@ -94,6 +98,7 @@ __device__ __forceinline__ void tmem_load_16(uint32_t taddr, float* v) {
 }
 // twice 32 columns: both loads are in flight before the one wait
 __device__ __forceinline__ void tmem_load_2x32(uint32_t taddr_a, uint32_t taddr_b, float* va, float* vb) {
+  __syncwarp();
   uint32_t r[64];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n"
@@ -140,13 +145,14 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 }
 // every thread of both blocks; a hardware barrier, not a spin
 __device__ __forceinline__ void cluster_sync_all() {
-  __syncwarp();  // a warp arrives as one
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 // By the same warp of both blocks, with the same address for the result.  The two blocks take their columns together, so each must
 // know that the other runs: after cluster_sync_all().  (A pair that was launched while the kernel before it drained, and asked ahead
 // of that barrier, once never got its columns.)
 __device__ __forceinline__ void tmem_alloc_pair(void* smem_result, uint32_t columns) {
+  __syncwarp();
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(smem_result)), "r"(columns)
                : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
@@ -226,6 +232,7 @@ int make_map(CUtensorMap* map, const void* base, long rows, int K, int box_rows 
 
 // 32 consecutive float32 columns of this thread's row (lane) of tensor memory, written
 __device__ __forceinline__ void tmem_store_32(uint32_t taddr, const float* v) {
+  __syncwarp();
   uint32_t r[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);

@@ -55,3 +55,19 @@ def test_the_next_kernel_is_let_in_when_a_block_has_its_tensor_memory(body):
     if "pdl_launch_dependents" in body:
         taken = body.rindex("tmem_alloc")
         assert body.index("pdl_launch_dependents") > taken + body[taken:].index("__syncthreads();")
+
+
+def test_a_warp_comes_together_before_an_instruction_of_all_of_it():
+    """tcgen05 instructions and cluster barriers that are .aligned are reached by all lanes at once: behind a loop that some lanes go
+    around early the compiler need not see to that."""
+    seen = 0
+    for name in sorted(os.listdir(CSRC)):
+        if not name.endswith((".cu", ".cuh")):
+            continue
+        with open(os.path.join(CSRC, name)) as f:
+            text = without_comments(f.read())
+        for found in re.finditer(r"(tcgen05|barrier\.cluster)[\w.:]*\.aligned", text):
+            function = text[text.rindex("__forceinline__", 0, found.start()): found.start()]
+            assert "__syncwarp();" in function, (name, found.group(0))
+            seen += 1
+    assert seen >= 18
