@@ -795,19 +795,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
   }
 }
 
+// Tokens of a pair's tile: the width whose tiles cost least in whole rounds of the pairs; below some 100 tokens a step takes what
+// unpacking takes.  A multiple of 32, which the instruction's shapes for a pair with A in tensor memory are.
+int pair_tokens(int M, int N) {
+  const int pairs = max(multiprocessors() / 2, 1), tiles_n = (N + 2 * TILE - 1) / (2 * TILE);
+  long best = -1;
+  int tokens = PAIR_TOKENS;
+  for (int tn = PAIR_TOKENS; tn >= 96; tn -= 32) {
+    const long tiles = (long)tiles_n * ((M + tn - 1) / tn), cost = (tiles + pairs - 1) / pairs * (max(tn, 100) + 24);
+    if (best < 0 || cost < best) {
+      best = cost;
+      tokens = tn;
+    }
+  }
+  return tokens;
+}
+
 int launch_pair(const Int4Args& p, int* error_flag, cudaStream_t stream) {
   RowsArgs a = {};
   a.p = p;
-  // the width whose tiles cost least in whole rounds of the pairs; below some 100 tokens a step takes what unpacking takes
   const int pairs = max(multiprocessors() / 2, 1), tiles_n = (p.N + 2 * TILE - 1) / (2 * TILE);
-  long best = -1;
-  for (int tn = PAIR_TOKENS; tn >= 64; tn -= 16) {
-    const long tiles = (long)tiles_n * ((p.M + tn - 1) / tn), cost = (tiles + pairs - 1) / pairs * (max(tn, 100) + 24);
-    if (best < 0 || cost < best) {
-      best = cost;
-      a.n_tokens = tn;
-    }
-  }
+  a.n_tokens = pair_tokens(p.M, p.N);
   const long tiles = (long)tiles_n * ((p.M + a.n_tokens - 1) / a.n_tokens);
   if (tiles > 0x7fffffffL) return fms_fail("gemm_int4: %ld tiles", tiles);
   const int stage_bytes = (a.n_tokens * BLOCK_K + TILE / BLOCK_ROWS * p.block_bytes() + 1023) / 1024 * 1024;
@@ -831,6 +839,9 @@ int check(const Int4Args& p) {
   return 0;
 }
 }  // namespace
+
+// Rows of x that a tile of fms_linear_int4 has where its pairs of thread blocks take M of them; 0: another kernel does.
+FMS_API int fms_linear_int4_tile(int M, int N) { return M <= FEW_ROWS || N <= 0 || M <= rows_most(N) ? 0 : pair_tokens(M, N); }
 
 // Floats of scratch memory that fms_linear_int4 wants.
 FMS_API long fms_linear_int4_scratch(long M, long N, long K) { return M <= FEW_ROWS || N <= 0 || K <= 0 || M > rows_most(N) ? 0 : rows_scratch(M, N, K); }

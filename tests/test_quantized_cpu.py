@@ -151,3 +151,17 @@ def test_the_plain_rounding_to_four_bits_is_the_same():
     w = (torch.randn(37, 200, generator=gen(4)) * 0.02).to(BF16)
     for group in (32, 64, 128, 256):
         assert torch.equal(ops.quantize_int4(w, group).dequantize().double(), pq.int4_of(w, group))
+
+
+# ---- how a product is cut ------------------------------------------------------------------------------------------------
+PAIR_SHAPES = [(300, 6144), (512, 6144), (512, 28672), (700, 6144), (1024, 28672), (2048, 4096), (2048, 6144), (4096, 4096), (257, 264), (113, 40000), (8192, 128256)]
+
+
+@pytest.mark.parametrize("m,n", PAIR_SHAPES)
+def test_pairs_of_blocks_take_rows_by_32(m, n):
+    """The instruction of a pair of thread blocks whose weights lie in tensor memory exists for 32, 64, ... 256 columns."""
+    from fms_b200.kernels.build import load_library
+
+    tile = load_library("gemm_int4").fms_linear_int4_tile
+    assert tile(m, n) in range(32, 257, 32)
+    assert tile(8, n) == tile(112, n) == 0

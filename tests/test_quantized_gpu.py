@@ -7,6 +7,8 @@ round, which is at most twice that).  Whole numbers whose sums stay below 2^24 a
 import pytest
 import torch
 
+from fms_b200.kernels.build import load_library
+
 pytestmark = pytest.mark.gpu
 
 BF16, F32 = torch.bfloat16, torch.float32
@@ -263,6 +265,22 @@ def test_linear_int4_whole_numbers_are_exact(ops, m, n, k, group, zeros):
     assert torch.equal(w.dequantize().double(), centred * scales.double()[:, at])
     want = x.double() @ (centred * scales.double()[:, at]).t()
     assert torch.equal(ops.linear_int4(x.to(BF16), w), want.float().to(BF16))  # exact in float32, rounded once
+
+
+# with the rows of x that a pair's tile has on 148 multiprocessors
+PAIR_TILES = [(270, 616, 136, 128, 96), (300, 6144, 136, 64, 128), (307, 4840, 392, 32, 128), (520, 4840, 136, 128, 192), (307, 6248, 136, 128, 160),
+              (407, 6248, 264, 64, 224), (700, 6144, 136, 128, 256), (720, 4840, 264, 256, 256)]
+
+
+@pytest.mark.parametrize("m,n,k,group,tile", PAIR_TILES)
+def test_linear_int4_of_tiles_of_every_width(ops, m, n, k, group, tile):
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert load_library("gemm_int4").fms_linear_int4_tile(m, n) == tile
+    g, q, z, centred, groups, at = int4_case(m, n, k, group, True, m + n + k)
+    scales = 2.0 ** whole(g, -2, 2, n, groups).float()
+    x = whole(g, -1, 1, m, k).float() * 2.0 ** whole(g, 0, 1, m, 1).float()
+    want = x.double() @ (centred * scales.double()[:, at]).t()
+    assert torch.equal(ops.linear_int4(x.to(BF16), ops.pack_int4(q, scales, z, group)), want.float().to(BF16))
 
 
 @pytest.mark.parametrize("biased", [False, True])
