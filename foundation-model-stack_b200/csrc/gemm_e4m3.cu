@@ -454,11 +454,12 @@ __global__ void __launch_bounds__(TILE) e4m3_join_kernel(Epilogue ep, int M, int
   const int row = (int)threadIdx.x & (row_step - 1), col = tile * row_step + row;
   const int t0 = (blockIdx.y * (TILE / row_step) + (int)threadIdx.x / row_step) * 4;
   if ((!ep.glu && from == to) || col >= ep.outputs || t0 >= M) return;  // some block of some tile goes on, and waits
-  const float sw = ep.sw[col], bias = ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;
   // only the first block of a tile can have begun with an earlier one
   const int head = tile - first_step(from, blocks, all) / k_steps;
   const size_t pitch = (size_t)ep.n_tokens * TILE;
+  const float sw = ep.sw[col];  // of the weight
   pdl_wait();
+  const float bias = ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;  // any tensor: the kernel before the product may have written it
   float sx[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) sx[j] = t0 + j < M ? ep.sx[t0 + j] : 0.f;

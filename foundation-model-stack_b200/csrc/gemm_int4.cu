@@ -571,12 +571,12 @@ __global__ void __launch_bounds__(TILE) int4_join_kernel(RowsArgs a, int blocks)
   const int from = block_of_step(start, blocks, all), to = block_of_step(start + p.k_blocks - 1, blocks, all);
   const int col = tile * TILE + (int)threadIdx.x, t0 = blockIdx.y * 4;
   if (from == to || col >= p.N || t0 >= p.M) return;  // some block of some tile goes on, and waits
-  const float bias = p.bias ? __bfloat162float(p.bias[col]) : 0.f;
   // only the first block of a tile can have begun with an earlier one
   const int head = first_step(from, blocks, all) / p.k_blocks == tile ? 0 : 1;
   const float* slots = a.scratch + (size_t)t0 * TILE + threadIdx.x;
   const size_t pitch = (size_t)a.n_tokens * TILE;
   pdl_wait();
+  const float bias = p.bias ? __bfloat162float(p.bias[col]) : 0.f;  // any tensor: the kernel before the product may have written it
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   for (int b = from; b <= to; b += 4) {
     float v[4][4];

@@ -165,3 +165,19 @@ def test_pairs_of_blocks_take_rows_by_32(m, n):
     tile = load_library("gemm_int4").fms_linear_int4_tile
     assert tile(m, n) in range(32, 257, 32)
     assert tile(8, n) == tile(112, n) == 0
+
+
+@pytest.mark.parametrize("file,kernel", [("gemm_e4m3.cu", "e4m3_join_kernel"), ("gemm_int4.cu", "int4_join_kernel"), ("gemm_int4.cu", "int4_few_rows_kernel"),
+                                         ("quantize_rows.cu", "quantize_rows_kernel")])
+def test_only_weights_are_read_before_the_kernel_in_front_is_done(file, kernel):
+    """A kernel starts while the one in front of it still runs, and may read a bias, scales or rows behind griddepcontrol.wait only."""
+    import os
+    import re
+
+    from fms_b200.kernels.build import CSRC
+
+    with open(os.path.join(CSRC, file)) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    body = text[re.search(rf"{kernel}\(", text).start():]
+    ahead = body[: body.index("pdl_wait();")]
+    assert not re.search(r"bias\[|sx\[|slots\[|rows\[|__ldg|load_gain\(\)|load_run<", ahead), ahead[-600:]
