@@ -245,21 +245,11 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2
   Run<float> x[KEPT];
   Run<TG> g[KEPT];
   pdl_launch_dependents();
-  int shift = 0;
-  auto load_gain = [&]() {
-#pragma unroll
-    for (int j = 0; j < KEPT; ++j)
-      if (RUNS > 0) load_run<NEIGHBOURS>(g[j], gain, j, shift, dim);
-  };
-  if (NEIGHBOURS) load_gain();  // a weight: it can be read before the kernel before this one is done
-  pdl_wait();
+  pdl_wait();  // any of the tensors, the gain among them, may be what the kernel before writes
   const int src = rows ? rows[blockIdx.x] : blockIdx.x;
   if (!FMS_IN(src, residual_rows)) return;  // the whole block alike
   float* res = residual + (size_t)src * dim;
-  if (!NEIGHBOURS) {
-    shift = shift_of(res);
-    load_gain();
-  }
+  const int shift = NEIGHBOURS ? 0 : shift_of(res);
   const T* del = delta ? delta + (size_t)src * dim : nullptr;
   const bool writes = del && rows == nullptr;
   auto add = [&](Run<float>& v, const Run<T>& d) {
@@ -270,6 +260,8 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2
     Run<T> d[KEPT];
 #pragma unroll
     for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(x[j], res, j, shift, dim);
+#pragma unroll
+    for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(g[j], gain, j, shift, dim);
     if (del) {
 #pragma unroll
       for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(d[j], del, j, shift, dim);

@@ -168,7 +168,7 @@ def test_pairs_of_blocks_take_rows_by_32(m, n):
 
 
 @pytest.mark.parametrize("file,kernel", [("gemm_e4m3.cu", "e4m3_join_kernel"), ("gemm_int4.cu", "int4_join_kernel"), ("gemm_int4.cu", "int4_few_rows_kernel"),
-                                         ("quantize_rows.cu", "quantize_rows_kernel")])
+                                         ("quantize_rows.cu", "quantize_rows_kernel"), ("quantize_rows.cu", "add_rmsnorm_quantized_kernel")])
 def test_only_weights_are_read_before_the_kernel_in_front_is_done(file, kernel):
     """A kernel starts while the one in front of it still runs, and may read a bias, scales or rows behind griddepcontrol.wait only."""
     import os

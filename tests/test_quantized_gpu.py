@@ -548,3 +548,17 @@ def test_a_bias_that_the_kernel_before_writes(ops, kind, m):
         return ops.gated_linear(rows, w, bias[0], 0) if "gated" in kind else ops.linear(rows, w, bias[0], BF16)
 
     behind(lambda held: ops.linear(held, wide), use, inputs)
+
+
+@pytest.mark.parametrize("rows,dim", [(8, 4096), (300, 4096), (5, 1001)])
+def test_a_gain_that_the_kernel_before_writes(ops, rows, dim):
+    g = gen(rows)
+    wide, res, delta = normal(g, dim, 16384, std=0.01).to(BF16), normal(g, rows, dim), normal(g, rows, dim).to(BF16)
+    inputs = [normal(g, 1, 16384, std=2.0 ** i).to(BF16) for i in range(4)]
+    picked = torch.arange(rows, dtype=torch.int32, device="cuda")
+
+    def use(gain):
+        y = ops.add_rmsnorm_quantized(res, delta, gain[0], 1e-5, picked)  # of gathered rows: the stream stays as it is
+        return torch.cat((y.values.view(torch.uint8).flatten(), y.scales.view(torch.uint8)))
+
+    behind(lambda held: ops.linear(held, wide), use, inputs)
