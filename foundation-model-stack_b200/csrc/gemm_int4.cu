@@ -167,10 +167,10 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 1) int4_few_rows_kernel(Int4Ar
       uint4 b[4];
       if (left >= BLOCK_K) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) b[v] = __ldg(xs + 4 * v);
+        for (int v = 0; v < 4; ++v) b[v] = xs[4 * v];
       } else {  // K is a multiple of 8: a lane's 8 values are all inside or all outside
 #pragma unroll
-        for (int v = 0; v < 4; ++v) b[v] = left > 32 * v + 8 * c ? __ldg(xs + 4 * v) : make_uint4(0, 0, 0, 0);
+        for (int v = 0; v < 4; ++v) b[v] = left > 32 * v + 8 * c ? xs[4 * v] : make_uint4(0, 0, 0, 0);
       }
       const uint32_t wl[4] = {wq[0].x, wq[0].y, wq[0].z, wq[0].w}, wh[4] = {wq[1].x, wq[1].y, wq[1].z, wq[1].w};
 #pragma unroll

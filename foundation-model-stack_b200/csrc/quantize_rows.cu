@@ -191,12 +191,15 @@ __device__ __forceinline__ float largest(const Run<__nv_bfloat16>& r) {
   return max_nan(__low2float(m), __high2float(m));
 }
 
+// No pointer of these kernels is __restrict__: what the kernel in front wrote must come through the coherent path, not through the one
+// for data that nobody writes while a kernel runs, which this one may begin to do before that one is done.
+
 // RUNS: runs of 8 values that a thread keeps; 0: any width, the row is read a second time.
 // What bounds many rows is how many of their bytes are on the way, so registers are kept few: three thread blocks of 448 for rows of
 // 14,336 (2,048 of them, bfloat16: 17.9 us, 4.9 TB/s; with two blocks 20.8, with four 19.2 for the registers that spill).
 template <typename T, int RUNS, bool NEIGHBOURS>
 __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && RUNS == 4 && sizeof(T) == 2 ? 3 : (RUNS != 1 && RUNS != 8 ? 2 : 1))
-    quantize_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scales, int n_rows, int dim, int pitch) {
+    quantize_rows_kernel(const T* x, uint8_t* q, float* scales, int n_rows, int dim, int pitch) {
   __shared__ float scratch[32];
   pdl_launch_dependents();
   pdl_wait();
@@ -236,9 +239,8 @@ __device__ __forceinline__ Pair larger(Pair a, Pair b) { return b.hi > a.hi || (
 
 template <typename T, typename TG, int RUNS, bool NEIGHBOURS>
 __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2 ? 2 : 1)
-    add_rmsnorm_quantized_kernel(float* __restrict__ residual, const T* __restrict__ delta, const TG* __restrict__ gain, float eps,
-                                 uint8_t* __restrict__ q, float* __restrict__ scales, const int* __restrict__ rows, int dim, int pitch,
-                                 int residual_rows) {
+    add_rmsnorm_quantized_kernel(float* residual, const T* delta, const TG* gain, float eps, uint8_t* q, float* scales, const int* rows,
+                                 int dim, int pitch, int residual_rows) {
   __shared__ float scratch[3][32];
   constexpr int KEPT = RUNS > 0 ? RUNS : 1;
   const int runs = RUNS > 0 ? RUNS : (pitch / 8 + !NEIGHBOURS + blockDim.x - 1) / blockDim.x;

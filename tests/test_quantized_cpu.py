@@ -181,3 +181,17 @@ def test_only_weights_are_read_before_the_kernel_in_front_is_done(file, kernel):
     body = text[re.search(rf"{kernel}\(", text).start():]
     ahead = body[: body.index("pdl_wait();")]
     assert not re.search(r"bias\[|sx\[|slots\[|rows\[|__ldg|load_gain\(\)|load_run<", ahead), ahead[-600:]
+
+
+def test_rows_come_through_the_coherent_path():
+    """A kernel that starts while the one in front still writes its rows must not read them as data that nobody writes meanwhile."""
+    import os
+    import re
+
+    from fms_b200.kernels.build import CSRC
+
+    with open(os.path.join(CSRC, "quantize_rows.cu")) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    assert "__restrict__" not in text and "__ldg" not in text and "ld.global.nc" not in text
+    with open(os.path.join(CSRC, "gemm_int4.cu")) as f:
+        assert "__ldg" not in f.read()

@@ -562,3 +562,23 @@ def test_a_gain_that_the_kernel_before_writes(ops, rows, dim):
         return torch.cat((y.values.view(torch.uint8).flatten(), y.scales.view(torch.uint8)))
 
     behind(lambda held: ops.linear(held, wide), use, inputs)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 20, 300])
+@pytest.mark.parametrize("dim", [512, 520])
+def test_a_run_of_them_replayed_with_other_inputs(ops, rows, dim):
+    """Every buffer between the operators holds other values with every replay: none may be those of the replay before."""
+    g = gen(rows + dim)
+    w8, w4 = ops.quantize_e4m3(normal(g, dim, dim, std=0.05)), ops.quantize_int4(normal(g, dim, dim, std=0.05), 64)
+    b8, b4 = ops.quantize_e4m3(normal(g, 2 * dim, dim, std=0.05)), ops.quantize_int4(normal(g, 2 * dim, dim, std=0.05))
+    res, gain = normal(g, rows, dim), 1 + normal(g, dim, std=0.1)
+    inputs = [normal(g, rows, dim, std=2.0 ** (i % 3)).to(BF16) for i in range(6)]
+
+    def run(delta):
+        stream = res.clone()
+        a = ops.linear_int4(ops.linear_e4m3(ops.add_rmsnorm_quantized(stream, delta, gain, 1e-5), w8), w4)
+        b = ops.linear_e4m3(ops.quantize_rows(ops.gated_linear_int4(a, b4, None, 0)), w8)
+        c = ops.gated_linear_e4m3(ops.add_rmsnorm_quantized(stream, b, gain, 1e-5), b8, None, 0)
+        return torch.cat((ops.linear_int4(c, w4).float(), stream))
+
+    behind(lambda held: held * 1, run, inputs)
