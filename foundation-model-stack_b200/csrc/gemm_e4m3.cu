@@ -18,6 +18,7 @@ constexpr int BOX_BYTES = TILE * TILE_K;  // 128 rows of an operand for one step
 
 #include "tcgen05.cuh"
 #include "umma_issue.cuh"
+#include "quantized.cuh"
 
 // instruction descriptor of kind::f8f6f4: float32 accumulator, e4m3 a and b, both K-major; the shape M x N
 __host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
@@ -37,7 +38,7 @@ __device__ __forceinline__ float activate(float g, int act) {
 
 struct Epilogue {
   void* out;                  // [M, outputs] bfloat16 or float32 (GLU: bfloat16)
-  const __nv_bfloat16* bias;  // [N] or null
+  Bias bias;
   const float *sx, *sw;       // [M], [N]
   int out_f32, glu, act;
   int outputs;                // columns of y: N, or the hidden values of GLU (half of N)
@@ -224,7 +225,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int at = up ? i - 64 : i, c = (at >> 4) * 32 + half * 16 + (at & 15);
         const int col = min(n0 + c, ep.outputs - 1) + (up ? ep.outputs : 0);
         scales[i] = ep.sw[col];
-        if (ep.bias) biases[i] = __bfloat162float(ep.bias[col]);
+        if (ep.bias) biases[i] = ep.bias[col];
       }
       __syncwarp();
       if (!warp_wait(&acc_full[acc], (j >> 1) & 1, failed)) break;
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) e4m3_rows_kernel(const __grid
     for (int i = lo; i < hi; ++segment) {
       const int tile = i / k_steps, k_lo = i - tile * k_steps, k_hi = min(k_steps, hi - tile * k_steps), col = tile * TILE + row;
       const bool whole = !ep.glu && k_lo == 0 && k_hi == k_steps, live = whole && col < ep.outputs;
-      const float sw = live ? ep.sw[col] : 0.f, bias = live && ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;
+      const float sw = live ? ep.sw[col] : 0.f, bias = live && ep.bias ? ep.bias[col] : 0.f;
       float* slot = ep.scratch + ((size_t)(ep.slots * blockIdx.x + segment) * ep.n_tokens) * TILE + row;
       if (!warp_wait(&acc_full[acc], acc_phase, failed)) break;
       tc_fence_after();
@@ -420,8 +421,8 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) e4m3_rows_kernel(const __grid
       const int e = threadIdx.x - 64, r = e & 63, col = blockIdx.x * (TILE / 2) + r;
       if (col < ep.outputs && !*failed) {
         const float sw = ep.sw[col], su = ep.sw[ep.outputs + col];
-        const float bias = ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;
-        const float bias_up = ep.bias ? __bfloat162float(ep.bias[ep.outputs + col]) : 0.f;
+        const float bias = ep.bias ? ep.bias[col] : 0.f;
+        const float bias_up = ep.bias ? ep.bias[ep.outputs + col] : 0.f;
         for (int t = 4 * (e >> 6); t < ep.n_tokens; t += 16) {
           const float4 g = *reinterpret_cast<const float4*>(sums + r * sums_pitch + t);
           const float4 u = *reinterpret_cast<const float4*>(sums + (TILE / 2 + r) * sums_pitch + t);
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(TILE) e4m3_join_kernel(Epilogue ep, int M, int
   const size_t pitch = (size_t)ep.n_tokens * TILE;
   const float sw = ep.sw[col];  // of the weight
   pdl_wait();
-  const float bias = ep.bias ? __bfloat162float(ep.bias[col]) : 0.f;  // any tensor: the kernel before the product may have written it
+  const float bias = ep.bias ? ep.bias[col] : 0.f;  // any tensor: the kernel before the product may have written it
   float sx[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) sx[j] = t0 + j < M ? ep.sx[t0 + j] : 0.f;
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(TILE) e4m3_join_kernel(Epilogue ep, int M, int
 #pragma unroll
   for (int j = 0; j < 4; ++j) y[j] = fmaf(y[j], sx[j] * sw, bias);
   if (ep.glu) {
-    const float su = ep.sw[ep.outputs + col], bias_up = ep.bias ? __bfloat162float(ep.bias[ep.outputs + col]) : 0.f;
+    const float su = ep.sw[ep.outputs + col], bias_up = ep.bias ? ep.bias[ep.outputs + col] : 0.f;
     float up[4];
     total(TILE / 2 + row, up);
 #pragma unroll
@@ -624,35 +625,37 @@ FMS_API long fms_e4m3_scratch(long M, long N, long pitch, long glu) {
 }
 
 // y [M, N] (bfloat16, or float32 with out_dtype FMS_F32) of x [M, pitch] and w [N, pitch], e4m3, with sx [M], sw [N] float32 and
-// bias [N] bfloat16 or null.
-FMS_API int fms_linear_e4m3(const void* x, const float* sx, const void* w, const float* sw, const void* bias, void* y, int out_dtype,
+// bias [N] bfloat16 or float32, or null.
+FMS_API int fms_linear_e4m3(const void* x, const float* sx, const void* w, const float* sw, const void* bias, int bias_dtype, void* y, int out_dtype,
                             int M, int N, long pitch, float* scratch, long scratch_floats, int* error_flag, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
   if (out_dtype != FMS_F32 && out_dtype != FMS_BF16) return fms_fail("linear_e4m3: out dtype %d", out_dtype);
   Epilogue ep = {};
   ep.out = y;
-  ep.bias = (const __nv_bfloat16*)bias;
+  ep.bias = {bias, bias_dtype == FMS_F32};
   ep.sx = sx;
   ep.sw = sw;
   ep.out_f32 = out_dtype == FMS_F32;
   ep.outputs = N;
+  if (check_bias("linear_e4m3", ep.bias, bias_dtype)) return 1;
   ep.scratch = scratch;
   return launch(x, w, ep, M, N, pitch, scratch_floats, error_flag, stream);
 }
 
 // y [M, hidden] bfloat16 = act(gate) * up for w = [gate; up] of 2 hidden rows (sw and bias [2 hidden]).
-FMS_API int fms_glu_e4m3(const void* x, const float* sx, const void* w, const float* sw, const void* bias, void* y, int M, int hidden,
+FMS_API int fms_glu_e4m3(const void* x, const float* sx, const void* w, const float* sw, const void* bias, int bias_dtype, void* y, int M, int hidden,
                          long pitch, int act, float* scratch, long scratch_floats, int* error_flag, cudaStream_t stream) {
   if (M <= 0 || hidden <= 0) return 0;
   if (act < 0 || act > 3) return fms_fail("glu_e4m3: activation %d", act);
   Epilogue ep = {};
   ep.out = y;
-  ep.bias = (const __nv_bfloat16*)bias;
+  ep.bias = {bias, bias_dtype == FMS_F32};
   ep.sx = sx;
   ep.sw = sw;
   ep.glu = 1;
   ep.act = act;
   ep.outputs = hidden;
   ep.scratch = scratch;
+  if (check_bias("glu_e4m3", ep.bias, bias_dtype)) return 1;
   return launch(x, w, ep, M, 2 * hidden, pitch, scratch_floats, error_flag, stream);
 }

@@ -21,6 +21,7 @@
 namespace {
 #include "tcgen05.cuh"
 #include "umma_issue.cuh"
+#include "quantized.cuh"
 
 constexpr int BLOCK_ROWS = 16, BLOCK_K = 128, WEIGHT_BYTES = 1024;
 
@@ -56,7 +57,7 @@ __device__ __forceinline__ __nv_bfloat162 scale_of(uint32_t word) {
 struct Int4Args {
   const __nv_bfloat16* x;     // [M, K]
   const unsigned char* w;     // the packed blocks
-  const __nv_bfloat16* bias;  // [N] or null
+  Bias bias;
   __nv_bfloat16* y;           // [M, outputs]
   int M, N, K, k_blocks, per, outputs, act;
   __host__ __device__ int block_bytes() const { return WEIGHT_BYTES + 64 * per; }
@@ -227,10 +228,10 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 1) int4_few_rows_kernel(Int4Ar
         return sum;
       };
       float v = total(tile);
-      if (p.bias) v += __bfloat162float(p.bias[col]);
+      if (p.bias) v += p.bias[col];
       if (GLU) {
         float up = total(count + tile);
-        if (p.bias) up += __bfloat162float(p.bias[p.outputs + col]);
+        if (p.bias) up += p.bias[p.outputs + col];
         v = activate(v, p.act) * up;
       }
       if (FMS_IN((size_t)m * p.outputs + col, (size_t)p.M * p.outputs)) p.y[(size_t)m * p.outputs + col] = __float2bfloat16_rn(v);
@@ -522,7 +523,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid
       const int col = tile * TILE + row;
       const bool whole = k_lo == 0 && k_hi == p.k_blocks;
       float* slot = a.scratch + ((size_t)(2 * blockIdx.x + (i == lo ? 0 : 1)) * a.n_tokens) * TILE + row;
-      const float bias = whole && p.bias && col < p.N ? __bfloat162float(p.bias[col]) : 0.f;
+      const float bias = whole && p.bias && col < p.N ? p.bias[col] : 0.f;
       if (!warp_wait(&acc_full[acc], acc_phase, failed)) break;
       tc_fence_after();
       for (int c0 = 0; c0 < a.n_tokens; c0 += 16) {
@@ -576,7 +577,7 @@ __global__ void __launch_bounds__(TILE) int4_join_kernel(RowsArgs a, int blocks)
   const float* slots = a.scratch + (size_t)t0 * TILE + threadIdx.x;
   const size_t pitch = (size_t)a.n_tokens * TILE;
   pdl_wait();
-  const float bias = p.bias ? __bfloat162float(p.bias[col]) : 0.f;  // any tensor: the kernel before the product may have written it
+  const float bias = p.bias ? p.bias[col] : 0.f;  // any tensor: the kernel before the product may have written it
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   for (int b = from; b <= to; b += 4) {
     float v[4][4];
@@ -769,7 +770,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
     int j = 0;
     for (int tile = pair; tile < n_tiles; tile += pairs, ++j) {
       const int m0 = (tile % tiles_m) * a.n_tokens, col = ((tile / tiles_m) * 2 + (int)rank) * TILE + quarter * 32 + lane;
-      const float bias = p.bias && col < p.N ? __bfloat162float(p.bias[col]) : 0.f;
+      const float bias = p.bias && col < p.N ? p.bias[col] : 0.f;
       if (!warp_wait(acc_full, j & 1, failed)) break;
       tc_fence_after();
       for (int c0 = 16 * half; c0 < a.n_tokens; c0 += 32) {
@@ -846,25 +847,25 @@ FMS_API int fms_linear_int4_tile(int M, int N) { return M <= FEW_ROWS || N <= 0 
 // Floats of scratch memory that fms_linear_int4 wants.
 FMS_API long fms_linear_int4_scratch(long M, long N, long K) { return M <= FEW_ROWS || N <= 0 || K <= 0 || M > rows_most(N) ? 0 : rows_scratch(M, N, K); }
 
-// y [M, N] bfloat16 of x [M, K] bfloat16, w packed with `per` scales a block, bias [N] bfloat16 or null.
-FMS_API int fms_linear_int4(const void* x, const void* w, const void* bias, void* y, int M, int N, int K, int k_blocks, int per,
+// y [M, N] bfloat16 of x [M, K] bfloat16, w packed with `per` scales a block, bias [N] bfloat16 or float32, or null.
+FMS_API int fms_linear_int4(const void* x, const void* w, const void* bias, int bias_dtype, void* y, int M, int N, int K, int k_blocks, int per,
                             float* scratch, long scratch_floats, int* error_flag, cudaStream_t stream) {
   if (M <= 0 || N <= 0) return 0;
-  const Int4Args p = {(const __nv_bfloat16*)x, (const unsigned char*)w, (const __nv_bfloat16*)bias, (__nv_bfloat16*)y,
+  const Int4Args p = {(const __nv_bfloat16*)x, (const unsigned char*)w, {bias, bias_dtype == FMS_F32}, (__nv_bfloat16*)y,
                       M, N, K, k_blocks, per, N, 0};
-  if (check(p)) return 1;
+  if (check(p) || check_bias("gemm_int4", p.bias, bias_dtype)) return 1;
   return M <= FEW_ROWS ? few<false>(p, stream)
                        : (M <= rows_most(N) ? launch_rows(p, scratch, scratch_floats, error_flag, stream) : launch_pair(p, error_flag, stream));
 }
 
 // y [M, hidden] = act(gate) * up for w = [gate; up] of 2 hidden rows, hidden a multiple of 16, up to 8 rows of x.
-FMS_API int fms_glu_int4(const void* x, const void* w, const void* bias, void* y, int M, int hidden, int K, int k_blocks, int per,
+FMS_API int fms_glu_int4(const void* x, const void* w, const void* bias, int bias_dtype, void* y, int M, int hidden, int K, int k_blocks, int per,
                          int act, cudaStream_t stream) {
   if (M <= 0 || hidden <= 0) return 0;
   if (M > FEW_ROWS || hidden % BLOCK_ROWS || act < 0 || act > 3)
     return fms_fail("glu_int4: %d rows of x, %d hidden values, activation %d", M, hidden, act);
-  const Int4Args p = {(const __nv_bfloat16*)x, (const unsigned char*)w, (const __nv_bfloat16*)bias, (__nv_bfloat16*)y,
+  const Int4Args p = {(const __nv_bfloat16*)x, (const unsigned char*)w, {bias, bias_dtype == FMS_F32}, (__nv_bfloat16*)y,
                       M, 2 * hidden, K, k_blocks, per, hidden, act};
-  if (check(p)) return 1;
+  if (check(p) || check_bias("gemm_int4", p.bias, bias_dtype)) return 1;
   return few<true>(p, stream);
 }

@@ -70,10 +70,10 @@ _SIGNATURES = {
                                    _I, _I, _I, _P],
     "fms_quantize_rows": [_P, _I, _P, _P, _I, _I, _I, _P],
     "fms_add_rmsnorm_quantized": [_P, _P, _I, _P, _I, _F, _P, _P, _P, _I, _I, _I, _I, _P],
-    "fms_linear_e4m3": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _L, _P, _L, _P, _P],
-    "fms_glu_e4m3": [_P, _P, _P, _P, _P, _P, _I, _I, _L, _I, _P, _L, _P, _P],
-    "fms_linear_int4": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _L, _P, _P],
-    "fms_glu_int4": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
+    "fms_linear_e4m3": [_P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _L, _P, _L, _P, _P],
+    "fms_glu_e4m3": [_P, _P, _P, _P, _P, _I, _P, _I, _I, _L, _I, _P, _L, _P, _P],
+    "fms_linear_int4": [_P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _L, _P, _P],
+    "fms_glu_int4": [_P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
     "fms_embed_pair_hash": [_P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _L, _L, _L, _F, _I, _I, _I, _P, _P],
     "fms_normed_add_rmsnorm": [_P, _P, _I, _P, _F, _F, _P, _F, _F, _I, _P, _I, _P, _I, _I, _I, _P],
     "fms_mingru_scan": [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _P, _P],

@@ -278,12 +278,15 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 128) -> Int4Weight:
 
 
 # ---- products --------------------------------------------------------------------------------------------------------
-def _bias(what: str, bias: Optional[torch.Tensor], out: int) -> Optional[torch.Tensor]:
+def _bias(what: str, bias: Optional[torch.Tensor], out: int):
+    """A bias as the products add it to their float32 sums, and its dtype's code: bfloat16 and float32 as they are, others in float32."""
     if bias is None:
-        return None
+        return None, ops.BF16
     if tuple(bias.shape) != (out,):
         raise ops.KernelError(f"{what}: a bias of {tuple(bias.shape)} for {out} output channels")
-    return bias if bias.dtype == torch.bfloat16 else bias.to(torch.bfloat16)
+    if bias.dtype not in (torch.bfloat16, torch.float32):
+        bias = bias.to(torch.float32)
+    return bias, ops._code(bias.dtype)
 
 
 def _rows_for(what: str, x, weight: E4M3Weight) -> QuantizedRows:
@@ -314,17 +317,17 @@ def _scratch(library: str, name: str, device, rows: int, *sizes):
 
 
 def linear_e4m3(x, weight: E4M3Weight, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """Rows ``x`` (``QuantizedRows``; a tensor is quantised first) times weight [out, in] transposed (+ bias), summed in float32,
-    in bfloat16 or float32."""
+    """Rows ``x`` (``QuantizedRows``; a tensor is quantised first) times weight [out, in] transposed (+ bias,
+    bfloat16 or float32), summed in float32, in bfloat16 or float32."""
     x = _rows_for("linear_e4m3", x, weight)
     (m, _), (n, _) = x.shape, weight.shape
-    bias = _bias("linear_e4m3", bias, n)
+    bias, bias_code = _bias("linear_e4m3", bias, n)
     _on_device("linear_e4m3", bias)
     code = ops._code(out_dtype)
     y = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=x.device)
     pitch = x.values.shape[1]
     scratch, floats = _scratch("gemm_e4m3", "fms_e4m3_scratch", x.device, m, n, pitch, 0)
-    ops._call("gemm_e4m3", "fms_linear_e4m3", x.values, x.scales, weight.rows.values, weight.rows.scales, bias, y, code, m, n,
+    ops._call("gemm_e4m3", "fms_linear_e4m3", x.values, x.scales, weight.rows.values, weight.rows.scales, bias, bias_code, y, code, m, n,
               pitch, scratch, floats, ops.error_flag(x.device), ops._stream())
     return y
 
@@ -335,17 +338,17 @@ def gated_linear_e4m3(x, weight: E4M3Weight, bias: Optional[torch.Tensor], activ
     (m, _), (n, _) = x.shape, weight.shape
     if n % 2:
         raise ops.KernelError(f"gated_linear_e4m3: {n} rows are no gate and up matrix")
-    bias = _bias("gated_linear_e4m3", bias, n)
+    bias, bias_code = _bias("gated_linear_e4m3", bias, n)
     _on_device("gated_linear_e4m3", bias)
     y = torch.empty((m, n // 2), dtype=torch.bfloat16, device=x.device)
     pitch = x.values.shape[1]
     scratch, floats = _scratch("gemm_e4m3", "fms_e4m3_scratch", x.device, m, n, pitch, 1)
-    ops._call("gemm_e4m3", "fms_glu_e4m3", x.values, x.scales, weight.rows.values, weight.rows.scales, bias, y, m, n // 2,
+    ops._call("gemm_e4m3", "fms_glu_e4m3", x.values, x.scales, weight.rows.values, weight.rows.scales, bias, bias_code, y, m, n // 2,
               pitch, int(activation), scratch, floats, ops.error_flag(x.device), ops._stream())
     return y
 
 
-def _int4_checked(what: str, x: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+def _int4_checked(what: str, x: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor]):
     if not isinstance(weight, Int4Weight):
         raise ops.KernelError(f"{what}: the weight is an Int4Weight, not {type(weight).__name__}")
     if not isinstance(x, torch.Tensor) or x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != weight.shape[1]:
@@ -353,19 +356,19 @@ def _int4_checked(what: str, x: torch.Tensor, weight: Int4Weight, bias: Optional
         raise ops.KernelError(f"{what}: x is bfloat16 [rows, {weight.shape[1]}], not {got}")
     if x.data_ptr() % 16:
         raise ops.KernelError(f"{what}: x must be 16-byte aligned")
-    bias = _bias(what, bias, weight.shape[0])
+    bias, code = _bias(what, bias, weight.shape[0])
     _on_device(what, x, weight.blocks, bias)
-    return bias
+    return bias, code
 
 
 def linear_int4(x: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Rows ``x`` [rows, in] bfloat16 times weight [out, in] transposed (+ bias), summed in float32, in bfloat16.  Up to 8 rows the
-    weights are multiplied as they stand; more rows meet them rounded to bfloat16."""
-    bias = _int4_checked("linear_int4", x, weight, bias)
+    """Rows ``x`` [rows, in] bfloat16 times weight [out, in] transposed (+ bias, bfloat16 or float32), summed in float32, in
+    bfloat16.  Up to 8 rows the weights are multiplied as they stand; more rows meet them rounded to bfloat16."""
+    bias, bias_code = _int4_checked("linear_int4", x, weight, bias)
     (n, k), blocks = weight.shape, weight.blocks
     y = torch.empty_strided((x.shape[0], n), (n, 1), dtype=torch.bfloat16, device=x.device)
     scratch, floats = _scratch("gemm_int4", "fms_linear_int4_scratch", x.device, x.shape[0], n, k)
-    ops._call("gemm_int4", "fms_linear_int4", x, blocks, bias, y, x.shape[0], n, k, blocks.shape[1], weight.per, scratch, floats,
+    ops._call("gemm_int4", "fms_linear_int4", x, blocks, bias, bias_code, y, x.shape[0], n, k, blocks.shape[1], weight.per, scratch, floats,
               ops.error_flag(x.device), ops._stream())
     return y
 
@@ -373,14 +376,14 @@ def linear_int4(x: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor
 def gated_linear_int4(x: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor], activation: int) -> torch.Tensor:
     """act(x Wg^T) * (x Wu^T) in bfloat16 for weight = [Wg; Wu]: one kernel for few rows (and a hidden size that is a
     multiple of 16), else the product and ``gated_activation``."""
-    bias = _int4_checked("gated_linear_int4", x, weight, bias)
+    bias, bias_code = _int4_checked("gated_linear_int4", x, weight, bias)
     (n, k), blocks = weight.shape, weight.blocks
     if n % 2:
         raise ops.KernelError(f"gated_linear_int4: {n} rows are no gate and up matrix")
     if x.shape[0] > INT4_FEW_ROWS or n % 32:
         return ops.gated_activation(linear_int4(x, weight, bias), activation)
     y = torch.empty((x.shape[0], n // 2), dtype=torch.bfloat16, device=x.device)
-    ops._call("gemm_int4", "fms_glu_int4", x, blocks, bias, y, x.shape[0], n // 2, k, blocks.shape[1], weight.per, int(activation),
+    ops._call("gemm_int4", "fms_glu_int4", x, blocks, bias, bias_code, y, x.shape[0], n // 2, k, blocks.shape[1], weight.per, int(activation),
               ops._stream())
     return y
 

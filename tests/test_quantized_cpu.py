@@ -195,3 +195,16 @@ def test_rows_come_through_the_coherent_path():
     assert "__restrict__" not in text and "__ldg" not in text and "ld.global.nc" not in text
     with open(os.path.join(CSRC, "gemm_int4.cu")) as f:
         assert "__ldg" not in f.read()
+
+
+def test_a_bias_is_added_as_it_is():
+    from fms_b200.kernels import quantized
+
+    b = 1 + torch.arange(16) * 2.0 ** -20
+    for kept in (b, b.to(BF16)):
+        got, code = quantized._bias("linear", kept, 16)
+        assert got is kept and code == (ops.F32 if kept.dtype == torch.float32 else ops.BF16)
+    got, code = quantized._bias("linear", b.half(), 16)
+    assert code == ops.F32 and torch.equal(got, b.half().float())
+    with pytest.raises(ops.KernelError):
+        quantized._bias("linear", b, 15)

@@ -582,3 +582,24 @@ def test_a_run_of_them_replayed_with_other_inputs(ops, rows, dim):
         return torch.cat((ops.linear_int4(c, w4).float(), stream))
 
     behind(lambda held: held * 1, run, inputs)
+
+
+# ---- biases ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16, torch.float16])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 72), (8, 320, 128), (9, 200, 640), (40, 72, 2600), (100, 1000, 272), (200, 20000, 96), (300, 520, 1040)])
+def test_a_bias_of_more_bits_keeps_them(ops, m, n, k, dtype):
+    """Whole numbers below 2^12 and a bias of 16 bits behind the point: their sum in float32 is exact up to its one rounding."""
+    g = gen(m + n + k)
+    x, w = whole(g, -1, 1, m, k).float(), whole(g, -1, 1, n, k).float()
+    bias = ((whole(g, -2 ** 20, 2 ** 20, n).double() + 0.5) * 2.0 ** -16).to(dtype)
+    want = (x.double() @ w.double().t() + bias.double()).float()
+    one = lambda r: torch.ones(r, device="cuda")  # noqa: E731
+    rows, w8 = ops.QuantizedRows.of(x.to(E4M3), one(m)), ops.e4m3_weight(w.to(E4M3), one(n))
+    assert torch.equal(ops.linear_e4m3(rows, w8, bias, F32), want)
+    assert torch.equal(ops.linear_e4m3(rows, w8, bias), want.to(BF16))
+    w4 = ops.pack_int4((w + 8).to(torch.uint8), torch.ones(n, -(-k // 128), device="cuda"))
+    assert torch.equal(ops.linear_int4(x.to(BF16), w4, bias), want.to(BF16))
+    relu = torch.relu(want[:, : n // 2].double()) * want[:, n // 2:].double()  # at most 12 + 16 bits each: rounded once to float32, once to bfloat16
+    assert torch.equal(ops.gated_linear_e4m3(rows, w8, bias, 3), relu.float().to(BF16))
+    if m <= 8 and n % 32 == 0:
+        assert torch.equal(ops.gated_linear_int4(x.to(BF16), w4, bias, 3), relu.float().to(BF16))
