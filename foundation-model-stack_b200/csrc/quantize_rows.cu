@@ -5,7 +5,8 @@
 //                     y = x * rsqrt(mean(x^2) + eps) * gain,  s = max |y| / 448,  q = e4m3(y * 448 / max |y|)
 //                                                                   (the norm: fms/modules/layernorm.py:56-69)
 // e4m3() rounds to the nearest value, ties to even.  A row whose scale would lie below 2^-110 (a row of zeros) gets scale 0
-// and zeros.  A row with a NaN or an infinity gets a scale that is not finite (NaN behind the norm),
+// and zeros.  A finite row whose squares overflow float32 (values beyond some 10^19) is summed again, with 2^-80 of every value, which
+// the quotient and the division by the root mean square cancel.  A row with a NaN or an infinity gets a scale that is not finite (NaN behind the norm),
 // so that what a product makes of it is not finite either, and the other rows do not see it.
 //
 // Both are bound by memory: a value is read once (2 or 4 bytes, behind the norm 4 and 2 or 4), the stream written (4) and
@@ -29,6 +30,7 @@
 namespace {
 constexpr float E4M3_MAX = 448.f;
 constexpr float LEAST = 0x1p-110f;  // a scale below is none
+constexpr float SHRUNK = 0x1p-80f;   // of a row whose squares overflow: then the sum of up to 2^31 does not
 
 // the larger of two, NaN where either is one
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -271,61 +273,77 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2
       for (int j = 0; j < KEPT; ++j) add(x[j], d[j]);
     }
   }
-  float ss = 0.f;
-  Pair most = {0.f, 0.f};
-#pragma unroll KEPT
-  for (int j = 0; j < runs; ++j) {
-    Run<float>& xs = x[RUNS > 0 ? j : 0];
-    Run<TG>& gs = g[RUNS > 0 ? j : 0];
-    if (RUNS == 0) {
-      load_run<NEIGHBOURS>(xs, res, j, shift, dim);
-      load_run<NEIGHBOURS>(gs, gain, j, shift, dim);
-      if (del) {
-        Run<T> d;
-        load_run<NEIGHBOURS>(d, del, j, shift, dim);
-        add(xs, d);
-      }
-    }
-    if (writes) {
-      const int c0 = place(j, shift);
-      if (c0 >= 0 && c0 + 8 <= dim) {
-        float4* to = reinterpret_cast<float4*>(res + c0);
-        to[0] = make_float4(xs.v[0], xs.v[1], xs.v[2], xs.v[3]);
-        to[1] = make_float4(xs.v[4], xs.v[5], xs.v[6], xs.v[7]);
-      } else if (!NEIGHBOURS) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c0 + e >= 0 && c0 + e < dim) res[c0 + e] = xs.v[e];
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      ss += xs[e] * xs[e];
-      const float t = xs[e] * gs[e], left = fmaf(xs[e], gs[e], -t);
-      most = larger(most, Pair{fabsf(t), t < 0.f ? -left : left});
-    }
-  }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
-  auto over_warp = [&]() {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      most = larger(most, Pair{__shfl_xor_sync(0xffffffffu, most.hi, o), __shfl_xor_sync(0xffffffffu, most.lo, o)});
+  // RUNS 0: a run's sums and gains, read again in every pass
+  auto fetch = [&](int j, bool stored) {
+    load_run<NEIGHBOURS>(x[0], res, j, shift, dim);  // the sum, where this thread has stored it
+    load_run<NEIGHBOURS>(g[0], gain, j, shift, dim);
+    if (del && !stored) {
+      Run<T> d;
+      load_run<NEIGHBOURS>(d, del, j, shift, dim);
+      add(x[0], d);
     }
   };
-  over_warp();
-  if (lane == 0) {
-    scratch[0][warp] = ss;
-    scratch[1][warp] = most.hi;
-    scratch[2][warp] = most.lo;
+  auto shrink = [&](Run<float>& v) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v.v[e] *= SHRUNK;
+  };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  float ss;
+  Pair most;
+  bool shrunk = false;  // the whole block alike
+#pragma unroll 1
+  while (true) {
+    ss = 0.f;
+    most = {0.f, 0.f};
+#pragma unroll KEPT
+    for (int j = 0; j < runs; ++j) {
+      Run<float>& xs = x[RUNS > 0 ? j : 0];
+      Run<TG>& gs = g[RUNS > 0 ? j : 0];
+      if (RUNS == 0) fetch(j, shrunk && writes);
+      if (writes && !shrunk) {
+        const int c0 = place(j, shift);
+        if (c0 >= 0 && c0 + 8 <= dim) {
+          float4* to = reinterpret_cast<float4*>(res + c0);
+          to[0] = make_float4(xs.v[0], xs.v[1], xs.v[2], xs.v[3]);
+          to[1] = make_float4(xs.v[4], xs.v[5], xs.v[6], xs.v[7]);
+        } else if (!NEIGHBOURS) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c0 + e >= 0 && c0 + e < dim) res[c0 + e] = xs.v[e];
+        }
+      }
+      if (shrunk) shrink(xs);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        ss += xs[e] * xs[e];
+        const float t = xs[e] * gs[e], left = fmaf(xs[e], gs[e], -t);
+        most = larger(most, Pair{fabsf(t), t < 0.f ? -left : left});
+      }
+    }
+    auto over_warp = [&]() {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        most = larger(most, Pair{__shfl_xor_sync(0xffffffffu, most.hi, o), __shfl_xor_sync(0xffffffffu, most.lo, o)});
+      }
+    };
+    over_warp();
+    if (lane == 0) {
+      scratch[0][warp] = ss;
+      scratch[1][warp] = most.hi;
+      scratch[2][warp] = most.lo;
+    }
+    __syncthreads();
+    ss = lane < nwarps ? scratch[0][lane] : 0.f;
+    most = lane < nwarps ? Pair{scratch[1][lane], scratch[2][lane]} : Pair{0.f, 0.f};
+    over_warp();
+    if (ss < INFINITY || shrunk) break;
+    shrunk = true;
+    __syncthreads();  // scratch is written again
   }
-  __syncthreads();
-  ss = lane < nwarps ? scratch[0][lane] : 0.f;
-  most = lane < nwarps ? Pair{scratch[1][lane], scratch[2][lane]} : Pair{0.f, 0.f};
-  over_warp();
 
-  // a NaN or an infinity in the row leaves `ss` not finite and the scale NaN (infinity times a root of 0, or NaN)
-  const float s = ss < INFINITY ? most.hi * rsqrtf(ss / (float)dim + eps) / E4M3_MAX : NAN;
+  // a NaN or an infinity in the row leaves `ss` not finite; eps is nothing beside the squares of a row that was shrunk
+  const float s = ss < INFINITY ? most.hi * rsqrtf(ss / (float)dim + (shrunk ? 0.f : eps)) / E4M3_MAX : NAN;
   const bool none = s < LEAST || most.hi < LEAST;  // far below, the reciprocal would overflow
   const float inv = none ? 0.f : (s == s ? E4M3_MAX / most.hi : NAN);
   const double exact = (double)most.hi + (double)most.lo;
@@ -334,13 +352,8 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2
     Run<float>& xs = x[RUNS > 0 ? j : 0];
     Run<TG>& gs = g[RUNS > 0 ? j : 0];
     if (RUNS == 0) {
-      load_run<NEIGHBOURS>(xs, res, j, shift, dim);  // the sum, where this thread has stored it
-      load_run<NEIGHBOURS>(gs, gain, j, shift, dim);
-      if (del && !writes) {
-        Run<T> d;
-        load_run<NEIGHBOURS>(d, del, j, shift, dim);
-        add(xs, d);
-      }
+      fetch(j, writes);
+      if (shrunk) shrink(xs);
     }
     store_run<NEIGHBOURS>(q + (size_t)blockIdx.x * pitch, quotients<NEIGHBOURS, true>(xs, gs, inv, exact, place(j, shift), dim), j, shift, pitch);
   }

@@ -603,3 +603,32 @@ def test_a_bias_of_more_bits_keeps_them(ops, m, n, k, dtype):
     assert torch.equal(ops.gated_linear_e4m3(rows, w8, bias, 3), relu.float().to(BF16))
     if m <= 8 and n % 32 == 0:
         assert torch.equal(ops.gated_linear_int4(x.to(BF16), w4, bias, 3), relu.float().to(BF16))
+
+
+# ---- rows whose squares overflow float32 -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, None])
+@pytest.mark.parametrize("rows,dim", [(5, 240), (3, 17), (2, 5001), (300, 4096), (300, 16384), (6, 8192), (4, 1000), (3, 20000), (2, 33001)])
+def test_the_norm_of_rows_with_large_values(ops, dtype, rows, dim):
+    g = gen(rows + dim)
+    res = normal(g, rows, dim)
+    res[0] *= 1e25
+    res[1, 0] = 3e38  # one value alone
+    if rows > 2:
+        res[2] = 3.4e38 * torch.sign(res[2])  # every value
+    delta = None if dtype is None else normal(g, rows, dim, std=1e24).to(dtype)
+    if delta is not None:
+        delta[1:] = 0
+    gain = 1 + normal(g, dim, std=0.1)
+    total = res.clone() if delta is None else res + delta.float()
+    y = ops.add_rmsnorm_quantized(res, delta, gain, 1e-5)
+    assert torch.equal(res, total)
+    t = total.double() * gain.double()
+    norm = t / (total.double().square().mean(1, keepdim=True) + 1e-5).sqrt()
+    # the sum of squares: a thread's runs of 8 values, 4 of them or one for every 4,096 values of the row, and 10 levels; the rest as above
+    terms = 8 * max(4, -(-(dim + 16) // 4096)) + 10
+    torch.testing.assert_close(y.scales.double(), norm.abs().amax(1) / 448, atol=0, rtol=2.0 ** -24 * (terms / 2 + 4 + 6))
+    want, _ = nearest_e4m3(t * 448 / t.abs().amax(1, keepdim=True))
+    assert torch.equal(y.values[:, :dim].double(), want)
+    if rows > 3:  # the others' rows do not see it
+        alone = ops.add_rmsnorm_quantized(total[3:].contiguous(), None, gain, 1e-5)
+        assert torch.equal(alone.values.view(torch.uint8), y.values[3:].view(torch.uint8))
