@@ -45,6 +45,7 @@ struct Epilogue {
   int tile_n, stages, n_tokens;
   float* scratch;             // [blocks][slots][n_tokens][128], of the second kernel
   int slots;                  // of a block in scratch, or 0: each takes one whole tile
+  long scratch_floats;        // for the bounds-checked build
 };
 
 // four sums times the scales of their row and columns (+ bias)
@@ -403,7 +404,8 @@ __global__ void __launch_bounds__(ROWS_THREADS, 2) e4m3_rows_kernel(const __grid
             *reinterpret_cast<float4*>(sums + row * sums_pitch + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         } else if (!whole) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) slot[(size_t)(c0 + j) * TILE] = v[j];
+          for (int j = 0; j < 16; ++j)
+            if (FMS_IN(slot + (c0 + j) * TILE - ep.scratch, max(ep.scratch_floats, 1L))) slot[(size_t)(c0 + j) * TILE] = v[j];
         } else if (live) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) v[j] = fmaf(v[j], row_scales[c0 + j] * sw, bias);
@@ -464,6 +466,7 @@ __global__ void __launch_bounds__(TILE) e4m3_join_kernel(Epilogue ep, int M, int
   float sx[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) sx[j] = t0 + j < M ? ep.sx[t0 + j] : 0.f;
+  auto sum_of = [&](const float* at) { return FMS_IN(at - ep.scratch, max(ep.scratch_floats, 1L)) ? __ldcg(at) : 0.f; };
   auto total = [&](int r, float* sum) {
     const float* slots = ep.scratch + (size_t)t0 * TILE + r;
     sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
@@ -473,7 +476,7 @@ __global__ void __launch_bounds__(TILE) e4m3_join_kernel(Epilogue ep, int M, int
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          v[i][j] = b + i <= to ? __ldcg(slots + ((size_t)ep.slots * (b + i) + (b + i == from ? head : 0)) * pitch + j * TILE) : 0.f;
+          v[i][j] = b + i <= to ? sum_of(slots + ((size_t)ep.slots * (b + i) + (b + i == from ? head : 0)) * pitch + j * TILE) : 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -588,6 +591,7 @@ int launch(const void* x, const void* w, Epilogue ep, int M, int N, long pitch, 
     const Cut c = cut_of(ep.outputs, ep.glu != 0, pitch);
     ep.n_tokens = (M + 15) / 16 * 16;
     ep.slots = c.slots;
+    ep.scratch_floats = scratch_floats;
     if ((long)c.tiles * c.k_steps > 0x3fffffffL) return fms_fail("gemm_e4m3: %d tiles of %d steps", c.tiles, c.k_steps);
     const long wanted = (long)c.blocks * c.slots * ep.n_tokens * TILE;
     if (scratch_floats < wanted) return fms_fail("gemm_e4m3: %ld floats of scratch memory, %ld are wanted", scratch_floats, wanted);

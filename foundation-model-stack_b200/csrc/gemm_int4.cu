@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 1) int4_few_rows_kernel(Int4Ar
     uint4 w[AHEAD][2];
     uint32_t gw[AHEAD][2 * PER];
     auto load = [&](int at) {
+      if (!FMS_IN(next - piece - p.w + BYTES - 1, (size_t)p.row_blocks() * p.k_blocks * BYTES)) return;
       w[at][0] = load_once(reinterpret_cast<const uint4*>(next));
       w[at][1] = load_once(reinterpret_cast<const uint4*>(next + 512));
 #pragma unroll
@@ -166,12 +167,13 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 1) int4_few_rows_kernel(Int4Ar
     const uint4* xs = reinterpret_cast<const uint4*>(xp + (p.K - left));
     auto multiply = [&](const uint4* wq, const uint32_t* gq) {
       uint4 b[4];
+      auto of_x = [&](int v) { return FMS_IN(xs + 4 * v - reinterpret_cast<const uint4*>(p.x), (size_t)p.M * p.K / 8) ? xs[4 * v] : make_uint4(0, 0, 0, 0); };
       if (left >= BLOCK_K) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) b[v] = xs[4 * v];
+        for (int v = 0; v < 4; ++v) b[v] = of_x(v);
       } else {  // K is a multiple of 8: a lane's 8 values are all inside or all outside
 #pragma unroll
-        for (int v = 0; v < 4; ++v) b[v] = left > 32 * v + 8 * c ? xs[4 * v] : make_uint4(0, 0, 0, 0);
+        for (int v = 0; v < 4; ++v) b[v] = left > 32 * v + 8 * c ? of_x(v) : make_uint4(0, 0, 0, 0);
       }
       const uint32_t wl[4] = {wq[0].x, wq[0].y, wq[0].z, wq[0].w}, wh[4] = {wq[1].x, wq[1].y, wq[1].z, wq[1].w};
 #pragma unroll
@@ -205,7 +207,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 1) int4_few_rows_kernel(Int4Ar
           left -= BLOCK_K;
           xs += BLOCK_K / 8;
           if (left <= 0 || todo == 0) {  // the tile's last block, or this warp's
-            sums[warp][slot++][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            if (FMS_IN(slot, 2)) sums[warp][slot][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            ++slot;
             acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
             left = p.K;
             xs = reinterpret_cast<const uint4*>(xp);
@@ -221,6 +224,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 1) int4_few_rows_kernel(Int4Ar
       const int at = ((row & 7) * 4 + (m >> 1)) * 4 + (row >> 3) * 2 + (m & 1);  // of 128
       auto total = [&](int t) {
         const int first = t * p.k_blocks, w_lo = warp_of(first), w_hi = warp_of(first + p.k_blocks - 1);
+        if (!FMS_IN(w_lo, warps) || !FMS_IN(w_hi, warps)) return 0.f;
         // only the first warp of a tile can have begun with an earlier one
         float sum = reinterpret_cast<const float*>(sums[w_lo][run(w_lo) < first ? 1 : 0])[at];
 #pragma unroll 4
@@ -393,6 +397,7 @@ struct RowsArgs {
   Int4Args p;
   int n_tokens, stages, groups, a_stages, issuers, accs, acc_columns;
   float* scratch;  // [2 blocks][n_tokens][128]: a block's first tile, then its last, where it has not all of it
+  long scratch_floats;  // for the bounds-checked build
 };
 __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid_constant__ CUtensorMap map_x,
                                                                     const __grid_constant__ CUtensorMap map_w, RowsArgs a,
@@ -544,7 +549,8 @@ __global__ void __launch_bounds__(ROWS_THREADS, 1) int4_rows_kernel(const __grid
           if (col < p.N) store_column<16>(p, v, c0, col, bias);
         } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) slot[(size_t)(c0 + j) * TILE] = v[j];
+          for (int j = 0; j < 16; ++j)
+            if (FMS_IN(slot + (c0 + j) * TILE - a.scratch, max(a.scratch_floats, 1L))) slot[(size_t)(c0 + j) * TILE] = v[j];
         }
       }
       tc_fence_before();
@@ -578,13 +584,14 @@ __global__ void __launch_bounds__(TILE) int4_join_kernel(RowsArgs a, int blocks)
   const size_t pitch = (size_t)a.n_tokens * TILE;
   pdl_wait();
   const float bias = p.bias ? p.bias[col] : 0.f;  // any tensor: the kernel before the product may have written it
+  auto sum_of = [&](const float* at) { return FMS_IN(at - a.scratch, max(a.scratch_floats, 1L)) ? __ldcg(at) : 0.f; };
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   for (int b = from; b <= to; b += 4) {
     float v[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = b + i <= to ? __ldcg(slots + (2 * (b + i) + (b + i == from ? head : 0)) * pitch + j * TILE) : 0.f;
+      for (int j = 0; j < 4; ++j) v[i][j] = b + i <= to ? sum_of(slots + (2 * (b + i) + (b + i == from ? head : 0)) * pitch + j * TILE) : 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -613,6 +620,7 @@ int launch_rows(const Int4Args& p, float* scratch, long scratch_floats, int* err
   a.p = p;
   a.n_tokens = (p.M + 15) / 16 * 16;
   a.scratch = scratch;
+  a.scratch_floats = scratch_floats;
   const int tiles = (p.N + TILE - 1) / TILE, blocks = rows_blocks(p.N, p.K);
   if ((long)tiles * p.k_blocks > 0x3fffffffL) return fms_fail("gemm_int4: %d tiles of %d blocks", tiles, p.k_blocks);
   if (scratch_floats < rows_scratch(p.M, p.N, p.K)) return fms_fail("gemm_int4: %ld floats of scratch memory, %ld are wanted", scratch_floats, rows_scratch(p.M, p.N, p.K));

@@ -77,20 +77,20 @@ template <> struct Run<__nv_bfloat16> {
 __device__ __forceinline__ int place(int j, int shift) { return 8 * (int)(threadIdx.x + j * blockDim.x) - shift; }
 // the values by which the runs of a row are moved so that 4 of them lie aligned
 template <typename T> __device__ __forceinline__ int shift_of(const T* row) { return (int)((uintptr_t)row / sizeof(T)) & 3; }
-// zeros outside the row
-template <bool NEIGHBOURS, typename T> __device__ __forceinline__ void load_run(Run<T>& run, const T* row, int j, int shift, int dim) {
+// zeros outside the row; `left`: the values from its first to the array's last, for the bounds-checked build
+template <bool NEIGHBOURS, typename T> __device__ __forceinline__ void load_run(Run<T>& run, const T* row, int j, int shift, int dim, long left) {
   const int c0 = place(j, NEIGHBOURS ? 0 : shift);
   if (NEIGHBOURS) {
-    if (c0 < dim) {
+    if (c0 < dim && FMS_IN(c0 + 7, left)) {
       run.load(row + c0);
       return;
     }
-  } else if (c0 >= 0 && c0 + 8 <= dim && Run<T>::aligned(row + c0)) {  // (taking the others as three aligned loads and picking was slower)
+  } else if (c0 >= 0 && c0 + 8 <= dim && Run<T>::aligned(row + c0) && FMS_IN(c0 + 7, left)) {  // (taking the others as three aligned loads and picking was slower)
     run.load_halves(row + c0);
     return;
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) run.set(e, !NEIGHBOURS && c0 + e >= 0 && c0 + e < dim ? row[c0 + e] : T(0.f));
+  for (int e = 0; e < 8; ++e) run.set(e, !NEIGHBOURS && c0 + e >= 0 && c0 + e < dim && FMS_IN(c0 + e, left) ? row[c0 + e] : T(0.f));
 }
 // 8 values as e4m3, nearest and ties to even, beyond 448 to 448
 __device__ __forceinline__ uint2 to_e4m3(const float* v) {
@@ -148,23 +148,23 @@ __device__ __forceinline__ uint2 quotients(const X& x, const G& g, float inv, do
   return to_e4m3(ended<NEIGHBOURS>(q, c0, dim));
 }
 // By a whole warp.  A run that is moved by `shift` holds the last bytes of its aligned 8 first: the next lane has the others.
-template <bool NEIGHBOURS> __device__ __forceinline__ void store_run(uint8_t* row, uint2 q, int j, int shift, int pitch) {
+template <bool NEIGHBOURS> __device__ __forceinline__ void store_run(uint8_t* row, uint2 q, int j, int shift, int pitch, long left) {
   const int at = place(j, 0);
   if (NEIGHBOURS || shift == 0) {
-    if (at < pitch) *reinterpret_cast<uint2*>(row + at) = q;
+    if (at < pitch && FMS_IN(at + 7, left)) *reinterpret_cast<uint2*>(row + at) = q;
     return;
   }
   const uint64_t own = ((uint64_t)q.y << 32) | q.x, next = __shfl_down_sync(0xffffffffu, own, 1);
   const int lane = threadIdx.x & 31, bits = 8 * shift;
   if (lane < 31) {
-    if (at < pitch) *reinterpret_cast<uint64_t*>(row + at) = (own >> bits) | (next << (64 - bits));
+    if (at < pitch && FMS_IN(at + 7, left)) *reinterpret_cast<uint64_t*>(row + at) = (own >> bits) | (next << (64 - bits));
   } else {
     for (int e = shift; e < 8; ++e)
-      if (at + e - shift < pitch) row[at + e - shift] = (uint8_t)(own >> (8 * e));
+      if (at + e - shift < pitch && FMS_IN(at + e - shift, left)) row[at + e - shift] = (uint8_t)(own >> (8 * e));
   }
   if (lane == 0 && at > 0)  // what the warp before could not store
     for (int e = 0; e < shift; ++e)
-      if (at + e - shift < pitch) row[at + e - shift] = (uint8_t)(own >> (8 * e));
+      if (at + e - shift < pitch && FMS_IN(at + e - shift, left)) row[at + e - shift] = (uint8_t)(own >> (8 * e));
 }
 
 __device__ __forceinline__ float block_max(float v, float* scratch) {
@@ -201,23 +201,23 @@ __device__ __forceinline__ float largest(const Run<__nv_bfloat16>& r) {
 // 14,336 (2,048 of them, bfloat16: 17.9 us, 4.9 TB/s; with two blocks 20.8, with four 19.2 for the registers that spill).
 template <typename T, int RUNS, bool NEIGHBOURS>
 __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && RUNS == 4 && sizeof(T) == 2 ? 3 : (RUNS != 1 && RUNS != 8 ? 2 : 1))
-    quantize_rows_kernel(const T* x, uint8_t* q, float* scales, int n_rows, int dim, int pitch) {
+    quantize_rows_kernel(const T* x, uint8_t* q, float* scales, int dim, int pitch) {
   __shared__ float scratch[32];
   pdl_launch_dependents();
   pdl_wait();
-  if (!FMS_IN(blockIdx.x, n_rows)) return;
   const T* row = x + (size_t)blockIdx.x * dim;
   uint8_t* out = q + (size_t)blockIdx.x * pitch;
+  const long left = (long)(gridDim.x - blockIdx.x) * dim;
   constexpr int KEPT = RUNS > 0 ? RUNS : 1;
   const int runs = RUNS > 0 ? RUNS : (pitch / 8 + !NEIGHBOURS + blockDim.x - 1) / blockDim.x, shift = NEIGHBOURS ? 0 : shift_of(row);
   Run<T> v[KEPT];
   float most = 0.f;
 #pragma unroll
   for (int j = 0; j < KEPT; ++j)
-    if (RUNS > 0) load_run<NEIGHBOURS>(v[j], row, j, shift, dim);
+    if (RUNS > 0) load_run<NEIGHBOURS>(v[j], row, j, shift, dim, left);
 #pragma unroll KEPT
   for (int j = 0; j < runs; ++j) {
-    if (RUNS == 0) load_run<NEIGHBOURS>(v[0], row, j, shift, dim);
+    if (RUNS == 0) load_run<NEIGHBOURS>(v[0], row, j, shift, dim, left);
     most = max_nan(most, largest(v[RUNS > 0 ? j : 0]));
   }
   most = block_max(most, scratch);
@@ -226,9 +226,9 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, NEIGHBOURS && RUNS == 
   const float inv = none ? 0.f : E4M3_MAX / most;
 #pragma unroll KEPT
   for (int j = 0; j < runs; ++j) {
-    if (RUNS == 0) load_run<NEIGHBOURS>(v[0], row, j, shift, dim);
+    if (RUNS == 0) load_run<NEIGHBOURS>(v[0], row, j, shift, dim, left);
     const Run<T>& u = v[RUNS > 0 ? j : 0];
-    store_run<NEIGHBOURS>(out, quotients<NEIGHBOURS, false>(u, u, inv, most, place(j, shift), dim), j, shift, pitch);
+    store_run<NEIGHBOURS>(out, quotients<NEIGHBOURS, false>(u, u, inv, most, place(j, shift), dim), j, shift, pitch, (long)(gridDim.x - blockIdx.x) * pitch);
   }
   if (threadIdx.x == 0) scales[blockIdx.x] = none ? 0.f : s;
 }
@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2
   const int src = rows ? rows[blockIdx.x] : blockIdx.x;
   if (!FMS_IN(src, residual_rows)) return;  // the whole block alike
   float* res = residual + (size_t)src * dim;
+  const long left = residual_rows > 0 ? (long)(residual_rows - src) * dim : 0;
   const int shift = NEIGHBOURS ? 0 : shift_of(res);
   const T* del = delta ? delta + (size_t)src * dim : nullptr;
   const bool writes = del && rows == nullptr;
@@ -263,23 +264,23 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2
   if (RUNS > 0) {
     Run<T> d[KEPT];
 #pragma unroll
-    for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(x[j], res, j, shift, dim);
+    for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(x[j], res, j, shift, dim, left);
 #pragma unroll
-    for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(g[j], gain, j, shift, dim);
+    for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(g[j], gain, j, shift, dim, dim);
     if (del) {
 #pragma unroll
-      for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(d[j], del, j, shift, dim);
+      for (int j = 0; j < KEPT; ++j) load_run<NEIGHBOURS>(d[j], del, j, shift, dim, left);
 #pragma unroll
       for (int j = 0; j < KEPT; ++j) add(x[j], d[j]);
     }
   }
   // RUNS 0: a run's sums and gains, read again in every pass
   auto fetch = [&](int j, bool stored) {
-    load_run<NEIGHBOURS>(x[0], res, j, shift, dim);  // the sum, where this thread has stored it
-    load_run<NEIGHBOURS>(g[0], gain, j, shift, dim);
+    load_run<NEIGHBOURS>(x[0], res, j, shift, dim, left);  // the sum, where this thread has stored it
+    load_run<NEIGHBOURS>(g[0], gain, j, shift, dim, dim);
     if (del && !stored) {
       Run<T> d;
-      load_run<NEIGHBOURS>(d, del, j, shift, dim);
+      load_run<NEIGHBOURS>(d, del, j, shift, dim, left);
       add(x[0], d);
     }
   };
@@ -302,14 +303,14 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2
       if (RUNS == 0) fetch(j, shrunk && writes);
       if (writes && !shrunk) {
         const int c0 = place(j, shift);
-        if (c0 >= 0 && c0 + 8 <= dim) {
+        if (c0 >= 0 && c0 + 8 <= dim && FMS_IN(c0 + 7, left)) {
           float4* to = reinterpret_cast<float4*>(res + c0);
           to[0] = make_float4(xs.v[0], xs.v[1], xs.v[2], xs.v[3]);
           to[1] = make_float4(xs.v[4], xs.v[5], xs.v[6], xs.v[7]);
         } else if (!NEIGHBOURS) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (c0 + e >= 0 && c0 + e < dim) res[c0 + e] = xs.v[e];
+            if (c0 + e >= 0 && c0 + e < dim && FMS_IN(c0 + e, left)) res[c0 + e] = xs.v[e];
         }
       }
       if (shrunk) shrink(xs);
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2
       fetch(j, writes);
       if (shrunk) shrink(xs);
     }
-    store_run<NEIGHBOURS>(q + (size_t)blockIdx.x * pitch, quotients<NEIGHBOURS, true>(xs, gs, inv, exact, place(j, shift), dim), j, shift, pitch);
+    store_run<NEIGHBOURS>(q + (size_t)blockIdx.x * pitch, quotients<NEIGHBOURS, true>(xs, gs, inv, exact, place(j, shift), dim), j, shift, pitch, (long)(gridDim.x - blockIdx.x) * pitch);
   }
   if (threadIdx.x == 0) scales[blockIdx.x] = none ? 0.f : s;
 }
@@ -376,7 +377,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 template <typename T, int RUNS>
 void launch_rows(int threads, bool neighbours, const void* x, uint8_t* q, float* scales, int n_rows, int dim, int pitch, cudaStream_t stream) {
   fms_launch(neighbours ? quantize_rows_kernel<T, RUNS, true> : quantize_rows_kernel<T, RUNS, false>, dim3(n_rows), dim3(threads), 0,
-             stream, (const T*)x, q, scales, n_rows, dim, pitch);
+             stream, (const T*)x, q, scales, dim, pitch);
 }
 template <typename T> int quantize(const void* x, uint8_t* q, float* scales, int n_rows, int dim, int pitch, cudaStream_t stream) {
   int threads;

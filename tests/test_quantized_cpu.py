@@ -208,3 +208,34 @@ def test_a_bias_is_added_as_it_is():
     assert code == ops.F32 and torch.equal(got, b.half().float())
     with pytest.raises(ops.KernelError):
         quantized._bias("linear", b, 15)
+
+
+def test_the_checked_build_checks_what_the_kernels_index():
+    """FMS_IN stands at what is computed per value: runs of a row, stores of bytes, the residual, sums in scratch memory, packed blocks."""
+    import os
+    import re
+
+    from fms_b200.kernels.build import CSRC
+
+    text = {}
+    for name in ("quantize_rows.cu", "gemm_e4m3.cu", "gemm_int4.cu"):
+        with open(os.path.join(CSRC, name)) as f:
+            text[name] = re.sub(r"//[^\n]*", "", f.read())
+    rows = text["quantize_rows.cu"]
+    for function in ("load_run", "store_run"):
+        body = rows[rows.index(f" {function}("):]
+        body = body[: body.index("\n}")]
+        for line in body.splitlines():
+            if re.search(r"row\[|run\.load|reinterpret_cast", line) and "FMS_IN" not in line:
+                before = body[: body.index(line)].rstrip().splitlines()[-1]
+                assert "FMS_IN" in before or re.match(r"\s*(static|template)", line), line
+    assert "FMS_IN(blockIdx" not in rows  # the grid's own size
+    for name in ("gemm_e4m3.cu", "gemm_int4.cu"):
+        lines = text[name].splitlines()
+        for i, line in enumerate(lines):
+            if re.search(r"\bslot\[\(size_t|__ldcg\(", line):
+                assert "FMS_IN" in line, line
+    few = text["gemm_int4.cu"]
+    few = few[few.index("int4_few_rows_kernel("):]
+    few = few[: few.index("\n}")]
+    assert few.count("FMS_IN(") >= 5
