@@ -554,7 +554,7 @@ Cut cut_of(int outputs, bool glu, long pitch) {
   if (3L * c.tiles >= 2L * sms || (long)c.k_steps * (sms - c.tiles) <= 16L * sms) {
     c.blocks = c.tiles;
     c.slots = 0;
-  } else {  // 18 steps a tile or more, so that there are more blocks than tiles, and a run reaches into two tiles at most
+  } else {  // more than 16 steps a tile and fewer tiles than multiprocessors, so more blocks than tiles: a run reaches into two at most
     const long runs = (long)c.tiles * c.k_steps / 4;
     c.blocks = runs < sms ? (int)runs : sms;
     c.slots = 2;

@@ -239,3 +239,25 @@ def test_the_checked_build_checks_what_the_kernels_index():
     few = few[few.index("int4_few_rows_kernel("):]
     few = few[: few.index("\n}")]
     assert few.count("FMS_IN(") >= 5
+
+
+def test_a_cut_has_more_blocks_than_tiles():
+    """Equal runs of an 8-bit product's steps: a run reaches into two tiles at most only where there are no fewer blocks than tiles, and a
+    block's sums have two places."""
+    import ctypes
+
+    from fms_b200.kernels.build import load_library
+
+    floats = load_library("gemm_e4m3").fms_e4m3_scratch
+    floats.restype, floats.argtypes = ctypes.c_long, [ctypes.c_long] * 4
+    cut = set()
+    for glu in (0, 1):
+        for steps in (1, 15, 16, 17, 18, 19, 24, 33, 64, 112, 400):
+            for tiles in range(1, 110):
+                columns = tiles * (64 if glu else 128)
+                got = floats(16, columns * (2 if glu else 1), steps * 128, glu)
+                if got:
+                    blocks = got // (2 * 16 * 128)
+                    assert got == blocks * 2 * 16 * 128 and tiles < blocks <= 148 and blocks * 4 <= tiles * steps
+                    cut.add(steps)
+    assert min(cut) == 17

@@ -632,3 +632,64 @@ def test_the_norm_of_rows_with_large_values(ops, dtype, rows, dim):
     if rows > 3:  # the others' rows do not see it
         alone = ops.add_rmsnorm_quantized(total[3:].contiguous(), None, gain, 1e-5)
         assert torch.equal(alone.values.view(torch.uint8), y.values[3:].view(torch.uint8))
+
+
+# ---- the gated product of more rows, and the sizes of calls on two streams, against 64 bits ------------------------------------
+def activated(gate, act):
+    f = torch.nn.functional
+    return [f.silu, f.gelu, lambda t: f.gelu(t, approximate="tanh"), torch.relu][act](gate)
+
+
+@pytest.mark.parametrize("act", [0, 1, 2, 3])
+@pytest.mark.parametrize("m,hidden,k,group", [(1, 5, 40, 32), (9, 80, 1040, 1040), (16, 4800, 384, 32), (17, 200, 256, 128), (64, 1000, 648, 64), (112, 9600, 136, 128),
+                                              (130, 2000, 264, 32), (300, 520, 1160, 160), (700, 3000, 136, 128)])
+def test_gated_linear_int4_of_more_rows(ops, act, m, hidden, k, group):
+    """The product in bfloat16, its weights rounded beyond 8 rows, then the activation of that: every rounding is counted."""
+    g = gen(act + m)
+    w = ops.quantize_int4(normal(g, 2 * hidden, k, std=k ** -0.5), group)
+    x, bias = normal(g, m, k).to(BF16), normal(g, 2 * hidden, std=0.1).to(BF16)
+    y = ops.gated_linear_int4(x, w, bias, act)
+    wd = w.dequantize().double() if m <= 8 else w.dequantize().to(BF16).double()
+    z = x.double() @ wd.t() + bias.double()
+    off = (k + 4) * 2.0 ** -23 * (x.double().abs() @ wd.abs().t()) + (HALF_STEP + 2.0 ** -22) * z.abs()
+    gate, up = z[:, :hidden], z[:, hidden:]
+    a = activated(gate, act)
+    # slopes of these activations stay below 1.2; expf, erff and tanhf are good to a few units of float32 in 1
+    a_off = 1.2 * off[:, :hidden] + 2.0 ** -20 * (a.abs() + gate.abs())
+    u_off = off[:, hidden:]
+    bound = a_off * up.abs() + (a.abs() + a_off) * u_off + (HALF_STEP + 2.0 ** -23) * (a.abs() + a_off) * (up.abs() + u_off) + 1e-30
+    assert y.shape == (m, hidden) and bool(((y.double() - a * up).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("m", [1, 8, 40, 200, 700])
+def test_products_of_a_wide_matrix(ops, m):
+    n, k = 6144, 2576
+    g = gen(m)
+    x, raw = normal(g, m, k).to(BF16), normal(g, n, k, std=0.02)
+    e4m3, int4 = ops.quantize_e4m3(raw), ops.quantize_int4(raw)
+    rows = ops.quantize_rows(x)
+    for xd, wd, linear, gated in ((rows.dequantize().double(), e4m3.dequantize().double(), lambda: ops.linear_e4m3(rows, e4m3), lambda: ops.gated_linear_e4m3(rows, e4m3, None, 1)),
+                                  (x.double(), int4.dequantize().double() if m <= 8 else int4.dequantize().to(BF16).double(),
+                                   lambda: ops.linear_int4(x, int4), lambda: ops.gated_linear_int4(x, int4, None, 1))):
+        z = xd @ wd.t()
+        off = (k + 6) * 2.0 ** -23 * (xd.abs() @ wd.abs().t()) + 2.0 ** -22 * z.abs()  # dequantize() rounds a value times its scale
+        assert bool(((linear().double() - z).abs() <= off + HALF_STEP * (z.abs() + off)).all())
+        gate, up = z[:, : n // 2], z[:, n // 2:]
+        off = off + HALF_STEP * z.abs()  # a product of its own in front of the activation
+        a, a_off, u_off = activated(gate, 1), 1.2 * off[:, : n // 2] + 2.0 ** -20 * gate.abs(), off[:, n // 2:]
+        a_off = a_off + 2.0 ** -20 * a.abs()
+        bound = a_off * up.abs() + (a.abs() + a_off) * u_off + (HALF_STEP + 2.0 ** -23) * (a.abs() + a_off) * (up.abs() + u_off)
+        assert bool(((gated().double() - a * up).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("m", [1, 16, 100])
+@pytest.mark.parametrize("n,k", [(100, 2176), (1000, 2176), (100, 2064), (128, 2048)])
+def test_linear_e4m3_at_the_fewest_steps_that_are_cut(ops, m, n, k):
+    """17 steps of 128 a tile and few tiles: equal runs, joined; 16: whole tiles."""
+    x, w, sx, sw, bias = e4m3_case(m, n, k, m + n + k)
+    y = ops.linear_e4m3(ops.QuantizedRows.of(x.to(E4M3), sx), ops.e4m3_weight(w.to(E4M3), sw), None, F32)
+    assert torch.equal(y.double(), (x.double() @ w.double().t()) * sx.double()[:, None] * sw.double()[None, :])
+    half = n // 2
+    relu = ops.gated_linear_e4m3(ops.QuantizedRows.of(x.to(E4M3), sx), ops.e4m3_weight(w.to(E4M3), sw), None, 3)
+    want = (torch.relu(y[:, :half].double()) * y[:, half:].double()).float().to(BF16)
+    assert torch.equal(relu, want)
