@@ -27,15 +27,6 @@ __device__ __forceinline__ bool warp_wait(void* bar, uint32_t parity, volatile i
   return __all_sync(0xffffffffu, wait_or_abort(bar, parity, failed));
 }
 
-__device__ __forceinline__ float activate(float g, int act) {
-  switch (act) {
-    case 0: return g / (1.f + expf(-g));
-    case 1: return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
-    case 2: return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g)));
-    default: return fmaxf(g, 0.f);
-  }
-}
-
 struct Epilogue {
   void* out;                  // [M, outputs] bfloat16 or float32 (GLU: bfloat16)
   Bias bias;
@@ -279,9 +270,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 // boxes of w are asked for before griddepcontrol.wait: weights do not depend on the kernel before.
 //   warp 0 the copies of w, warp 10 those of x (one thread for both: 4,096 x 14,336 by 8 rows 14.5 us, 6,144 x 4,096 by 64 10.2; so
 //   13.3 and 9.0), warp 1 the instructions, warps 2-9 the epilogue, under the next tile's steps up to 128 tokens
-__host__ __device__ inline int first_step(int b, int blocks, int steps) { return (int)((long)b * steps / blocks); }
-__device__ __forceinline__ int block_of_step(int step, int blocks, int steps) { return (int)((((long)step + 1) * blocks - 1) / steps); }
-
 __global__ void __launch_bounds__(ROWS_THREADS, 2) e4m3_rows_kernel(const __grid_constant__ CUtensorMap map_x,
                                                                const __grid_constant__ CUtensorMap map_w, Epilogue ep, int M,
                                                                int tiles, int k_steps, int* __restrict__ error_flag) {
@@ -510,16 +498,6 @@ int make_byte_map(CUtensorMap* map, const void* base, long rows, long pitch, int
   return 0;
 }
 
-int multiprocessors() {
-  static int sms = 0;
-  if (sms == 0) {
-    int device = 0;
-    cudaGetDevice(&device);
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) sms = 148;
-  }
-  return sms;
-}
-
 // The width of a pair's tile: the one whose tiles cost least in whole rounds of the pairs, a tile costing what its copies or its
 // instructions take, whichever is more.
 int choose_tile_n(int tiles_m, int cols, bool glu, int pairs) {
@@ -566,17 +544,6 @@ constexpr int ROWS_MOST = 256;  // rows of x that the second kernel takes
 // A block that holds all of the tensor memory takes so much shared memory that no block that wants some fits beside it: one that
 // waits for it could be what this one waits for (the partner of a pair, the kernel before).
 constexpr size_t PAIR_RING = 200 * 1024, EXTRA = 1024 /* alignment */ + 512 /* barriers */;
-
-// Asks for a kernel's shared memory once on every device.
-template <typename Kernel> int allow_smem(const char* what, Kernel kernel, int bytes, uint64_t* done) {
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess && device < 64 && (*done >> device & 1)) return 0;
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return fms_fail("%s: %d bytes of shared memory refused: %s", what, bytes, cudaGetErrorString(e));
-  if (device < 64) *done |= 1ull << device;
-  return 0;
-}
 
 int launch(const void* x, const void* w, Epilogue ep, int M, int N, long pitch, long scratch_floats, int* error_flag, cudaStream_t stream) {
   if (pitch <= 0 || pitch % 16 || pitch > 0x7fffff00L) return fms_fail("gemm_e4m3: rows of %ld bytes, a multiple of 16 is wanted", pitch);

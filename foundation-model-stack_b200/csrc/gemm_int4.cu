@@ -25,15 +25,6 @@ namespace {
 
 constexpr int BLOCK_ROWS = 16, BLOCK_K = 128, WEIGHT_BYTES = 1024;
 
-__device__ __forceinline__ float activate(float g, int act) {
-  switch (act) {
-    case 0: return g / (1.f + expf(-g));
-    case 1: return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
-    case 2: return 0.5f * g * (1.f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g)));
-    default: return fmaxf(g, 0.f);
-  }
-}
-
 // the 8 values of a word as four pairs of bfloat16 q - z
 __device__ __forceinline__ void unpack8(uint32_t word, __nv_bfloat162 zero, uint32_t* pairs) {
 #pragma unroll
@@ -63,30 +54,6 @@ struct Int4Args {
   __host__ __device__ int block_bytes() const { return WEIGHT_BYTES + 64 * per; }
   __host__ __device__ int row_blocks() const { return (N + BLOCK_ROWS - 1) / BLOCK_ROWS; }
 };
-
-// Asks for a kernel's shared memory once on every device.
-template <typename Kernel> int allow_smem(Kernel kernel, int bytes, uint64_t* done) {
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e == cudaSuccess && device < 64 && (*done >> device & 1)) return 0;
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return fms_fail("gemm_int4: %d bytes of shared memory refused: %s", bytes, cudaGetErrorString(e));
-  if (device < 64) *done |= 1ull << device;
-  return 0;
-}
-int multiprocessors() {
-  static int sms = 0;
-  if (sms == 0) {
-    int device = 0;
-    cudaGetDevice(&device);
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) sms = 148;
-  }
-  return sms;
-}
-
-// The run of steps of block b of `blocks`: [first_step(b), first_step(b + 1)); and the block of a step
-__host__ __device__ inline int first_step(int b, int blocks, int steps) { return (int)((long)b * steps / blocks); }
-__device__ __forceinline__ int block_of_step(int step, int blocks, int steps) { return (int)((((long)step + 1) * blocks - 1) / steps); }
 
 // ---- up to 8 rows -------------------------------------------------------------------------------------------------------
 // Bound by reading the weights once, and by the instructions that unpack them.  A thread block, one or two a multiprocessor,
@@ -639,7 +606,7 @@ int launch_rows(const Int4Args& p, float* scratch, long scratch_floats, int* err
   CUtensorMap map_x, map_w;
   if (make_map(&map_x, p.x, p.M, p.K, a.n_tokens) || make_block_map(&map_w, p)) return 1;
   static uint64_t allowed = 0;
-  if (allow_smem(int4_rows_kernel, (int)SMEM_MOST, &allowed)) return 1;
+  if (allow_smem("gemm_int4", int4_rows_kernel, (int)SMEM_MOST, &allowed)) return 1;
   const size_t smem = (size_t)a.stages * stage_bytes + EXTRA;
   fms_launch(int4_rows_kernel, dim3(blocks), dim3(ROWS_THREADS), smem < SMEM_LEAST ? SMEM_LEAST : smem, stream, map_x, map_w, a, error_flag);
   if (fms_launch_status("gemm_int4")) return 1;
@@ -832,7 +799,7 @@ int launch_pair(const Int4Args& p, int* error_flag, cudaStream_t stream) {
   CUtensorMap map_x, map_w;
   if (make_map(&map_x, p.x, p.M, p.K, a.n_tokens / 2) || make_block_map(&map_w, p)) return 1;
   static uint64_t allowed = 0;
-  if (allow_smem(int4_pair_kernel, (int)SMEM_MOST, &allowed)) return 1;
+  if (allow_smem("gemm_int4", int4_pair_kernel, (int)SMEM_MOST, &allowed)) return 1;
   const size_t smem = (size_t)a.stages * stage_bytes + EXTRA;
   // a plain launch: the pairs, which want all of the tensor memory, run beside no block of another kernel of the stream
   int4_pair_kernel<<<dim3(2 * (int)(tiles < pairs ? tiles : pairs)), dim3(PAIR_THREADS), smem < SMEM_LEAST ? SMEM_LEAST : smem, stream>>>(

@@ -383,7 +383,7 @@ template <typename T> int quantize(const void* x, uint8_t* q, float* scales, int
   int threads;
   const bool neighbours = dim % 8 == 0 && aligned16(x);
   const int kept = kept_for(pitch / 8 + !neighbours, n_rows, 4, 8, &threads);  // a run more for rows that begin anywhere
-  (kept == 1 ? launch_rows<T, 1> : kept == 2 ? launch_rows<T, 2> : kept == 4 ? launch_rows<T, 4> : kept == 8 ? launch_rows<T, 8> : launch_rows<T, 0>)(
+  (kept == 1 ? launch_rows<T, 1> : kept == 4 ? launch_rows<T, 4> : kept == 8 ? launch_rows<T, 8> : launch_rows<T, 0>)(
       threads, neighbours, x, q, scales, n_rows, dim, pitch, stream);
   return fms_launch_status("quantize_rows");
 }
