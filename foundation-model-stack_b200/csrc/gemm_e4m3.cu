@@ -588,6 +588,12 @@ int launch(const void* x, const void* w, Epilogue ep, int M, int N, long pitch, 
 }
 }  // namespace
 
+// Columns of the accumulator of a tile where pairs of thread blocks take M rows; 0: the other kernel does.
+FMS_API int fms_e4m3_tile(int M, int N, int glu) {
+  if (M <= ROWS_MOST || N <= 0) return 0;
+  return choose_tile_n((M + 2 * TILE - 1) / (2 * TILE), glu ? N / 2 : N, glu != 0, max(multiprocessors() / 2, 1));
+}
+
 // Floats of scratch memory that the products of M rows with weights of N rows (glu 1: of N / 2 gate and N / 2 up rows) want.
 FMS_API long fms_e4m3_scratch(long M, long N, long pitch, long glu) {
   if (M <= 0 || N <= 0 || pitch <= 0 || M > ROWS_MOST) return 0;

@@ -693,3 +693,17 @@ def test_linear_e4m3_at_the_fewest_steps_that_are_cut(ops, m, n, k):
     relu = ops.gated_linear_e4m3(ops.QuantizedRows.of(x.to(E4M3), sx), ops.e4m3_weight(w.to(E4M3), sw), None, 3)
     want = (torch.relu(y[:, :half].double()) * y[:, half:].double()).float().to(BF16)
     assert torch.equal(relu, want)
+
+
+# with the accumulator's columns of a pair's tile on 148 multiprocessors
+E4M3_TILES = [(257, 264, 64), (257, 2376, 80), (257, 3056, 96), (257, 3600, 112), (257, 4280, 128), (257, 4824, 144), (257, 5368, 160), (257, 6048, 176),
+              (517, 4280, 192), (517, 4688, 208), (517, 5096, 224), (517, 5504, 240), (517, 5776, 256)]
+
+
+@pytest.mark.parametrize("m,n,tile", E4M3_TILES)
+def test_linear_e4m3_of_tiles_of_every_width(ops, m, n, tile):
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert load_library("gemm_e4m3").fms_e4m3_tile(m, n, 0) == tile
+    x, w, sx, sw, _ = e4m3_case(m, n, 272, m + n)
+    y = ops.linear_e4m3(ops.QuantizedRows.of(x.to(E4M3), sx), ops.e4m3_weight(w.to(E4M3), sw), None, F32)
+    assert torch.equal(y.double(), (x.double() @ w.double().t()) * sx.double()[:, None] * sw.double()[None, :])
