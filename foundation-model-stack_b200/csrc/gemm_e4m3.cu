@@ -265,11 +265,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 // tiles (cut_of): every multiprocessor takes an equal run of the steps of all tiles; where a tile's steps fall to several blocks,
 // each leaves its sums in a slot of its own in scratch memory, and a second kernel adds them in the order of k; under GLU all
 // tiles of such a cut go that way, since a gate and its up value lie in different lanes.  (Clusters that shared a tile and added
-// their sums through distributed shared memory: 6,144 x 4,096 by 64 rows 11.8 us, 4,096 x 14,336 17.7 us; so 9.0 and 14.4.)  The
+// their sums through distributed shared memory: 6,144 x 4,096 by 64 rows 11.8 us, 4,096 x 14,336 17.7 us; so 9.5 and 14.1.)  The
 // cut depends on the weights' shape alone, so a row's result does not depend on the rest of the batch.  The first stages'
 // boxes of w are asked for before griddepcontrol.wait: weights do not depend on the kernel before.
 //   warp 0 the copies of w, warp 10 those of x (one thread for both: 4,096 x 14,336 by 8 rows 14.5 us, 6,144 x 4,096 by 64 10.2; so
-//   13.3 and 9.0), warp 1 the instructions, warps 2-9 the epilogue, under the next tile's steps up to 128 tokens
+//   12.8 and 9.5), warp 1 the instructions, warps 2-9 the epilogue, under the next tile's steps up to 128 tokens
 __global__ void __launch_bounds__(ROWS_THREADS, 2) e4m3_rows_kernel(const __grid_constant__ CUtensorMap map_x,
                                                                const __grid_constant__ CUtensorMap map_w, Epilogue ep, int M,
                                                                int tiles, int k_steps, int* __restrict__ error_flag) {
@@ -498,8 +498,10 @@ int make_byte_map(CUtensorMap* map, const void* base, long rows, long pitch, int
   return 0;
 }
 
-// The width of a pair's tile: the one whose tiles cost least in whole rounds of the pairs, a tile costing what its copies or its
-// instructions take, whichever is more.
+// The width of a pair's tile: the one whose tiles cost least in whole rounds of the pairs.  A tile costs, in one round (2,304 rows, 8 tiles
+// a row, k 8,192), 29.8 us at 256 columns, 28.5 at 240, 27.4 at 224, 25.3 at 208, 24.2 at 192, 23.2 at 176, 22.0 at 160, 21.2 at 128 and
+// 19.4 at 64: of the widest tile 0.96, 0.92, 0.85, 0.81, 0.78, 0.74, 0.71 and 0.65.  The line below is within 6% of that.  Widths by 16
+// are a pair's shapes where both operands come from shared memory; GLU: by 32, so that a half is a multiple of 16.
 int choose_tile_n(int tiles_m, int cols, bool glu, int pairs) {
   const int step = glu ? 32 : 16;
   long best_cost = -1;
@@ -519,8 +521,10 @@ int choose_tile_n(int tiles_m, int cols, bool glu, int pairs) {
 // How the second kernel cuts a product; slots 0: a block takes one whole tile, and there is nothing to join.  Equal runs cost the
 // second launch and a trip through scratch memory, about what 16 steps of a block cost, and more the more tiles there are.  By
 // 64 rows, equal runs against whole tiles, us: 4,096 x 4,096 8.1 : 11.4, 6,144 x 4,096 10.0 : 11.5, 8,192 x 4,096 11.0 : 11.7,
-// 6,144 x 2,560 8.3 : 8.3, 8,192 x 2,048 8.4 : 7.5, 12,288 x 4,096 14.1 : 12.6, 12,288 x 12,288 31.6 : 30.0,
-// 28,672 x 4,096 28.7 : 21.7.  A run is 4 steps or more: the sums of 32 blocks of one step each take longer to join than to make.
+// 6,144 x 2,560 8.3 : 8.3, 8,192 x 2,048 8.4 : 7.5, 12,288 x 4,096 14.1 : 12.6, 28,672 x 4,096 28.7 : 21.7.  That is what the line was
+// drawn by; since whole tiles take no more tensor memory than their sums they are ahead on a part of this side of it too: 7.8 : 8.5,
+// 9.5 : 9.1, 10.3 : 9.7, 7.8 : 6.5, 8.1 : 6.4, 14.1 : 11.6, and 12,288 x 12,288 30.8 : 27.6.
+// A run is 4 steps or more: the sums of 32 blocks of one step each take longer to join than to make.
 struct Cut {
   int tiles, k_steps, blocks, slots;
 };
@@ -582,7 +586,8 @@ int launch(const void* x, const void* w, Epilogue ep, int M, int N, long pitch, 
   if (tiles > 0x7fffffffL) return fms_fail("gemm_e4m3: %ld tiles", tiles);
   const int busy = (int)(tiles < pairs ? tiles : pairs);
   // A plain launch: the pairs, which want all of the tensor memory, run beside no block of another kernel of the stream.  (Launched
-  // while the kernel before was still draining, a pair of blocks in a prompt of 8,192 tokens began and never got its tensor memory.)
+  // while the kernel before was still draining, and asking for its tensor memory ahead of the cluster's barrier, a pair of blocks in a
+  // prompt of 8,192 tokens began and never got it.)
   e4m3_pair_kernel<<<dim3(2 * busy), dim3(THREADS), PAIR_RING + EXTRA, stream>>>(map_x, map_w, ep, M, k_steps, error_flag);
   return fms_launch_status("gemm_e4m3");
 }

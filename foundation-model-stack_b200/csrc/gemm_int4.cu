@@ -13,7 +13,8 @@
 // 0x4300 | q is the bfloat16 128 + q; minus 128 + z it is q - z, exact.
 //   few rows: mma.sync over q - z, whole numbers, a group's float32 sum times its scale: nothing is rounded but the result.
 //   more rows: tcgen05 over (q - z) * s rounded to bfloat16 on its way into the operand, as a bfloat16 weight would be: the
-//             tensor cores' sums run over all of k and cannot be scaled group by group.
+//             tensor cores' sums run over all of k and cannot be scaled group by group.  What that costs, in the root mean square
+//             against 64 bits: 0.0021 to 0.0022 of y, where the result's own rounding to bfloat16 leaves 0.0017.
 #include <cuda.h>
 
 #include "common.cuh"
@@ -61,8 +62,8 @@ struct Int4Args {
 // has warps; each warp takes an equal run of their 128-k blocks, whatever tiles these belong to, two at most, and leaves a sum of
 // each in shared memory; after the one barrier those of a tile are added in the order of k.  A lane loads its pieces of two rows
 // of a block straight into registers, AHEAD blocks ahead, as many as 64 registers hold (28,672 x 4,096 by one row with groups of
-// 128, 1 / 2 / 3 ahead 14.8 / 14.2 / 16.6 us; of 64, 1 / 2 ahead 15.2 / 17.1); x comes from the first-level cache.
-// 28,672 x 4,096 by one row 14.2 us, by eight 15.6, gated 16.0 (tiles shared by the warps of a block one after the other, with a
+// 128, 1 / 2 / 3 ahead 14.6 / 14.2 / 16.6 us; of 64 17.0 / 17.1 / 19.7; of 32 18.0 / 20.0 / 24.7); x comes from the first-level cache.
+// 28,672 x 4,096 by one row 14.2 us, by eight 15.7, gated 16.1 (tiles shared by the warps of a block one after the other, with a
 // barrier each: 17.0, gated 23.5; rings in shared memory fed by bulk copies 22.7; without unpacking 12.6, without that and
 // the loads of x 11.2; with half the shifts as wide products 18.0; 16 warps 4 blocks ahead 17.6).
 constexpr int FEW_ROWS = 8, FEW_WARPS = 32;
@@ -346,7 +347,7 @@ template <int N> __device__ __forceinline__ void store_column(const Int4Args& p,
 //               threads more than the tensor cores (some 700 cycles against 260 at 64 tokens), so up to 64 tokens warp 23 takes every
 //               second step, into accumulators of its own that the epilogue adds, and a step's copies are waited for by those who unpack
 //               it alone: an issuer sees them by way of the operand's barrier.  (One issuer, one thread for all copies: 4,096 x 14,336
-//               by 16 rows 13.6 us, by 64 16.8, 28,672 x 4,096 22.7 and 26.5; so 11.6, 15.6, 19.6, 24.0.  Two issuers for
+//               by 16 rows 13.6 us, by 64 16.8, 28,672 x 4,096 22.7 and 26.5; so 11.9, 15.8, 19.8, 24.4.  Two issuers for
 //               128 tokens leave room for 4 stages of the operand and 4 of copies: 100 rows 18.7 -> 21.9 us.)
 //   warps 2-17  up to four groups of four unpack every fourth step each, a thread a row of w, into the next of up to 7 stages of the
 //               operand, 64 columns each
@@ -572,8 +573,8 @@ __global__ void __launch_bounds__(TILE) int4_join_kernel(RowsArgs a, int blocks)
 constexpr size_t SMEM_LEAST = 200 * 1024, SMEM_MOST = 225 * 1024, EXTRA = 1024 /* alignment */ + 512 /* barriers */;
 
 // The most rows of x that this kernel takes: 256, but 112 where the pairs of the kernel below have a tile each.  This one / that one in
-// us, by rows: 28,672 x 4,096 96 31.4 / 32.3, 128 38.7 / 32.4, 256 72.2 / 60.6; 6,144 x 4,096 128 13.5 / 16.3, 256 20.5 / 17.3; 4,096 x
-// 14,336 128 20.4 / 42.9, 256 30.9 / 44.7.
+// us, by rows: 28,672 x 4,096 96 31.9 / 32.3, 112 34.5 / 34.3, 128 39.0 / 34.4, 256 70.6 / 57.2; 6,144 x 4,096 128 14.1 / 18.6, 256 21.0 / 19.0;
+// 4,096 x 14,336 128 20.7 / 44.9, 256 31.1 / 45.6.
 int rows_most(int N) { return (long)N >= 2L * TILE * (multiprocessors() / 2) ? 112 : 256; }
 int rows_blocks(int N, int K) {
   const long steps = (long)((N + TILE - 1) / TILE) * ((K + BLOCK_K - 1) / BLOCK_K);
@@ -622,7 +623,7 @@ int launch_rows(const Int4Args& p, float* scratch, long scratch_floats, int* err
 // block unpacks its own 128 rows of w into its own tensor memory and brings half of the tokens, so a multiprocessor takes in
 // 128 rows of x and 128 half-bytes a k for 2 * 128 * 256 operations.  The accumulator takes half of the 512 columns and four stages
 // of the operand the other half: a stage goes round in some 2,400 cycles (barriers, unpacking, the instructions), so that two of
-// them, which left room for two accumulators of 192 columns, kept the tensor cores waiting (2,048 x 28,672 x 4,096 454 us).
+// them, which left room for two accumulators of 192 columns, kept the tensor cores waiting (2,048 x 28,672 x 4,096 454 us; so 412).
 // The next tile's first four steps are unpacked under the epilogue.
 //   warp 0      per step of 128 k: two 64-k boxes of x, counted on block 0's barrier, and one of eight blocks of w, counted on its own
 //   warp 1      (of block 0) issues 8 instructions (256 x tokens x 16) a step

@@ -14,7 +14,7 @@
 // so that nothing is read twice.  A thread owns runs of 8 neighbours, 16-byte loads and 8-byte stores.  Rows of a width that is no
 // multiple of 8 begin anywhere: their runs are moved forward by up to 3 values to where the rows' own loads are aligned, and a
 // warp's lanes hand one another the bytes that make aligned stores (1,100 x 5,001 bfloat16 7.7 us, and behind the norm, float32,
-// 21.7; 11.4 and 25.1 with single loads and stores).  Rows of q are `pitch` bytes apart, dim rounded up to 16 with zeros behind the last value, as the products'
+// 21.1; 11.4 and 25.1 with single loads and stores).  Rows of q are `pitch` bytes apart, dim rounded up to 16 with zeros behind the last value, as the products'
 // copies want them.
 //
 // q is what the exact quotient rounds to.  Of bfloat16 rows it is often a tie, and otherwise, a ratio of numbers of 11 and 8 bits,
@@ -356,7 +356,8 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2
       fetch(j, writes);
       if (shrunk) shrink(xs);
     }
-    store_run<NEIGHBOURS>(q + (size_t)blockIdx.x * pitch, quotients<NEIGHBOURS, true>(xs, gs, inv, exact, place(j, shift), dim), j, shift, pitch, (long)(gridDim.x - blockIdx.x) * pitch);
+    store_run<NEIGHBOURS>(q + (size_t)blockIdx.x * pitch, quotients<NEIGHBOURS, true>(xs, gs, inv, exact, place(j, shift), dim), j, shift, pitch,
+                          (long)(gridDim.x - blockIdx.x) * pitch);
   }
   if (threadIdx.x == 0) scales[blockIdx.x] = none ? 0.f : s;
 }
@@ -364,7 +365,8 @@ __global__ void __launch_bounds__(RUNS == 1 ? 1024 : 512, RUNS == 0 || RUNS == 2
 // The runs of 8 that a thread keeps (0: the row is too wide for registers) and the threads for a row of `runs` of them.  Few
 // rows: a thread a run as far as 1,024 go, since only latency counts.  Many: `many` runs a thread, so that more bytes a thread and
 // more rows a multiprocessor are on their way (8,192 x 4,096 bfloat16 to e4m3 with 1 / 2 / 4 / 8 runs: 27.5 / 22.8 / 16.9 / 19.8 us;
-// behind the norm, whose runs take 12 registers and more, 2,048 x 4,096 with 1 / 2 / 4: 22.4 / 17.3 / 18.4 us).
+// behind the norm, whose runs take 12 registers and more, 2,048 x 4,096 with 1 / 2 / 4: 22.4 / 17.3 / 18.4 us; since the gain waits for
+// the kernel in front and rows that overflow are summed again, 17.6).
 int kept_for(int runs, int n_rows, int many, int most_kept, int* threads) {
   int kept = n_rows <= 296 ? (runs <= 1024 ? 1 : 4) : (runs <= 128 ? 1 : many);
   if (runs > 512 * kept && kept > 1) kept = runs <= 512 * 4 ? 4 : (runs <= 512 * most_kept ? most_kept : 0);
